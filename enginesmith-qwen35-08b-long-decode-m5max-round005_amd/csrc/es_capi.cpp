@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstring>
+#include <initializer_list>
 #include <string>
 
 #include "es_checkpoint.hpp"
@@ -34,6 +35,33 @@ bool to_q4(const es_q4* in, es::Q4* out) {
   if (!in) return false;
   *out = es::Q4{in->codes, in->scales, in->biases, in->n, in->k};
   return in->codes && in->scales && in->biases && in->n > 0 && in->k > 0;
+}
+
+// The cache of an 8-bit operator and the positions it touches; "" when they hold.
+const char* kv8_fault(const es_kv8* c, int position, int rows) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return "null cache";
+  if (c->heads < 1 || c->heads > 256 || c->capacity < 1 || c->capacity > (1 << 22))
+    return "cache heads 1 .. 256 and capacity 1 .. 2^22 required";
+  if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return "cache codes must be 16-byte aligned";
+  if (rows < 1 || position < 0 || (int64_t)position + rows > c->capacity)
+    return "rows >= 1 and 0 <= position, position + rows <= capacity required";
+  return "";
+}
+es::Kv8 to_kv8(const es_kv8* c) {
+  return es::Kv8{c->k, c->v, c->k_scale, c->v_scale, c->heads, (c->capacity + es::kKv8Block - 1) / es::kKv8Block};
+}
+bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p & 15) return false;
+  return true;
+}
+// Strides of bf16 rows, in elements; up to 2^40 no product with a row or head number passes 64 bits.
+bool kv8_strides_fit(int64_t row, int64_t head) {
+  const int64_t most = int64_t(1) << 40;
+  return row >= 0 && head >= 0 && row <= most && head <= most && row % 8 == 0 && head % 8 == 0;
+}
+bool kv8_heads_fit(int q_heads, int kv_heads, int rows) {
+  return q_heads >= 1 && kv_heads >= 1 && q_heads % kv_heads == 0 && rows >= 1 && (int64_t)rows * q_heads <= (1 << 22);
 }
 
 hipStream_t S(void* s) { return static_cast<hipStream_t>(s); }
@@ -415,6 +443,82 @@ int es_attn_decode(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_
   a.pos_val = position;
   if (int rc = hip_status(es::launch_attn_fused(a, S(stream)), "es_attn_decode chains")) return rc;
   return hip_status(es::launch_attn_merge(a, S(stream)), "es_attn_decode merge");
+}
+
+// ---- key/value cache in 8 bits ----
+int es_kv8_write(const es_kv8* cache, const uint16_t* k, const uint16_t* v, int64_t row_stride,
+                 int64_t head_stride, int position, int rows, void* stream) {
+  const char* fault = kv8_fault(cache, position, rows);
+  if (*fault) return fail(ES_ERR_INVALID, std::string("es_kv8_write: ") + fault);
+  if (!k || !v) return fail(ES_ERR_INVALID, "es_kv8_write: null argument");
+  if (!aligned16({k, v}) || !kv8_strides_fit(row_stride, head_stride))
+    return fail(ES_ERR_INVALID, "es_kv8_write: k and v 16-byte aligned, strides multiples of 8 in 0 .. 2^40 required");
+  const es::Kv8Rows r{k, v, row_stride, head_stride, position, rows};
+  return hip_status(es::launch_kv8_write(to_kv8(cache), r, S(stream)), "es_kv8_write");
+}
+
+int es_kv8_read(const es_kv8* cache, int position, int rows, uint16_t* k, uint16_t* v, int64_t row_stride,
+                int64_t head_stride, void* stream) {
+  const char* fault = kv8_fault(cache, position, rows);
+  if (*fault) return fail(ES_ERR_INVALID, std::string("es_kv8_read: ") + fault);
+  if (!k || !v || k == v) return fail(ES_ERR_INVALID, "es_kv8_read: null argument or k == v");
+  if (!aligned16({k, v}) || !kv8_strides_fit(row_stride, head_stride))
+    return fail(ES_ERR_INVALID, "es_kv8_read: k and v 16-byte aligned, strides multiples of 8 in 0 .. 2^40 required");
+  // the inner of the two strides clears a row, the outer all rows of the inner; no stride matters where it is not taken
+  const int64_t n = rows, h = cache->heads, wide = es::kHeadDim;
+  const bool rows_apart = n == 1 || row_stride >= wide, heads_apart = h == 1 || head_stride >= wide;
+  const bool token_major = heads_apart && (n == 1 || row_stride >= (h - 1) * head_stride + wide);
+  const bool head_major = rows_apart && (h == 1 || head_stride >= (n - 1) * row_stride + wide);
+  if (!(token_major || head_major))
+    return fail(ES_ERR_INVALID, "es_kv8_read: rows overlap");
+  return hip_status(es::launch_kv8_read(to_kv8(cache), position, rows, k, v, row_stride, head_stride, S(stream)),
+                    "es_kv8_read");
+}
+
+int es_attn_prepare_rows_kv8(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t* v_proj,
+                             const uint16_t* q_gain, const uint16_t* k_gain, const float* inv_freq,
+                             int position, int rows, int q_heads, uint16_t* query, const es_kv8* cache,
+                             void* stream) {
+  const char* fault = kv8_fault(cache, position, rows);
+  if (*fault) return fail(ES_ERR_INVALID, std::string("es_attn_prepare_rows_kv8: ") + fault);
+  if (!q_proj || !k_proj || !v_proj || !q_gain || !k_gain || !inv_freq || !query)
+    return fail(ES_ERR_INVALID, "es_attn_prepare_rows_kv8: null argument");
+  if (!kv8_heads_fit(q_heads, cache->heads, rows))
+    return fail(ES_ERR_INVALID, "es_attn_prepare_rows_kv8: q_heads a multiple of the cache's heads and rows * q_heads <= 2^22 required");
+  if (!aligned16({q_proj, k_proj, v_proj, q_gain, k_gain, inv_freq, query}))
+    return fail(ES_ERR_INVALID, "es_attn_prepare_rows_kv8: pointers must be 16-byte aligned");
+  const es::Kv8Rows r{k_proj, v_proj, (int64_t)cache->heads * es::kHeadDim, es::kHeadDim, position, rows};
+  const es::Kv8Prep p{q_proj, q_gain, k_gain, inv_freq, q_heads, query};
+  return hip_status(es::launch_kv8_prepare(to_kv8(cache), r, p, S(stream)), "es_attn_prepare_rows_kv8");
+}
+
+size_t es_attn_kv8_scratch_bytes(int q_heads, int kv_heads, int rows) {
+  if (kv_heads > 256 || !kv8_heads_fit(q_heads, kv_heads, rows)) return 0;
+  return es::kv8_attn_scratch_bytes(q_heads, kv_heads, rows);
+}
+
+int es_attn_kv8(const uint16_t* query, int q_heads, const es_kv8* cache, int position, int rows,
+                const uint16_t* gate, void* scratch, size_t scratch_bytes, uint16_t* out, void* stream) {
+  const char* fault = kv8_fault(cache, position, rows);
+  if (*fault) return fail(ES_ERR_INVALID, std::string("es_attn_kv8: ") + fault);
+  if (!query || !out) return fail(ES_ERR_INVALID, "es_attn_kv8: null argument");
+  if (!kv8_heads_fit(q_heads, cache->heads, rows))
+    return fail(ES_ERR_INVALID, "es_attn_kv8: q_heads a multiple of the cache's heads and rows * q_heads <= 2^22 required");
+  if (!aligned16({query, gate, scratch, out})) return fail(ES_ERR_INVALID, "es_attn_kv8: pointers must be 16-byte aligned");
+  if (out == query || out == gate) return fail(ES_ERR_INVALID, "es_attn_kv8: out must not alias query or gate");
+  const size_t need = es::kv8_attn_scratch_bytes(q_heads, cache->heads, rows);
+  if (need && (!scratch || scratch_bytes < need))
+    return fail(ES_ERR_INVALID, "es_attn_kv8: scratch smaller than es_attn_kv8_scratch_bytes(q_heads, heads, rows)");
+  es::Kv8Attn a{};
+  a.query = query;
+  a.gate = gate;
+  a.out = out;
+  a.part = static_cast<float*>(scratch);
+  a.q_heads = q_heads;
+  a.group = q_heads / cache->heads;
+  a.position = position;
+  a.rows = rows;
+  return hip_status(es::launch_kv8_attn(to_kv8(cache), a, S(stream)), "es_attn_kv8");
 }
 
 // ---- head ----

@@ -100,10 +100,9 @@ __device__ __forceinline__ float es_log(float x) {
   return fmaf(ef, 0.693145751953125f, fmaf(ef, 1.42860682030941723212e-6f, lm));
 }
 
-// sin and cos of an fp32 angle: quadrant reduction in double precision, then
+// sin and cos of an angle: quadrant reduction in double precision, then
 // Taylor polynomials on |r| <= pi/4.
-__device__ __forceinline__ void es_sincos(float x, float* sn, float* cs) {
-  const double xd = (double)x;
+__device__ __forceinline__ void es_sincos_angle(double xd, float* sn, float* cs) {
   const double kd = rint(xd * 0.63661977236758134308);
   double rd = fma(-kd, 1.5707963267948966192, xd);
   rd = fma(-kd, 6.123233995736766036e-17, rd);
@@ -124,6 +123,7 @@ __device__ __forceinline__ void es_sincos(float x, float* sn, float* cs) {
   *sn = q == 0 ? sr : q == 1 ? cr : q == 2 ? -sr : -cr;
   *cs = q == 0 ? cr : q == 1 ? -sr : q == 2 ? -cr : sr;
 }
+__device__ __forceinline__ void es_sincos(float x, float* sn, float* cs) { es_sincos_angle((double)x, sn, cs); }
 
 // MLX unary sigmoid in bf16: round after exp, add, reciprocal, subtraction
 // (linear.metal:389-395, gdn.metal:10-15). The reciprocal is the hardware's

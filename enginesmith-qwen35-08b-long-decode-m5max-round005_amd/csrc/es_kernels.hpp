@@ -334,4 +334,39 @@ hipError_t launch_read(const void* src, size_t bytes, void* out, hipStream_t s);
 hipError_t launch_fill_normal_f32(float* dst, size_t n, float sigma, uint64_t seed,
                                   hipStream_t s);
 
+// ---- key/value cache in 8 bits, k_kv8.hip ----
+// Callers check shapes, alignment and bounds; the launchers do not.
+constexpr int kKv8Block = 64;         // tokens of a block
+constexpr int kKv8PartFloats = 260;   // a range's 256 sums, maximum and sum of exponentials, to a multiple of 16 bytes
+struct Kv8 {
+  uint8_t *k, *v, *k_scale, *v_scale;  // [heads, blocks, 16384] codes, [heads, blocks] exponents + 127
+  int heads, blocks;
+};
+// Rows of K and V (or of their projections) for positions position .. position + rows - 1.
+struct Kv8Rows {
+  const uint16_t *k, *v;
+  int64_t row_stride, head_stride;  // in elements
+  int position, rows;
+};
+struct Kv8Prep {
+  const uint16_t *q_proj, *q_gain, *k_gain;
+  const float* inv_freq;
+  int q_heads;
+  uint16_t* query;
+};
+struct Kv8Attn {
+  const uint16_t* query;
+  const uint16_t* gate;  // q_proj rows, or null
+  uint16_t* out;
+  float* part;           // kv8_attn_scratch_bytes
+  int q_heads, group, position, rows;
+  int tiles, splits;     // set by the launcher
+};
+size_t kv8_attn_scratch_bytes(int q_heads, int kv_heads, int rows);
+hipError_t launch_kv8_write(const Kv8& c, const Kv8Rows& r, hipStream_t s);
+hipError_t launch_kv8_prepare(const Kv8& c, const Kv8Rows& r, const Kv8Prep& p, hipStream_t s);
+hipError_t launch_kv8_read(const Kv8& c, int position, int rows, uint16_t* k, uint16_t* v, int64_t row_stride,
+                           int64_t head_stride, hipStream_t s);
+hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s);
+
 }  // namespace es

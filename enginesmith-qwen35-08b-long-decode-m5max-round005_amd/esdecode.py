@@ -9,7 +9,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import (POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64,
+                    c_void_p)
 
 import numpy as np
 
@@ -31,6 +32,11 @@ class EsError(RuntimeError):
 
 class Q4(ctypes.Structure):
     _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("biases", c_void_p), ("n", c_int32), ("k", c_int32)]
+
+
+class KV8(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("heads", c_int32),
+                ("capacity", c_int32)]
 
 
 _lib = None
@@ -95,6 +101,12 @@ _SIGNATURES = {
     "es_attn_prepare_rows": (c_int, [c_void_p] * 6 + [c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     "es_attn_prefill": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "es_attn_gate_rows": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "es_kv8_write": (c_int, [POINTER(KV8), c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "es_kv8_read": (c_int, [POINTER(KV8), c_int, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "es_attn_prepare_rows_kv8": (c_int, [c_void_p] * 6 + [c_int, c_int, c_int, c_void_p, POINTER(KV8), c_void_p]),
+    "es_attn_kv8_scratch_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "es_attn_kv8": (c_int, [c_void_p, c_int, POINTER(KV8), c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p,
+                            c_void_p]),
     "es_weights_tensor_shape": (c_int, [c_int, c_int, c_int, POINTER(ctypes.c_int64), c_int]),
     "es_checkpoint_config": (c_int, [c_char_p, POINTER(c_int), POINTER(c_int)]),
     "es_checkpoint_load": (c_int, [c_char_p, c_int, c_int, c_void_p, c_size_t]),
@@ -231,6 +243,20 @@ class DeviceQ4:
         self.scales = DeviceBuffer.from_numpy(scales.astype(np.uint16))
         self.biases = DeviceBuffer.from_numpy(biases.astype(np.uint16))
         self.struct = Q4(self.codes.ptr, self.scales.ptr, self.biases.ptr, self.n, self.k)
+
+
+class DeviceKV8:
+    """A key/value cache in 8 bits resident on the device (es_kv8)."""
+
+    BLOCK = 64
+
+    def __init__(self, heads: int, capacity: int):
+        self.heads, self.capacity = int(heads), int(capacity)
+        self.blocks = -(-self.capacity // self.BLOCK)
+        n = self.heads * self.blocks
+        self.k, self.v = DeviceBuffer(n * self.BLOCK * 256), DeviceBuffer(n * self.BLOCK * 256)
+        self.k_scale, self.v_scale = DeviceBuffer(n), DeviceBuffer(n)
+        self.struct = KV8(self.k.ptr, self.v.ptr, self.k_scale.ptr, self.v_scale.ptr, self.heads, self.capacity)
 
 
 # ---------------------------------------------------------------- weights

@@ -298,6 +298,90 @@ int es_attn_decode(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_
                    uint16_t* query_out, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* Key/value cache in 8 bits                                           */
+/* ------------------------------------------------------------------ */
+/* A K/V cache of half the bytes of the bf16 kcache/vcache above, with the
+ * operators that write it, read it and attend over it. No reference
+ * counterpart. Heads of 256 dims, any number of KV heads, any number of query
+ * heads that is a multiple of it (query head h reads KV head h / (q_heads /
+ * heads)).
+ *
+ * Codes are e4m3 (fp8, largest 448) with one power of two for each block of 64
+ * positions of a head, K and V apart: value = code * 2^(scale byte - 127), the
+ * smallest power (2^-127 at least) that brings the block's largest finite
+ * magnitude to at most 448. With blocks = (capacity + 63) / 64: k and v hold
+ * [heads, blocks, 16384] codes (16-byte aligned), k_scale and v_scale [heads,
+ * blocks] bytes, device memory of the caller, which needs no initialisation. In
+ * a block the codes lie in the order of the matrix instructions:
+ *   k [position/32 %2][d/64][d/16 %2][d/32 %2][position %32][d %16]
+ *   v [d/32][position/8 %2][position/4 %2][d %32][position/16 %4][position %4]
+ * heads 1 .. 256, capacity 1 .. 2^22.
+ *
+ * A write at `position` keeps the rows before it and leaves rows from position +
+ * rows on without meaning (their codes keep their bits). The block that holds
+ * `position` keeps its power of two if rows of it stay, raised where the new rows
+ * need it: its earlier codes are then rounded again, exact except where they
+ * become subnormal (below 2^-6 of the power). So rows written one by one get the
+ * same powers as rows written at once. Where no row of that block before
+ * `position` was ever written, its scale bytes must be 255 (a block without rows).
+ *
+ * A position whose K or V row of a head holds a NaN or an infinity is stored as
+ * NaN: it reads back as NaN throughout, and every query that attends to it
+ * in that head gets NaN, no other does. Calls that write the same block must not
+ * overlap, nor a write and a call that reads its block. */
+typedef struct es_kv8 {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int32_t heads;
+  int32_t capacity;
+} es_kv8;
+
+/* Writes K and V rows of positions position .. position+rows-1 from bf16: row r
+ * of head h is 256 elements at r * row_stride + h * head_stride (elements,
+ * multiples of 8 in 0 .. 2^40; k and v 16-byte aligned), so [rows, heads, 256]
+ * projections and [heads, capacity, 256] caches both serve. Rounds to nearest,
+ * ties to even. position + rows <= capacity. */
+int es_kv8_write(const es_kv8* cache, const uint16_t* k, const uint16_t* v, int64_t row_stride,
+                 int64_t head_stride, int position, int rows, void* stream);
+
+/* Reads positions position .. position+rows-1 back to bf16, laid out as for
+ * es_kv8_write (rows that do not overlap; k and v distinct). Every value is
+ * exact, except that values below bf16's normal range round to nearest and one
+ * that the codes rounded up to 2^128 is an infinity. */
+int es_kv8_read(const es_kv8* cache, int position, int rows, uint16_t* k, uint16_t* v, int64_t row_stride,
+                int64_t head_stride, void* stream);
+
+/* es_attn_prepare_rows for this cache: per row, query [rows, q_heads, 256] =
+ * RoPE(RMSNorm(q head) * q_gain) at its position, and the K and V rows written
+ * as es_kv8_write does, K = RoPE(RMSNorm(k head) * k_gain). q_proj [rows,
+ * q_heads, 512] (query|gate), k_proj, v_proj [rows, heads, 256], inv_freq 32
+ * device floats. Computed in fp32 with one rounding at the end (to bf16 the
+ * query, to the codes K), angles in double; eps 1e-6. Pointers 16-byte aligned,
+ * rows * q_heads <= 2^22. */
+int es_attn_prepare_rows_kv8(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t* v_proj,
+                             const uint16_t* q_gain, const uint16_t* k_gain, const float* inv_freq,
+                             int position, int rows, int q_heads, uint16_t* query, const es_kv8* cache,
+                             void* stream);
+
+/* Scratch bytes of es_attn_kv8 for these heads and this number of rows, at any
+ * position and capacity (0 where it needs none, or for bad arguments). */
+size_t es_attn_kv8_scratch_bytes(int q_heads, int kv_heads, int rows);
+
+/* Causal attention of `rows` queries at positions position .. position+rows-1
+ * over this cache, one token or many: row r attends to positions 0 ..
+ * position+r; o = softmax(q.K^T / 16) V in fp32 (queries exact, probabilities
+ * to 8 significant bits, products on 8-bit matrix instructions), out [rows,
+ * q_heads, 256] = bf16(o), or with gate (q_proj rows [rows, q_heads, 512],
+ * optional) bf16(o * sigmoid(gate)), gate the second half of each head. query
+ * [rows, q_heads, 256] bf16. Pointers 16-byte aligned, rows * q_heads <= 2^22.
+ * out must not alias query or gate; scratch must not be used by two
+ * calls at once. */
+int es_attn_kv8(const uint16_t* query, int q_heads, const es_kv8* cache, int position, int rows,
+                const uint16_t* gate, void* scratch, size_t scratch_bytes, uint16_t* out, void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Vocab head (head_lse.metal:11-98 with rms_norm_bf16, model.rs:290-300) */
 /* ------------------------------------------------------------------ */
 /* Scratch for es_head_greedy: per-block (max, sum exp) partials. */
