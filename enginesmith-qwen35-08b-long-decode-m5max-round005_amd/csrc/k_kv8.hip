@@ -24,6 +24,8 @@
 // 8-bit product to about 2^-13 of the largest: measured rms 1e-5 of it).
 #include "es_kernels.hpp"
 
+#include <type_traits>
+
 namespace es {
 namespace {
 
@@ -345,239 +347,399 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8 c, int position, int rows,
 
 // ---- attention ----
 constexpr float kLog2e = 1.44269504088896341f;
-// Scale operands of the matrix instructions (2^(byte - 127), one byte used).
-constexpr int kOne = 127, kLo = 127 - 4, kProb = 127 - 8;
-
-__device__ __forceinline__ float gated(float o, const uint16_t* gate) {
-  return o / (1.0f + __expf(-bf2f(*gate)));
+// Four values (at most 448, of eight significant bits) in two parts: the nearest
+// codes, and the codes of 16 times the rest.
+__device__ __forceinline__ int2 split_e4m3(float a, float b, float c, float d) {
+  const int h = pack_e4m3(a, b, c, d);
+  const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), v = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
+  return make_int2(h, pack_e4m3((a - u[0]) * 16.0f, (b - u[1]) * 16.0f, (c - v[0]) * 16.0f, (d - v[1]) * 16.0f));
+}
+// A float's magnitude as bits that compare as integers, zero for a NaN or infinity.
+__device__ __forceinline__ uint32_t finite_bits(uint32_t x) {
+  x &= 0x7fffffffu;
+  return x < 0x7f800000u ? x : 0;
 }
 
-// Few queries: 16 (row, query head) pairs of one KV head a block, four waves
-// that take every fourth 64-token block of the block's range of keys, operands
-// straight from memory to registers, a softmax state for each wave.
-//   S[token, query] = K Q^T, 16x16x128: lane (n = lane % 16, g = lane / 16) gives
-//   K bytes of token n and Q bytes of query n, receives tokens 4 g .. 4 g + 3
-//   of query n;
-//   O^T[d, query] += V^T P^T: the 128 places along tokens hold the hi parts of
-//   the 64 probabilities and their lo parts, against V twice.
-__global__ __launch_bounds__(256, 1) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
-  __shared__ __attribute__((aligned(16))) float sum[4][16][260];
-  __shared__ float mx[4][16], den[4][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  const int split = (int)blockIdx.x % a.splits, unit = (int)blockIdx.x / a.splits;
-  const int head = unit / a.tiles, tile = unit % a.tiles;
-  const int pairs = a.rows * a.group;
-  const int pair = min(tile * 16 + n, pairs - 1);
-  const int row = pair / a.group, qh = head * a.group + pair % a.group;
-  // queries: bytes d = 128 s + 32 g .. + 31
-  i32x8 qhi[2], qlo[2];
-  float cq;
+// Most that the scores may pass the exponent's reference before it moves (base
+// 2): e^-reference is at most 2^kSlack, and 2^(kSlack + kShift) is below 448.
+constexpr float kSlack = 4.0f, kShift = 4.0f;
+constexpr int kOne = 127, kLo = 127 - 4, kProb = 127 - 4;  // scale operands, 2^(byte - 127)
+
+// the hardware's reciprocal, within 1 ulp
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+// Numbers 0 .. 2^22 by a small divisor: (int)(n * inv) is off by one at most.
+__device__ __forceinline__ int2 divide(int n, int by, float inv) {
+  int q = (int)((float)n * inv), r = n - q * by;
+  if (r < 0) q -= 1, r += by;
+  if (r >= by) q += 1, r -= by;
+  return make_int2(q, r);
+}
+
+// Barrier that publishes LDS writes but leaves DMA on its way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Few queries: 16 NT (row, query head) pairs of one KV head against a range of
+// keys. Four waves share a 64-token block of it; a block of threads is one to
+// four such groups, which take the range's blocks in turn.
+//   S[token, query] = K Q^T, 16x16x128: wave w takes tokens 16 w .. 16 w + 15; lane
+//   (n = lane % 16, g = lane / 16) gives K bytes of token n and Q bytes of query n
+//   and receives tokens 4 g .. 4 g + 3 of query n;
+//   O^T[d, query] += V^T P^T: wave w takes dims 64 w .. 64 w + 63; the 128 places along
+//   tokens hold the hi parts of the 64 probabilities and their lo parts,
+//   against V twice.
+// So each byte of K and V enters one wave's registers once, straight from memory,
+// and the probabilities alone pass between waves (through LDS, one barrier a
+// block). What bounds a short context is how many bytes each CU must fetch
+// (measured 20 a cycle): one group of 64 tokens is enough work for a CU there. In
+// a long one 16 waves of a CU have 4 to 8 KB each on their way: the next block's K
+// is fetched as soon as this one's products have read it, its V likewise. A
+// group's waves share the exponent's reference of a query; it moves when a score
+// of any passes it by more than kSlack.
+// The bound of 1024 threads holds for every G: it keeps the compiler to the 128
+// vector registers of 16 waves a CU and off the accumulator registers.
+template <int NT, int G>
+__global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
+  constexpr int kQueryBytes = NT * 8192, kProbBytes = NT * 4096;  // bytes: the queries' parts; a group's two buffers
+  constexpr int kSumRow = 260, kSum = NT * 16 * kSumRow;  // floats: a query's row of sums; a group's sums
+  // the queries and probabilities; at the end, in their place, the groups' sums
+  constexpr int kIn = kQueryBytes + G * kProbBytes, kOut = G > 1 ? G * kSum * 4 : 0;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kIn > kOut ? kIn : kOut];
+  __shared__ __attribute__((aligned(16))) int moves[2][4 * G];
+  __shared__ __attribute__((aligned(16))) float tops[G][NT * 16][4];
+  __shared__ float scaled[NT * 16], most[G][NT * 16];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), group = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int split = blockIdx.x, tile = blockIdx.y, head = blockIdx.z;
+  const int pairs = a.rows * a.group, end = a.position + a.rows;  // keys that exist
+  const int pair0 = tile * 16 * NT;
+  const int tile_last = a.position + divide(min(pair0 + 16 * NT - 1, pairs - 1), a.group, a.inv_group).x;
+  const int nblk = tile_last / kKv8Block + 1;
+  const int b0 = split * a.per, b1 = min(b0 + a.per, nblk), turns = max(0, (b1 - b0 + G - 1) / G);
+  const size_t store = (size_t)head * c.blocks;
+  const uint8_t* kp = c.k + store * kBlockBytes + (wave >> 1) * 8192 + (wave & 1) * 256 + (g >> 1) * 2048 + (g & 1) * 512 + n * 16;
+  const uint8_t* vp = c.v + store * kBlockBytes + wave * 4096 + (g >> 1) * 1024 + (g & 1) * 512 + n * 16;
+  i32x4 kr[4], vr[4];
+  int ke = 0, ve = 0;
+  auto fetch_k = [&](int b) {
+    const uint8_t* at = kp + (size_t)b * kBlockBytes;
+    ke = c.k_scale[store + b];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kr[i] = *reinterpret_cast<const i32x4*>(at + (i >> 1) * 4096 + (i & 1) * 1024);
+  };
+  auto fetch_v = [&](int b) {
+    const uint8_t* at = vp + (size_t)b * kBlockBytes;
+    ve = c.v_scale[store + b];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vr[i] = *reinterpret_cast<const i32x4*>(at + (i >> 1) * 2048 + (i & 1) * 256);
+  };
+  // queries: 16 lanes a query, 16 dims a lane; their loads go out before the first
+  // keys' (loads return in order), which are on their way during the conversion
   {
-    const uint16_t* q = a.query + ((size_t)row * a.q_heads + qh) * 256 + g * 32;
-    float x[4][16];
-    float top = 0.0f;
+    const int chunk = tid & 15;
+    u32x4 x[2];
+    const int at = min(tid >> 4, 16 * NT - 1);
+    const int2 rq = divide(min(pair0 + at, pairs - 1), a.group, a.inv_group);
+    const u32x4* qp = reinterpret_cast<const u32x4*>(
+        a.query + ((size_t)rq.x * a.q_heads + head * a.group + rq.y) * 256 + chunk * 16);
+    x[0] = qp[0];
+    x[1] = qp[1];
+    issue_fence();
+    const int first = b0 < b1 ? min(b0 + group, b1 - 1) : nblk - 1;
+    fetch_k(first);
+    fetch_v(first);
+    issue_fence();
+    // 256 threads convert 16 queries at a time
+    for (int q = tid >> 4; q < 16 * NT; q += G * 16) {
+      if (q != at) {
+        const int2 next = divide(min(pair0 + q, pairs - 1), a.group, a.inv_group);
+        qp = reinterpret_cast<const u32x4*>(a.query + ((size_t)next.x * a.q_heads + head * a.group + next.y) * 256 + chunk * 16);
+        x[0] = qp[0];
+        x[1] = qp[1];
+      }
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      load16(q + (i >> 1) * 128 + (i & 1) * 16, x[i]);
+      for (int i = 0; i < 8; ++i)
+        top = max(top, max(finite_bits(x[i >> 2][i & 3] << 16), finite_bits(x[i >> 2][i & 3] & 0xffff0000u)));
+      const int e = scale_exponent(row16_max(__uint_as_float(top)), -100);
+      if (chunk == 0) scaled[q] = ldexpf(kLog2e / 16.0f, e);
+      i32x4 hi, lo;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) top = finite(x[i][j]) ? fmaxf(top, fabsf(x[i][j])) : top;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = x[i >> 1][(i & 1) * 2], w = x[i >> 1][(i & 1) * 2 + 1];
+        const int2 p = split_e4m3(ldexpf(bf_lo(u), -e), ldexpf(bf_hi(u), -e), ldexpf(bf_lo(w), -e), ldexpf(bf_hi(w), -e));
+        hi[i] = p.x;
+        lo[i] = p.y;
+      }
+      // [tile][part][128 dims][16 of 32 dims][lane of the product]
+      uint8_t* to = lds + (q >> 4) * 8192 + (chunk >> 3) * 2048 + (chunk & 1) * 1024 + ((chunk >> 1) & 3) * 256 + (q & 15) * 16;
+      *reinterpret_cast<i32x4*>(to) = hi;
+      *reinterpret_cast<i32x4*>(to + 4096) = lo;
     }
-    float2 t = rows_xor16(top);
-    t = rows_xor32(fmaxf(t.x, t.y));
-    const int e = scale_exponent(fmaxf(t.x, t.y), -100);
-    cq = ldexpf(kLog2e / 16.0f, e);
+  }
+  lds_barrier();
+  f32x4 o[NT][4];
+  float m[NT], l[NT], cq[NT];  // the reference, less kShift; the lane's part of the sum, times 2^kShift
+  int last[NT];                // last key of the lane's query
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int q = 0; q < NT; ++q) {
+    m[q] = kNone;
+    l[q] = 0.0f;
+    cq[q] = scaled[16 * q + n];
+    last[q] = a.position + divide(min(pair0 + 16 * q + n, pairs - 1), a.group, a.inv_group).x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+    for (int i = 0; i < 4; ++i) o[q][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  int* const prob = reinterpret_cast<int*>(lds + kQueryBytes + group * kProbBytes);
+  auto block = [&](int turn, auto more) {
+    const int mine = b0 + group + turn * G, b = min(mine, b1 - 1), buf = turn & 1;
+    f32x4 s[NT];
+    {
+      i32x8 k[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) k[h] = __builtin_shufflevector(kr[2 * h], kr[2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int q = 0; q < NT; ++q) {
+        const i32x4* at = reinterpret_cast<const i32x4*>(lds + q * 8192) + lane;
+        i32x8 w[4];  // hi of dims 0 .. 127 and 128 .. 255, lo of both
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_shufflevector(at[i * 128], at[i * 128 + 64], 0, 1, 2, 3, 4, 5, 6, 7);
+        const f32x4 zero = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        s[q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k[0], w[0], zero, 0, 0, 0, kOne, 0, kOne);
+        f32x4 rest = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k[0], w[2], zero, 0, 0, 0, kOne, 0, kLo);
+        s[q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k[1], w[1], s[q], 0, 0, 0, kOne, 0, kOne);
+        rest = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k[1], w[3], rest, 0, 0, 0, kOne, 0, kLo);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[q][i] += rest[i];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NT; ++q) asm volatile("" : "+v"(s[q]));  // the keys' registers are free
+    const float scale = ldexpf(1.0f, ke - 127);
+    issue_fence();
+    if constexpr (decltype(more)::value) fetch_k(min(mine + G, b1 - 1));
+    issue_fence();
+    float top[NT], part[NT];
+    bool pass = false;
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      const float cs = fmaxf(cq[q] * scale, 1e-37f);
+      const int left = (mine < b1 ? last[q] : -1) - (b * 64 + 16 * wave + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[q][i] = i <= left ? s[q][i] * cs : -__builtin_inff();
+      top[q] = fmaxf(fmaxf(s[q][0], s[q][1]), fmaxf(s[q][2], s[q][3])) - kShift;
+      pass |= top[q] > m[q] + kSlack;
+    }
+    auto probabilities = [&]() {
+#pragma unroll
+      for (int q = 0; q < NT; ++q) {
         float y[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) y[b] = ldexpf(x[i][4 * j + b], -e);
+        for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_exp2f(s[q][i] - m[q]);
         const int h = pack_e4m3(y[0], y[1], y[2], y[3]);
-        const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), v = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
-        qhi[i >> 1][(i & 1) * 4 + j] = h;
-        qlo[i >> 1][(i & 1) * 4 + j] = pack_e4m3((y[0] - u[0]) * 16.0f, (y[1] - u[1]) * 16.0f, (y[2] - v[0]) * 16.0f,
-                                                 (y[3] - v[1]) * 16.0f);
+        const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), w = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
+        int* to = prob + ((buf * NT + q) * 2) * 256 + lane * 4 + wave;
+        to[0] = h;
+        to[256] = pack_e4m3(y[0] - u[0], y[1] - u[1], y[2] - w[0], y[3] - w[1]);
+        part[q] = (y[0] + y[1]) + (y[2] + y[3]);
       }
+    };
+    const bool move = __any(pass);
+    if (lane == 0) moves[buf][group * 4 + wave] = move;
+    if (!move) probabilities();
+    lds_barrier();
+    int moved = 0;
+    if (lane < G * 4) moved = moves[buf][lane];
+    if (__any(moved)) {
+#pragma unroll
+      for (int q = 0; q < NT; ++q) {
+        const float2 x = rows_xor16(top[q]);
+        const float2 y = rows_xor32(fmaxf(x.x, x.y));
+        if (g == 0) tops[group][q * 16 + n][wave] = fmaxf(y.x, y.y);
+      }
+      lds_barrier();
+#pragma unroll
+      for (int q = 0; q < NT; ++q) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(tops[group][q * 16 + n]);
+        const float mn = fmaxf(m[q], fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+        const float f = __builtin_amdgcn_exp2f(m[q] - mn);
+        m[q] = mn;
+        l[q] *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[q][i][k] *= f;
+      }
+      probabilities();
+      lds_barrier();
+    }
+#pragma unroll
+    for (int q = 0; q < NT; ++q) l[q] += part[q];
+    if (b * 64 + 64 > end) {  // bytes behind the last key may be anything
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int left = end - (b * 64 + 16 * t + 4 * g);
+        const int mask = left >= 4 ? -1 : left <= 0 ? 0 : (1 << (8 * left)) - 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vr[i][t] &= mask;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      const i32x4* at = reinterpret_cast<const i32x4*>(prob + ((buf * NT + q) * 2) * 256) + lane;
+      const i32x8 p = __builtin_shufflevector(at[0], at[64], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const i32x8 v = __builtin_shufflevector(vr[i], vr[i], 0, 1, 2, 3, 0, 1, 2, 3);
+        o[q][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, p, o[q][i], 0, 0, 0, ve, 0, kProb);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(o[q][i]));
+    issue_fence();
+    if constexpr (decltype(more)::value) fetch_v(min(mine + G, b1 - 1));
+    issue_fence();
+  };
+  // two bodies, so that the waits for loads count what is on its way in each
+  for (int turn = 0; turn + 1 < turns; ++turn) block(turn, std::true_type{});
+  if (turns > 0) block(turns - 1, std::false_type{});
+  // the lanes and waves of a query hold its tokens' parts of the sum
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < NT; ++q) {
+    const float2 x = rows_xor16(l[q]);
+    const float2 y = rows_xor32(x.x + x.y);
+    if (g == 0) {
+      tops[group][q * 16 + n][wave] = (y.x + y.y) * (1.0f / 16.0f);
+      if (wave == 0) most[group][q * 16 + n] = m[q];
+    }
   }
-  const int last = a.position + row, end = a.position + a.rows;  // last key of the query; keys that exist
-  const int tile_end = a.position + min(tile * 16 + 15, pairs - 1) / a.group + 1;
-  const int nblk = (tile_end + kKv8Block - 1) / kKv8Block;
-  const int b0 = (int)((int64_t)nblk * split / a.splits), b1 = (int)((int64_t)nblk * (split + 1) / a.splits);
-  const size_t store = (size_t)head * c.blocks;
-  const uint8_t* kp = c.k + store * kBlockBytes + (g >> 1) * 2048 + (g & 1) * 512 + n * 16;
-  const uint8_t* vp = c.v + store * kBlockBytes + (g >> 1) * 1024 + (g & 1) * 512 + n * 16;
-  f32x4 o[16];
+  if constexpr (G > 1) {
+    float* sum = reinterpret_cast<float*>(lds) + group * kSum;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = kNone, l = 0.0f;
-  for (int b = b0 + wave; b < b1; b += 4) {
-    const uint8_t* kb = kp + (size_t)b * kBlockBytes;
-    const uint8_t* vb = vp + (size_t)b * kBlockBytes;
-    f32x4 s[4];
+    for (int q = 0; q < NT; ++q)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(sum + (q * 16 + n) * kSumRow + wave * 64 + i * 16 + g * 4) = o[q][i];
+  }
+  __syncthreads();
+  // group k finishes tiles k, k + G, ..
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* at = kb + (t >> 1) * 8192 + (t & 1) * 256 + h * 4096;
-        const i32x4 x = *reinterpret_cast<const i32x4*>(at), y = *reinterpret_cast<const i32x4*>(at + 1024);
-        const i32x8 k = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, qhi[h], s[t], 0, 0, 0, kOne, 0, kOne);
-        s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, qlo[h], s[t], 0, 0, 0, kOne, 0, kLo);
-      }
+  for (int q = 0; q < NT; ++q) {
+    const int pair = pair0 + 16 * q + n, at = q * 16 + n;
+    if (q % G != group || pair >= pairs) continue;
+    float ref = kNone, f[G], total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < G; ++k) ref = fmaxf(ref, most[k][at]);
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(tops[k][at]);
+      f[k] = __builtin_amdgcn_exp2f(most[k][at] - ref);
+      total = fmaf((t[0] + t[1]) + (t[2] + t[3]), f[k], total);
     }
-    const float cs = ldexpf(cq, (int)c.k_scale[store + b] - 127);
-    float top = kNone;
+    const int2 to = divide(pair, a.group, a.inv_group);
+    const size_t row = (size_t)to.x * a.q_heads + head * a.group + to.y;
+    const int d = wave * 64 + g * 4;
+    float* part = a.part + (row * a.splits + split) * kKv8PartFloats;
+    const float inv = 1.0f / total;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int i = 0; i < 4; ++i) {
+      f32x4 x = o[q][i];
+      if constexpr (G > 1) {
+        x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = s[t][i] * cs;
-        if (b * 64 + 63 > a.position) x = b * 64 + 16 * t + 4 * g + i <= last ? x : -__builtin_inff();
-        s[t][i] = x;
-        top = fmaxf(top, x);
-      }
-    float2 u = rows_xor16(top);
-    u = rows_xor32(fmaxf(u.x, u.y));
-    const float mn = fmaxf(m, fmaxf(u.x, u.y));
-    const float f = __builtin_amdgcn_exp2f(m - mn);
-    m = mn;
-    l *= f;
-    i32x8 p;
+        for (int k = 0; k < G; ++k) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(lds) + k * kSum +
+                                                          at * kSumRow + d + 16 * i);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[i] = __builtin_amdgcn_exp2f(s[t][i] - mn + 8.0f);
-        l += y[i];
-      }
-      const int h = pack_e4m3(y[0], y[1], y[2], y[3]);
-      const f32x2 v = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), w = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
-      p[t] = h;
-      p[4 + t] = pack_e4m3(y[0] - v[0], y[1] - v[1], y[2] - w[0], y[3] - w[1]);
-    }
-    const int vs = c.v_scale[store + b];
-#pragma unroll
-    for (int d = 0; d < 16; ++d) {
-      i32x4 x = *reinterpret_cast<const i32x4*>(vb + (d >> 1) * 2048 + (d & 1) * 256);
-      if (b * 64 + 64 > end) {  // bytes behind the last key may be anything
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int left = end - (b * 64 + 16 * t + 4 * g);
-          x[t] = left >= 4 ? x[t] : left <= 0 ? 0 : x[t] & ((1 << (8 * left)) - 1);
+          for (int j = 0; j < 4; ++j) x[j] = fmaf(y[j], f[k], x[j]);
         }
       }
-      const i32x8 v = __builtin_shufflevector(x, x, 0, 1, 2, 3, 0, 1, 2, 3);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[d][i] *= f;
-      o[d] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, p, o[d], 0, 0, 0, vs, 0, kProb);
-    }
-  }
-  // l counts p * 2^8; the lanes of a query hold its tokens' parts
-  float2 t = rows_xor16(l);
-  t = rows_xor32(t.x + t.y);
-  if (lane < 16) {
-    mx[wave][n] = m;
-    den[wave][n] = (t.x + t.y) * (1.0f / 256.0f);
-  }
-#pragma unroll
-  for (int d = 0; d < 16; ++d) *reinterpret_cast<f32x4*>(&sum[wave][n][d * 16 + g * 4]) = o[d];
-  __syncthreads();
-  const int qi = tid >> 4, dd = (tid & 15) * 4;
-  if (tile * 16 + qi >= pairs) return;
-  float top = kNone;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, mx[w][qi]);
-  float f[4], total = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = __builtin_amdgcn_exp2f(mx[w][qi] - top);
-    total = fmaf(den[w][qi], f[w], total);
-  }
-  const int i = tile * 16 + qi, r = i / a.group, hq = head * a.group + i % a.group;
-  const size_t at = (size_t)r * a.q_heads + hq;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(&sum[w][qi][dd + 64 * j]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = fmaf(y[k], f[w], x[k]);
-    }
-    if (a.splits > 1) {
-      float* part = a.part + (at * a.splits + split) * kKv8PartFloats;
-      *reinterpret_cast<f32x4*>(part + dd + 64 * j) = x;
-      if (tid % 16 == 0 && j == 0) {
-        part[256] = top;
-        part[257] = total;
+      if (a.splits > 1) {
+        *reinterpret_cast<f32x4*>(part + d + 16 * i) = x;
+        if (i == 0 && wave == 0 && g == 0) *reinterpret_cast<float2*>(part + 256) = make_float2(ref, total);
+        continue;
       }
-      continue;
-    }
-    const uint16_t* gp = a.gate ? a.gate + at * 512 + 256 + dd + 64 * j : nullptr;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[k] = x[k] / total;
-      if (gp) x[k] = gated(x[k], gp + k);
+      for (int k = 0; k < 4; ++k) x[k] *= inv;
+      if (a.gate) {
+        const uint2 gate = *reinterpret_cast<const uint2*>(a.gate + row * 512 + 256 + d + 16 * i);
+        x[0] *= sigmoid(bf_lo(gate.x));
+        x[1] *= sigmoid(bf_hi(gate.x));
+        x[2] *= sigmoid(bf_lo(gate.y));
+        x[3] *= sigmoid(bf_hi(gate.y));
+      }
+      *reinterpret_cast<uint2*>(a.out + row * 256 + d + 16 * i) = make_uint2(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]));
     }
-    *reinterpret_cast<uint2*>(a.out + at * 256 + dd + 64 * j) = make_uint2(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]));
   }
 }
 
-// Joins the ranges of keys of one (row, query head): four waves take every
-// fourth range, lane = four dims.
+// Joins the ranges of keys of one (row, query head), 64 dims a block: thread t
+// holds range t's maximum and sum, and four dims of ranges t / 16 + 16 i, all
+// fetched at once.
 __global__ __launch_bounds__(256) void k_kv8_attn_join(Kv8Attn a) {
-  __shared__ __attribute__((aligned(16))) float sum[4][256];
-  __shared__ float mx[4], den[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const size_t at = blockIdx.x;
+  __shared__ __attribute__((aligned(16))) float sum[16][64];
+  __shared__ float weight[256], wmax[4], wden[4];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, slot = t >> 4;
+  const size_t at = blockIdx.x >> 2;
+  const int d0 = (blockIdx.x & 3) * 64;
   const float* part = a.part + at * a.splits * kKv8PartFloats;
-  float m = kNone, l = 0.0f;
-  f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = wave; s < a.splits; s += 4) {
-    const float* p = part + (size_t)s * kKv8PartFloats;
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p + lane * 4);
-    const float mn = fmaxf(m, p[256]), f = __builtin_amdgcn_exp2f(m - mn), fx = __builtin_amdgcn_exp2f(p[256] - mn);
-    l = fmaf(p[257], fx, l * f);
+  const float2 md = t < a.splits ? *reinterpret_cast<const float2*>(part + (size_t)t * kKv8PartFloats + 256)
+                                 : make_float2(kNone, 0.0f);
+  const float* mine = part + (size_t)slot * kKv8PartFloats + d0 + (t & 15) * 4;
+  f32x4 x[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = fmaf(x[k], fx, o[k] * f);
-    m = mn;
-  }
-  if (lane == 0) {
-    mx[wave] = m;
-    den[wave] = l;
-  }
-  *reinterpret_cast<f32x4*>(&sum[wave][lane * 4]) = o;
+  for (int i = 0; i < 8; ++i)
+    if (slot + 16 * i < a.splits) x[i] = *reinterpret_cast<const f32x4*>(mine + (size_t)i * 16 * kKv8PartFloats);
+  const float wm = wave_max(md.x);
+  if (lane == 0) wmax[wave] = wm;
   __syncthreads();
-  const int d = threadIdx.x;
-  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-  float x = 0.0f, total = 0.0f;
+  const float top = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+  const float f = __builtin_amdgcn_exp2f(md.x - top);
+  weight[t] = f;
+  const float den = tree64(md.y * f);
+  if (lane == 0) wden[wave] = den;
+  __syncthreads();
+  f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float f = __builtin_amdgcn_exp2f(mx[w] - top);
-    x = fmaf(sum[w][d], f, x);
-    total = fmaf(den[w], f, total);
+  for (int i = 0; i < 8; ++i) {
+    if (slot + 16 * i >= a.splits) break;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = fmaf(x[i][k], weight[slot + 16 * i], o[k]);
   }
-  x = x / total;
-  if (a.gate) x = gated(x, a.gate + at * 512 + 256 + d);
-  a.out[at * 256 + d] = (uint16_t)f2bf(x);
+  for (int s = slot + 128; s < a.splits; s += 16) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(mine + (size_t)(s - slot) * kKv8PartFloats);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = fmaf(y[k], weight[s], o[k]);
+  }
+  *reinterpret_cast<f32x4*>(&sum[slot][(t & 15) * 4]) = o;
+  __syncthreads();
+  if (t >= 64) return;
+  const float total = (wden[0] + wden[1]) + (wden[2] + wden[3]);
+  float y = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) y += sum[i][t];
+  y = y / total;
+  if (a.gate) y *= sigmoid(bf2f(a.gate[at * 512 + 256 + d0 + t]));
+  a.out[at * 256 + d0 + t] = (uint16_t)f2bf(y);
 }
 
-int few_tiles(int rows, int group) { return (rows * group + 15) / 16; }
-// Ranges of keys of one call: enough blocks for the chip's 256 CUs, none without work for its four waves.
-int few_splits(int heads, int tiles, int position, int rows) {
-  const int nblk = (position + rows + kKv8Block - 1) / kKv8Block;
-  const int most = 256 / (heads * tiles), want = (nblk + 3) / 4;
-  return most < 2 || want < 2 ? 1 : most < want ? most : want;
-}
+// 16-query tiles of a block: as many as the pairs fill, two at most.
+int few_nt(int pairs) { return pairs <= 16 ? 1 : 2; }
+int few_tiles(int pairs) { return (pairs + 16 * few_nt(pairs) - 1) / (16 * few_nt(pairs)); }
+// Ranges of keys of one call: enough blocks for the chip's 256 CUs.
+int few_ranges(int heads, int tiles) { return max(1, 256 / (heads * tiles)); }
 
 }  // namespace
 
 size_t kv8_attn_scratch_bytes(int q_heads, int kv_heads, int rows) {
-  const int tiles = few_tiles(rows, q_heads / kv_heads);
-  const int most = 256 / (kv_heads * tiles);
+  const int most = few_ranges(kv_heads, few_tiles(rows * (q_heads / kv_heads)));
   return most < 2 ? 0 : (size_t)rows * q_heads * most * kKv8PartFloats * sizeof(float);
 }
 
@@ -602,12 +764,19 @@ hipError_t launch_kv8_read(const Kv8& c, int position, int rows, uint16_t* k, ui
 }
 
 hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
-  a.tiles = few_tiles(a.rows, a.group);
-  a.splits = few_splits(c.heads, a.tiles, a.position, a.rows);
-  hipLaunchKernelGGL(k_kv8_attn_few, dim3(a.splits * c.heads * a.tiles), dim3(256), 0, s, c, a);
+  const int tiles = few_tiles(a.rows * a.group), nblk = (a.position + a.rows - 1) / kKv8Block + 1;
+  const int ranges = few_ranges(c.heads, tiles);
+  a.inv_group = 1.0f / (float)a.group;
+  a.per = (nblk + ranges - 1) / ranges;
+  a.splits = (nblk + a.per - 1) / a.per;
+  const int g = a.per >= 4 ? 4 : a.per >= 2 ? 2 : 1;
+  const auto few = few_nt(a.rows * a.group) == 1
+                       ? (g == 4 ? k_kv8_attn_few<1, 4> : g == 2 ? k_kv8_attn_few<1, 2> : k_kv8_attn_few<1, 1>)
+                       : (g == 4 ? k_kv8_attn_few<2, 4> : g == 2 ? k_kv8_attn_few<2, 2> : k_kv8_attn_few<2, 1>);
+  hipLaunchKernelGGL(few, dim3(a.splits, tiles, c.heads), dim3(256 * g), 0, s, c, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL(k_kv8_attn_join, dim3(a.rows * a.q_heads), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(k_kv8_attn_join, dim3(a.rows * a.q_heads * 4), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
