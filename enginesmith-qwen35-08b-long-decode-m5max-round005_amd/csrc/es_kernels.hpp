@@ -360,7 +360,8 @@ struct Kv8Attn {
   uint16_t* out;
   float* part;           // kv8_attn_scratch_bytes
   int q_heads, group, position, rows;
-  int splits, per;       // ranges of keys and 64-key blocks of each (by the launcher, as inv_group)
+  int splits, per;       // ranges of keys and 64-key blocks of each (by the launcher, as the rest)
+  int tiles;
   float inv_group;
 };
 size_t kv8_attn_scratch_bytes(int q_heads, int kv_heads, int rows);

@@ -730,6 +730,325 @@ __global__ __launch_bounds__(256) void k_kv8_attn_join(Kv8Attn a) {
   a.out[at * 256 + d0 + t] = (uint16_t)f2bf(y);
 }
 
+// DMA into LDS: 16 bytes a lane from `uniform` + `lane` of a buffer, piece I of
+// 1024 bytes behind each other, to LDS `to`; or one byte of a buffer to each dword of
+// the 64 at `to`. In assembly, so that the compiler's waits before it reads LDS do
+// not count these (the kernel's own do); a buffer spans all 32-bit offsets: what is
+// in range is the caller's affair.
+typedef __attribute__((address_space(3))) void* lptr_t;
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+__device__ __forceinline__ u32x4 buffer_of(const uint8_t* base) {
+  return u32x4{(uint32_t)(uintptr_t)base, (uint32_t)((uintptr_t)base >> 32), 0xffffffffu, 0x00020000u};
+}
+template <int I>
+__device__ __forceinline__ void dma16(u32x4 from, uint32_t lane, uint32_t uniform, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen offset:%4 lds"
+               :
+               : "s"(to), "v"(lane), "s"(from), "s"(uniform), "n"(I * 1024)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma1(u32x4 from, uint32_t uniform, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ubyte off, %1, %2 lds"
+               :
+               : "s"(to), "s"(from), "s"(uniform)
+               : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// Many queries: 128 (row, query head) pairs of one KV head, eight waves, two a SIMD.
+// Wave w holds the 32 pairs 32 (w % 4) ..; the lower four waves take the even blocks
+// of keys, the upper four the odd ones, and both halves are joined at the end.
+//   S^T[token, query] = K Q^T and O^T[d, query] += V^T P^T on 32x32x64, each query
+//   (probability) as the sum of two e4m3 numbers, the lower one 16 times too large
+//   and with a power of two of its own. Lane (r = lane % 32, h = lane / 32) gives K's
+//   bytes of token r (V's of dim r) and those of query r, and receives tokens (dims)
+//   8 i + 4 h .. + 3 of query r: the tokens whose probabilities it has to give next.
+// In phase p the waves of block p make its scores, those of block p - 1 its
+// probabilities and their products, so that of a SIMD's two waves one uses the
+// matrix core while the other works on its softmax. K and V reach LDS by DMA, in the
+// order of the operands, two to three phases ahead; the queries' lower part stays in
+// LDS, as registers are full: 128 of sums, 24 of queries, 32 of scores, operands.
+// Measured: 4096 rows behind 28672, 8 query and 2 KV heads, 806 to 853 us (1.0e12
+// operations, 1.2e15 a second). A phase takes 3040 cycles, 2048 of them
+// of the matrix core (without the softmax 2660, without the DMA 3010), and with all
+// 256 CUs at it the clock falls from 2.4 to 1.9 GHz. Four waves with 32 queries and
+// all keys each, the same steps interleaved within a wave, took 3530 cycles; eight
+// with 16 queries, both parts as columns of one product, 3560.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+constexpr int kRowPairs = 128, kRowDma = 3;      // DMA instructions of a wave for a block's K (or V)
+constexpr int kKStages = 3, kVStages = 4;
+// LDS: the queries' lower parts, 64 dims of their upper ones, K, V
+constexpr int kRowLast = kRowPairs * 256, kRowStages = kRowLast + kRowPairs * 64;
+constexpr int kRowBytes = kRowStages + (kKStages + kVStages) * kBlockBytes;
+__global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kRowBytes];
+  __shared__ int exponent[kKStages + kVStages][64];  // each 64 times
+  __shared__ float scaled[kRowPairs], most[2][kRowPairs], sums[2][kRowPairs];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), upper = wave >> 2, mine = (wave & 3) * 32 + r;
+  // heads in turn, so that an XCD's blocks share a head's keys where the heads
+  // divide the XCDs; the longest ranges of keys first
+  const int head = (int)blockIdx.x % c.heads, tile = a.tiles - 1 - (int)blockIdx.x / c.heads;
+  const int pairs = a.rows * a.group, end = a.position + a.rows, pair0 = tile * kRowPairs;
+  const int nblk = (a.position + divide(min(pair0 + kRowPairs - 1, pairs - 1), a.group, a.inv_group).x) / kKv8Block + 1;
+  const size_t store = (size_t)head * c.blocks;
+  const auto kbuf = buffer_of(c.k + store * kBlockBytes), vbuf = buffer_of(c.v + store * kBlockBytes);
+  const auto kscale = buffer_of(c.k_scale + store), vscale = buffer_of(c.v_scale + store);
+  const uint32_t part = wave * 2048;
+  auto kstage = [](int b) { return (uint32_t)b % kKStages; };
+  auto vstage = [](int b) { return kKStages + (uint32_t)b % kVStages; };
+  // K and V of block b. One behind the last is fetched as the last, into the stage of
+  // a block that is done with, so that every phase's wait counts the same instructions.
+  auto issue = [&](int b) {
+    const uint32_t at = min(b, nblk - 1), k = kstage(b), v = vstage(b), to = lds_address(lds) + kRowStages + part;
+    dma16<0>(kbuf, part + lane * 16, at * kBlockBytes, to + k * kBlockBytes);
+    dma16<1>(kbuf, part + lane * 16, at * kBlockBytes, to + k * kBlockBytes);
+    dma1(kscale, at, lds_address(exponent) + k * 256);
+    dma16<0>(vbuf, part + lane * 16, at * kBlockBytes, to + v * kBlockBytes);
+    dma16<1>(vbuf, part + lane * 16, at * kBlockBytes, to + v * kBlockBytes);
+    dma1(vscale, at, lds_address(exponent) + v * 256);
+  };
+  auto read = [&](uint32_t at) {  // 32 bytes a lane of 2048
+    const i32x4* from = reinterpret_cast<const i32x4*>(lds + at) + lane;
+    return __builtin_shufflevector(from[0], from[64], 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  // queries: 16 lanes a query, 16 dims a lane; the upper parts through V's last stages
+  i32x8 qhi[3];
+  {
+    const int chunk = tid & 15;
+    u32x4 x[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int2 rq = divide(min(pair0 + 32 * i + (tid >> 4), pairs - 1), a.group, a.inv_group);
+      const u32x4* qp = reinterpret_cast<const u32x4*>(
+          a.query + ((size_t)rq.x * a.q_heads + head * a.group + rq.y) * 256 + chunk * 16);
+      x[i][0] = qp[0];
+      x[i][1] = qp[1];
+    }
+    issue_fence();
+    issue(0);
+    issue(1);
+    issue_fence();
+    const int upper_parts = kRowStages + vstage(2) * kBlockBytes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        top = max(top, max(finite_bits(x[i][j >> 2][j & 3] << 16), finite_bits(x[i][j >> 2][j & 3] & 0xffff0000u)));
+      const int e = scale_exponent(row16_max(__uint_as_float(top)), -100);
+      scaled[32 * i + (tid >> 4)] = ldexpf(kLog2e / 16.0f, e);
+      i32x4 hi, lo;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = x[i][j >> 1][(j & 1) * 2], w = x[i][j >> 1][(j & 1) * 2 + 1];
+        const int2 p = split_e4m3(ldexpf(bf_lo(u), -e), ldexpf(bf_hi(u), -e), ldexpf(bf_lo(w), -e), ldexpf(bf_hi(w), -e));
+        hi[j] = p.x;
+        lo[j] = p.y;
+      }
+      // [32 queries][64 dims][16 of 32 dims][lane of the product]
+      const int to = i * 8192 + (chunk >> 2) * 2048 + (chunk & 1) * 1024 + ((chunk >> 1) & 1) * 512 + (tid >> 4) * 16;
+      *reinterpret_cast<i32x4*>(lds + (chunk < 12 ? upper_parts + to : kRowLast + to - i * 6144 - 6144)) = hi;
+      *reinterpret_cast<i32x4*>(lds + to) = lo;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) qhi[i] = read(upper_parts + (wave & 3) * 8192 + i * 2048);
+  }
+  const float cq = scaled[mine];
+  const int2 rq = divide(min(pair0 + mine, pairs - 1), a.group, a.inv_group);
+  const int last = a.position + rq.x;  // last key of the lane's query
+  f32x16 o[8], s[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[i][k] = 0.0f;
+  float m = kNone, l = 0.0f, cs = 0.0f;  // reference less kShift; the lane's part of the sum, times 2^kShift
+  auto scores = [&](int b) {
+    const uint32_t from = kRowStages + kstage(b) * kBlockBytes, lower = (wave & 3) * 8192;
+    const int ke = exponent[kstage(b)][lane];
+    auto key = [&](int t) { return read(from + (t & 1) * 8192 + (t >> 1) * 2048); };
+    i32x8 k[8], ql[4], qh[4] = {qhi[0], qhi[1], qhi[2]};
+    k[0] = key(0);
+    k[1] = key(1);
+    ql[0] = read(lower);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 9; ++t) {  // 64 dims t / 2 by 32 tokens t % 2, the lower parts a step later
+      issue_fence();
+      if (t < 8) s[t & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k[t], qh[t / 2], s[t & 1], 0, 0, 0, kOne, 0, kOne);
+      if (t > 0) {
+        const int u = t - 1;
+        s[u & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k[u], ql[u / 2], s[u & 1], 0, 0, 0, kOne, 0, kLo);
+      }
+      issue_fence();
+      if (t < 6) k[t + 2] = key(t + 2);
+      if (t == 4) qh[3] = read(kRowLast + (wave & 3) * 2048);
+      if (t % 2 == 0 && t > 0 && t < 8) ql[t / 2] = read(lower + t * 1024);
+    }
+    if (b * 64 + 63 > a.position) {  // the causal border
+      const int left = last - b * 64 - 4 * h;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) s[i][k] = 32 * i + 8 * (k >> 2) + (k & 3) <= left ? s[i][k] : -__builtin_inff();
+    }
+    float tops[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) tops[k] = s[k >> 1][8 * (k & 1)];
+#pragma unroll
+    for (int k = 1; k < 8; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // the larger; fmaxf would first quiet what a product gave
+        tops[i] = __builtin_amdgcn_fmed3f(tops[i], s[i >> 1][8 * (i & 1) + k], __builtin_inff());
+    float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    cs = fmaxf(ldexpf(cq, ke - 127), 1e-37f);
+    top = top * cs - kShift;
+    if (__any(top > m + kSlack)) {
+      const float2 u = rows_xor32(top);
+      const float next = fmaxf(m, fmaxf(u.x, u.y)), f = __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[i][k] *= f;
+    }
+  };
+  auto values = [&](int b) {
+    const uint32_t from = kRowStages + vstage(b) * kBlockBytes;
+    const int ve = exponent[vstage(b)][lane];
+    i32x8 v[8], phi, plo;
+    // sums 0 .. 3 are of the wave's own half of the dims, 4 .. 7 of the other's
+    auto fetch = [&](int t) { v[t] = read(t < 4 ? from + upper * 8192 + t * 2048 : from - upper * 8192 + t * 2048); };
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[k] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][4 * (i & 3) + k], cs, -m));
+      sum += (y[0] + y[1]) + (y[2] + y[3]);
+      const int hi = pack_e4m3(y[0], y[1], y[2], y[3]);
+      const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), w = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+      i16x2 q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(i16x2{0, 0}, y[0] - u[0], y[1] - u[1], 0.0625f, false);
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(q, y[2] - w[0], y[3] - w[1], 0.0625f, true);
+      phi[(i & 1) * 4 + (i >> 1)] = hi;
+      plo[(i & 1) * 4 + (i >> 1)] = __builtin_bit_cast(int, q);
+    }
+    l += sum;
+    fetch(0);
+    fetch(1);
+#pragma unroll
+    for (int t = 0; t < 9; ++t) {
+      issue_fence();
+      if (t < 8) o[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v[t], phi, o[t], 0, 0, 0, ve, 0, kProb);
+      if (t < 6) fetch(t + 2);
+      if (t > 0) o[t - 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v[t - 1], plo, o[t - 1], 0, 0, 0, ve, 0, kProb - 4);
+    }
+  };
+  // K of the phase and V of the one before have arrived once all but the last three
+  // groups have; every wave is past what the next ones replace.
+  auto phase = [&](int p) {
+    wait_vmcnt<3 * kRowDma>();
+    lds_barrier();
+    issue(p + 2);
+    issue_fence();
+    if (p == nblk - 1 && nblk * 64 > end) {  // bytes behind the last key may be anything
+      wait_vmcnt<4 * kRowDma>();             // V of the phase's block: each wave clears what it fetched
+      int own = lane;
+      asm volatile("" : "+v"(own));  // masks are no registers of the loop's
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        i32x4* at = reinterpret_cast<i32x4*>(lds + kRowStages + vstage(p) * kBlockBytes + part) + i * 64 + own;
+        i32x4 w = *at;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int left = end - p * 64 - (16 * k + 8 * i + 4 * (own >> 5));
+          w[k] &= (int)((1ull << (8 * min(max(left, 0), 4))) - 1);
+        }
+        *at = w;
+      }
+    }
+  };
+  if (upper) phase(0);
+  for (int b = upper; b < nblk; b += 2) {
+    phase(b);
+    scores(b);
+    phase(b + 1);
+    values(b);
+  }
+  if ((nblk & 1) == upper) lds_barrier();
+  wait_vmcnt<0>();  // no DMA outlives this
+  // Both halves: each wave finishes half of the dims.
+  const float2 t = rows_xor32(l);
+  if (h == 0) {
+    most[upper][mine] = m;
+    sums[upper][mine] = t.x + t.y;
+  }
+  lds_barrier();
+  f32x4* const swap = reinterpret_cast<f32x4*>(lds) + lane;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f32x4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = o[4 + i][4 * k + j];
+      swap[wave * 1024 + (4 * i + k) * 64] = x;
+    }
+  lds_barrier();
+  const float other = most[1 - upper][mine], ref = fmaxf(m, other);
+  float f = __builtin_amdgcn_exp2f(m - ref), fo = __builtin_amdgcn_exp2f(other - ref);
+  const float inv = 16.0f / fmaf(sums[upper][mine], f, sums[1 - upper][mine] * fo);  // 2^kShift
+  f *= inv;
+  fo *= inv;
+  const size_t row = (size_t)rq.x * a.q_heads + head * a.group + rq.y;
+  // a lane without a pair stores behind the end of the buffer, which drops it
+  const auto out = __builtin_amdgcn_make_buffer_rsrc((void*)a.out, 0, (int)((uint32_t)a.rows * a.q_heads * 512u), 0x00020000);
+  const uint32_t to = pair0 + mine < pairs ? (uint32_t)row * 512u + upper * 256 + h * 16 : 0xfffff000u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {  // 16 dims: lower lanes end with 0 .. 7, upper with 8 .. 15
+      float z[8], y[8];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const f32x4 x = swap[(wave ^ 4) * 1024 + (4 * i + 2 * j + k) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          z[4 * k + e] = fmaf(o[i][8 * j + 4 * k + e], f, x[e] * fo);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(z[k]), __float_as_uint(z[4 + k]), false, false);
+        y[k] = __uint_as_float(w[0]);
+        y[4 + k] = __uint_as_float(w[1]);
+      }
+      if (a.gate) {
+        const u32x4 gate = *reinterpret_cast<const u32x4*>(a.gate + row * 512 + 256 + upper * 128 + 32 * i + 16 * j + 8 * h);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          y[2 * k] *= sigmoid(bf_lo(gate[k]));
+          y[2 * k + 1] *= sigmoid(bf_hi(gate[k]));
+        }
+      }
+      const u32x4 packed{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]), pack_bf2(y[4], y[5]), pack_bf2(y[6], y[7])};
+      __builtin_amdgcn_raw_buffer_store_b128(packed, out, to + (32 * i + 16 * j) * 2, 0, 0);
+    }
+}
+
+// Whether 128 pairs a block, all keys each, fill enough of the chip's 256 CUs: with
+// 160 full blocks' worth. (At 128 of them, 2048 rows behind 30000 and 2 heads, the
+// form with ranges takes 582 us and this 659; at 176, 700 rows behind 20000 and 8
+// heads, 586 and 443; at 256, 4096 rows behind 28672 and 2 heads, 1145 and 853.)
+bool many(int pairs, int heads) { return (int64_t)pairs * heads >= 160 * kRowPairs; }
 // 16-query tiles of a block: as many as the pairs fill, two at most.
 int few_nt(int pairs) { return pairs <= 16 ? 1 : 2; }
 int few_tiles(int pairs) { return (pairs + 16 * few_nt(pairs) - 1) / (16 * few_nt(pairs)); }
@@ -739,7 +1058,7 @@ int few_ranges(int heads, int tiles) { return max(1, 256 / (heads * tiles)); }
 }  // namespace
 
 size_t kv8_attn_scratch_bytes(int q_heads, int kv_heads, int rows) {
-  const int most = few_ranges(kv_heads, few_tiles(rows * (q_heads / kv_heads)));
+  const int pairs = rows * (q_heads / kv_heads), most = many(pairs, kv_heads) ? 1 : few_ranges(kv_heads, few_tiles(pairs));
   return most < 2 ? 0 : (size_t)rows * q_heads * most * kKv8PartFloats * sizeof(float);
 }
 
@@ -764,9 +1083,14 @@ hipError_t launch_kv8_read(const Kv8& c, int position, int rows, uint16_t* k, ui
 }
 
 hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
+  a.inv_group = 1.0f / (float)a.group;
+  if (many(a.rows * a.group, c.heads)) {
+    a.tiles = (a.rows * a.group + kRowPairs - 1) / kRowPairs;
+    hipLaunchKernelGGL(k_kv8_attn_rows, dim3(a.tiles * c.heads), dim3(512), 0, s, c, a);
+    return hipGetLastError();
+  }
   const int tiles = few_tiles(a.rows * a.group), nblk = (a.position + a.rows - 1) / kKv8Block + 1;
   const int ranges = few_ranges(c.heads, tiles);
-  a.inv_group = 1.0f / (float)a.group;
   a.per = (nblk + ranges - 1) / ranges;
   a.splits = (nblk + a.per - 1) / a.per;
   const int g = a.per >= 4 ? 4 : a.per >= 2 ? 2 : 1;

@@ -353,6 +353,91 @@ def test_growing_scores_move_the_maximum_in_every_block(rows):
     kv8.check_attention(kv8.attend(cache, q, n - rows), q, k, v, n - rows, spread=False)
 
 
+def same_as_in_parts(got, cache, q, position, g=None, rows=48):
+    """Many rows and the same ones some at a time, which other kernels compute:
+    NaN in the same places, and each output's error of 2^-8 at most (root mean square) on
+    either side, so one vector of another row would be seen among 20000."""
+    parts = [kv8.attend(cache, q[i:i + rows], position + i, None if g is None else g[i:i + rows])
+             for i in range(0, len(q), rows)]
+    a, b = f64(got), f64(np.concatenate(parts))
+    assert np.array_equal(np.isnan(a), np.isnan(b))
+    ok = ~np.isnan(a)
+    assert np.linalg.norm((a - b)[ok]) <= 2 * 2.0 ** -8 * np.linalg.norm(b[ok])
+
+
+def check_some_rows(got, q, k, v, position, group, g=None, heads=(0, -1)):
+    n, hk = len(q), k.shape[1]
+    for h in sorted({h % hk for h in heads}):
+        of = slice(h * group, h * group + group)
+        for i in sorted({0, 1, 31 % n, 32 % n, 63 % n, 64 % n, n // 2, n - 2, n - 1}):
+            kv8.check_attention(got[i:i + 1, of], q[i:i + 1, of], k[:position + i + 1, h:h + 1], v[:position + i + 1, h:h + 1],
+                                position + i, None if g is None else g[i:i + 1, of])
+
+
+MANY = [(32, 8, 640, 0), (32, 8, 651, 64), (8, 2, 2570, 100), (28, 4, 740, 37), (256, 256, 80, 0), (256, 256, 81, 64),
+        (200, 200, 129, 5), (8, 1, 2600, 191), (16, 4, 1300, 700)]
+
+
+@pytest.mark.parametrize("hq,hk,rows,position", MANY)
+@pytest.mark.parametrize("gate", [False, True])
+def test_attention_of_many_rows(hq, hk, rows, position, gate):
+    r = rng(hq * 100000 + rows * 1000 + position)
+    cache, (k, v) = filled(r, hk, position + rows, position + rows + 5)
+    q = kv8.keys(r, rows, hq)
+    g = bf16(r.normal(0, 2, (rows, hq, 2 * DIM))) if gate else None
+    got = kv8.attend(cache, q, position, g)
+    assert np.array_equal(got, kv8.attend(cache, q, position, g))
+    same_as_in_parts(got, cache, q, position, g)
+    check_some_rows(got, q, k, v, position, hq // hk, g)
+
+
+@pytest.mark.parametrize("which", ["k", "v", "q"])
+def test_a_nan_in_many_rows(which):
+    r = rng(23)
+    rows, position = 650, 40
+    k, v, q = kv8.keys(r, position + rows, 8), kv8.keys(r, position + rows, 8), kv8.keys(r, rows, 32)
+    want = np.zeros((rows, 32), bool)
+    if which == "q":
+        q[400, 9, 3] = 0x7fc0
+        want[400, 9] = True
+    else:
+        (k if which == "k" else v)[position + 333, 5, 77] = 0xff80
+        want[333:, 20:24] = True
+    cache = kv8.new_cache(8, position + rows + 64, 0xff)
+    kv8.write(cache, k, v, 0)
+    got = kv8.attend(cache, q, position)
+    nan = np.isnan(f32(got))
+    assert np.array_equal(nan.all(2), want) and np.array_equal(nan.any(2), want)
+    same_as_in_parts(got, cache, q, position)
+
+
+@pytest.mark.parametrize("kind", ["growing", "peaked", "powers", "queries", "zero"])
+def test_scores_of_many_rows(kind):
+    r = rng(24)
+    rows, position, heads = 660, 130, 8
+    n = position + rows
+    k, v, q = f32(kv8.keys(r, n, heads)), f32(kv8.keys(r, n, heads)), f32(kv8.keys(r, rows, 32))
+    if kind == "growing":  # each block's scores larger than the last's
+        k = np.abs(k) * (1 + np.arange(n) // 32)[:, None, None] / 8
+        q = np.abs(q)
+    elif kind == "peaked":
+        q *= 20
+    elif kind == "powers":
+        k *= np.exp2(r.integers(-10, 3, n // 64 + 1))[np.arange(n) // 64][:, None, None]
+        v *= np.exp2(r.integers(-10, 3, n // 64 + 1))[np.arange(n) // 64][:, None, None]
+    elif kind == "queries":
+        q *= np.exp2(r.integers(-30, 2, (rows, 32)))[..., None]
+    else:
+        k[:], q[::2] = 0, 0
+    cache = kv8.new_cache(heads, n, 0xff)
+    kv8.write(cache, bf16(k), bf16(v), 0)
+    q = bf16(q)
+    got = kv8.attend(cache, q, position)
+    same_as_in_parts(got, cache, q, position)
+    k, v = (f64(x) for x in kv8.read(cache, 0, n))
+    check_some_rows(got, q, k, v, position, 4)
+
+
 def test_far_behind_in_a_long_cache():
     """Codes of a head beyond 2^31 bytes from the first: capacity 2^22, three heads."""
     cache = kv8.new_cache(3, 1 << 22, 0xff)
