@@ -29,9 +29,11 @@
 namespace es {
 namespace {
 
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kBlockBytes = kKv8Block * kHeadDim;
 constexpr int kNanCode = 0x7f;
@@ -50,6 +52,12 @@ __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0
 __device__ __forceinline__ int pack_e4m3(float a, float b, float c, float d) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+// The same of four values times 2^-e; scale: 2^e.
+__device__ __forceinline__ int pack_e4m3(float scale, float a, float b, float c, float d) {
+  i16x2 r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(i16x2{0, 0}, a, b, scale, false);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
+  return __builtin_bit_cast(int, r);
 }
 // Four codes of a block whose power of two rises by 2^shift; those of a NaN row stay.
 __device__ __forceinline__ int rescale_e4m3(int codes, int shift) {
@@ -109,136 +117,212 @@ __device__ __forceinline__ float2 angle_cs(int position, float inv) {
   return make_float2(c, s);
 }
 
+// The same of a row of K, in 64 bits up to its e4m3: a code is decided by the last
+// bits of a value at a boundary between two (one in four million is within 32 bits'
+// rounding of one). The sum of squares, the root by one Newton step, a dim times its gain
+// (exact in 32 bits, eight significant ones each), the angles.
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const i32x2 w = __builtin_bit_cast(i32x2, v);
+  return __builtin_bit_cast(double, i32x2{__builtin_amdgcn_update_dpp(0, w[0], CTRL, 0xf, 0xf, false),
+                                          __builtin_amdgcn_update_dpp(0, w[1], CTRL, 0xf, 0xf, false)});
+}
+// To 32 bits, an inexact value to the neighbour with an odd last bit: the
+// rounding to e4m3 that follows is that of the value itself.
+__device__ __forceinline__ float to_odd(double v) {
+  const float f = (float)v;
+  const double back = (double)f;
+  const uint32_t bits = __float_as_uint(f), down = bits - (fabs(back) > fabs(v));
+  return back == v || !finite(f) ? f : __uint_as_float(down | 1);
+}
+__device__ __forceinline__ double2 angle_cs64(int position, float inv) {
+  const double x = (double)position * (double)inv, k = rint(x * 0.63661977236758134308);
+  double r = fma(-k, 1.5707963267948966192, x);
+  r = fma(-k, 6.123233995736766036e-17, r);
+  const double z = r * r;
+  double sp = -1.0 / 1307674368000.0, cp = 1.0 / 20922789888000.0;  // Taylor's, |r| <= pi / 4
+  const double st[] = {1.0 / 6227020800.0, -1.0 / 39916800.0, 1.0 / 362880.0, -1.0 / 5040.0, 1.0 / 120.0, -1.0 / 6.0};
+  const double ct[] = {-1.0 / 87178291200.0, 1.0 / 479001600.0, -1.0 / 3628800.0, 1.0 / 40320.0, -1.0 / 720.0, 1.0 / 24.0, -0.5};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) sp = fma(sp, z, st[i]);
+#pragma unroll
+  for (int i = 0; i < 7; ++i) cp = fma(cp, z, ct[i]);
+  const double sn = fma(sp * z, r, r), cs = fma(cp, z, 1.0);
+  const int q = (int)((long long)k & 3);
+  return make_double2(q == 0 ? cs : q == 1 ? -sn : q == 2 ? -cs : sn, q == 0 ? sn : q == 1 ? cs : q == 2 ? -sn : -cs);
+}
+__device__ __forceinline__ void prepare_key(float* x, const float* gain, const double2* cs, int c) {
+  double ss = 0.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) ss = fma((double)x[i], (double)x[i], ss);
+  ss += dpp64<0xB1>(ss);  // xor 1, xor 2, mirrors of 8 and 16 lanes
+  ss += dpp64<0x4E>(ss);
+  ss += dpp64<0x141>(ss);
+  ss += dpp64<0x140>(ss);
+  ss = fma(ss, 1.0 / 256.0, 1e-6);
+  double inv = 1.0f / sqrtf((float)ss);
+  inv = fma(0.5 * inv, fma(-ss * inv, inv, 1.0), inv);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const double y = (double)(x[i] * gain[i]) * inv, other = dpp64<0x4E>(y);
+    const double2 t = cs[(c & 1) * 16 + i];
+    x[i] = to_odd(c < 2 ? fma(y, t.x, -(other * t.y)) : c < 4 ? fma(other, t.y, y * t.x) : y);
+  }
+}
+// One (row, query head): 16 lanes, 16 dims in each.
+__device__ __forceinline__ void prepare_query(const Kv8Prep& p, size_t at, const float* gain, const float2* cs, int chunk) {
+  float x[16];
+  load16(p.q_proj + at * 512 + chunk * 16, x);
+  norm16(x, gain);
+  rotate16(x, cs, chunk);
+  u32x4 o[2];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j >> 2][j & 3] = pack_bf2(x[2 * j], x[2 * j + 1]);
+  u32x4* q = reinterpret_cast<u32x4*>(p.query + at * 256 + chunk * 16);
+  q[0] = o[0];
+  q[1] = o[1];
+}
+
 // ---- writing ----
-// Block of 512 threads = 64 tokens x one KV head: waves 0..3 K, 4..7 V. A
-// thread holds 64 values; the block's largest magnitudes meet in LDS, then K
-// goes out in pieces as it is held (a wave's four tokens make 64-byte lines) and V
-// through LDS, where its tokens and dims change places (padded: 16 bytes
-// every 16 pieces). A piece whose tokens are not all written is read,
-// merged and written back; no other byte changes. Prepare (PREP) makes the K
-// rows from projections by norm and rotation, and further blocks make the
-// queries, eight rows each.
+// Block of 64 tokens x one KV head: half of its waves K, half V. A thread holds 16
+// dims of T tokens; the block's largest magnitudes meet in LDS, then K goes out in
+// pieces as it is held (a wave's four tokens make 64-byte lines) and V through LDS,
+// where its tokens and dims change places (padded: 16 bytes every 16 pieces). A
+// piece whose tokens are not all written is read, merged and written back; no
+// other byte changes. Prepare (PREP) makes the K rows from projections by norm and
+// rotation, two tokens a thread so that their 64-bit work spreads over more waves, and
+// further blocks make the queries, eight rows each.
+// Memory bounds it: 131072 rows of 2 heads, 403 MB, take 80 us (5.0 TB/s, what a
+// large copy reaches). Prepare of 4096 rows, 8 query and 2 KV heads: 63 MB in
+// 15.8 us (13.4 with all of K's arithmetic in 32 bits, 18.3 with four tokens a
+// thread).
 constexpr int kVPad = kBlockBytes + (kBlockBytes / 256) * 16;
 __device__ __forceinline__ int v_lds(int byte) { return byte + (byte >> 8) * 16; }
 
-template <bool PREP>
-__global__ __launch_bounds__(512) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Prep p) {
+template <bool PREP, int T = PREP ? 2 : 4>
+__global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Prep p) {
+  constexpr int kHalf = 1024 / T, kWaves = kHalf / 64;  // threads and waves of K (of V)
   __shared__ __attribute__((aligned(16))) uint8_t vt[kVPad];
-  __shared__ float2 cs[PREP ? 64 : 1][32];
-  __shared__ uint32_t top[2];
-  __shared__ int bad[64];
+  __shared__ double2 cs[PREP ? 64 : 1][32];
+  __shared__ float top[2 * kWaves];       // the waves' largest magnitudes
+  __shared__ uint64_t bad[2 * kWaves][T];  // and their lanes with a NaN or infinity, of their T tokens each
   const int tid = threadIdx.x, chunk = tid & 15;
   const int first = r.position / kKv8Block, nblk = (r.position + r.rows - 1) / kKv8Block - first + 1;
   if (PREP && (int)blockIdx.x >= nblk * c.heads) {
     // queries: 32 (row, head) pairs at a time, 16 lanes each
     const int row0 = ((int)blockIdx.x - nblk * c.heads) * 8, rows = min(8, r.rows - row0);
-    if (tid < rows * 32) cs[tid >> 5][tid & 31] = angle_cs(r.position + row0 + (tid >> 5), p.inv_freq[tid & 31]);
+    float2(*qcs)[32] = reinterpret_cast<float2(*)[32]>(cs);
+    if (tid < rows * 32) qcs[tid >> 5][tid & 31] = angle_cs(r.position + row0 + (tid >> 5), p.inv_freq[tid & 31]);
     float gain[16];
     load16(p.q_gain + chunk * 16, gain);
     __syncthreads();
-    for (int i = tid >> 4; i < rows * p.q_heads; i += 32) {
-      const int row = i / p.q_heads;
-      const size_t at = (size_t)row0 * p.q_heads + i;
-      float x[16];
-      load16(p.q_proj + at * 512 + chunk * 16, x);
-      norm16(x, gain);
-      rotate16(x, cs[row], chunk);
-      u32x4 o[2];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o[j >> 2][j & 3] = pack_bf2(x[2 * j], x[2 * j + 1]);
-      u32x4* q = reinterpret_cast<u32x4*>(p.query + at * 256 + chunk * 16);
-      q[0] = o[0];
-      q[1] = o[1];
-    }
+    for (int i = tid >> 4; i < rows * p.q_heads; i += 2 * kHalf / 16)
+      prepare_query(p, (size_t)row0 * p.q_heads + i, gain, qcs[i / p.q_heads], chunk);
     return;
   }
   const int blk = first + (int)blockIdx.x % nblk, head = (int)blockIdx.x / nblk;
   const int base = blk * kKv8Block;
   const int lo = max(r.position - base, 0), hi = min(r.position + r.rows - base, kKv8Block);
-  const bool is_v = tid >= 256;
-  const int g = (tid & 255) >> 4;
-  if (tid < 2) top[tid] = 0;
-  if (tid < 64) bad[tid] = 0;
-  if (PREP) {
-    for (int i = tid; i < (hi - lo) * 32; i += 512)
-      cs[lo + (i >> 5)][i & 31] = angle_cs(base + lo + (i >> 5), p.inv_freq[i & 31]);
-  }
-  __syncthreads();
+  const bool is_v = tid >= kHalf;
+  const int g = (tid % kHalf) >> 4;
   const size_t store = (size_t)head * c.blocks + blk;
   uint8_t* codes = (is_v ? c.v : c.k) + store * kBlockBytes;
   uint8_t* scale = (is_v ? c.v_scale : c.k_scale) + store;
-  // K: tokens g, g + 16, ..: V: tokens 4 g .. 4 g + 3
-  float x[4][16];
+  // All that is read is on its way before any of it is used. K: tokens g,
+  // g + 64 / T, ..: V: tokens T g .. T g + T - 1. Pieces that keep other tokens' codes:
+  // K's of tokens before the first (if the power of two rises), any of V.
+  u32x4 row[T][2], old[T];
+#pragma unroll
+  for (int i = 0; i < T; ++i) {
+    const int t = min(max(is_v ? T * g + i : 64 / T * i + g, lo), hi - 1);
+    const u32x4* from = reinterpret_cast<const u32x4*>((is_v ? r.v : r.k) + (int64_t)(base + t - r.position) * r.row_stride +
+                                                       (int64_t)head * r.head_stride + chunk * 16);
+    row[i][0] = from[0];
+    row[i][1] = from[1];
+  }
+  const bool whole = lo == 0 && hi == kKv8Block;
+  int before = 255;  // 255: the block holds none
+  if (!whole) {
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+      old[i] = *reinterpret_cast<const u32x4*>(codes + (is_v ? (tid % kHalf + kHalf * i) * 16 : k_piece(64 / T * i + g, chunk)));
+    if (lo > 0) before = (int)*scale;
+  }
+  issue_fence();
+  if (PREP) {
+    for (int i = tid; i < (hi - lo) * 32; i += 2 * kHalf)
+      cs[lo + (i >> 5)][i & 31] = angle_cs64(base + lo + (i >> 5), p.inv_freq[i & 31]);
+    __syncthreads();
+  }
+  float x[T][16];
   float largest = 0.0f;
   float gain[16];
+  uint64_t own_bad[T];
   if (PREP && !is_v) load16(p.k_gain + chunk * 16, gain);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = is_v ? 4 * g + i : 16 * i + g;
+  for (int i = 0; i < T; ++i) {
+    const int t = is_v ? T * g + i : 64 / T * i + g;
     const bool in = t >= lo && t < hi;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) x[i][j] = 0.0f;
-    if (in) {
-      const int64_t at = (int64_t)(base + t - r.position) * r.row_stride + (int64_t)head * r.head_stride + chunk * 16;
-      load16((is_v ? r.v : r.k) + at, x[i]);
-    }
-    if (PREP && !is_v) {
-      norm16(x[i], gain);
-      rotate16(x[i], cs[t], chunk);
-    }
+    unpack16(row[i][0], row[i][1], x[i]);
+    if (PREP && !is_v) prepare_key(x[i], gain, cs[min(max(t, lo), hi - 1)], chunk);
     // magnitudes compare as integers, a NaN or infinity above every number
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < 16; ++j) most = max(most, __float_as_uint(x[i][j]) & 0x7fffffffu);
-    if (most >= 0x7f800000u) {
+    most = in ? most : 0;
+    own_bad[i] = __ballot(most >= 0x7f800000u);
+    if (own_bad[i]) {
       most = 0;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         x[i][j] = finite(x[i][j]) ? x[i][j] : 0.0f;
         most = max(most, __float_as_uint(x[i][j]) & 0x7fffffffu);
       }
-      if (in) bad[t] = 1;
+      most = in ? most : 0;
     }
     largest = fmaxf(largest, __uint_as_float(most));
   }
   largest = wave_max(largest);
-  if ((tid & 63) == 0) atomicMax(&top[is_v], __float_as_uint(largest));  // not negative: ordered as integers
-  __syncthreads();
-  int e = scale_exponent(__uint_as_float(top[is_v]), -127), shift = 0;
-  if (lo > 0) {  // earlier rows of the block stay: its power of two only rises
-    const int before = (int)*scale;
-    if (before != 255) {  // 255: the block holds none
-      e = max(e, before - 127);
-      shift = e + 127 - before;
-    }
+  const int wave = tid >> 6;
+  if ((tid & 63) == 0) {
+    top[wave] = largest;
+#pragma unroll
+    for (int i = 0; i < T; ++i) bad[wave][i] = own_bad[i];
   }
+  __syncthreads();
+  for (int i = 0; i < kWaves; ++i) largest = fmaxf(largest, top[kWaves * is_v + i]);
+  int e = scale_exponent(largest, -127), shift = 0;
+  if (before != 255) {  // earlier rows of the block stay: its power of two only rises
+    e = max(e, before - 127);
+    shift = e + 127 - before;
+  }
+  const float power = __uint_as_float((uint32_t)(e + 127) << 23);
   if (is_v) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = ldexpf(x[i][j], -e);
-      // piece of dim 16 chunk + j, dword token / 16
-      *reinterpret_cast<int*>(&vt[v_lds(v_piece(4 * g, chunk * 16 + j)) + (g >> 2) * 4]) =
-          pack_e4m3(y[0], y[1], y[2], y[3]);
+    for (int j = 0; j < 16; ++j) {  // piece of dim 16 chunk + j, dword token / 16
+      uint8_t* const to = &vt[v_lds(v_piece(T * g, chunk * 16 + j)) + (T * g >> 4) * 4];
+      const int w = pack_e4m3(power, x[0][j], x[1][j], x[T - 2][j], x[T - 1][j]);
+      if constexpr (T == 4)
+        *reinterpret_cast<int*>(to) = w;
+      else
+        reinterpret_cast<uint16_t*>(to)[g & 1] = (uint16_t)w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = 16 * i + g;
+    for (int i = 0; i < T; ++i) {
+      const int t = 64 / T * i + g;
+      u32x4* at = reinterpret_cast<u32x4*>(codes + k_piece(t, chunk));
+      u32x4 o;
       if (t >= lo && t < hi) {
-        u32x4 o;
+        const uint64_t lanes = (own_bad[i] >> ((g & 3) * 16)) | (bad[kWaves + t / (4 * T)][t % T] >> (t / T % 4 * 16));
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          o[j] = bad[t] ? 0x01010101u * kNanCode
-                        : (uint32_t)pack_e4m3(ldexpf(x[i][4 * j], -e), ldexpf(x[i][4 * j + 1], -e),
-                                              ldexpf(x[i][4 * j + 2], -e), ldexpf(x[i][4 * j + 3], -e));
-        *reinterpret_cast<u32x4*>(codes + k_piece(t, chunk)) = o;
+          o[j] = lanes & 0xffff ? 0x01010101u * kNanCode
+                                : (uint32_t)pack_e4m3(power, x[i][4 * j], x[i][4 * j + 1], x[i][4 * j + 2], x[i][4 * j + 3]);
+        *at = o;
       } else if (t < lo && shift > 0) {
-        u32x4* at = reinterpret_cast<u32x4*>(codes + k_piece(t, chunk));
-        u32x4 o = *at;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = (uint32_t)rescale_e4m3((int)o[j], shift);
+        for (int j = 0; j < 4; ++j) o[j] = (uint32_t)rescale_e4m3((int)old[i][j], shift);
         *at = o;
       }
     }
@@ -248,14 +332,14 @@ __global__ __launch_bounds__(512) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Prep p) 
     if (tid == 0) *scale = (uint8_t)(e + 127);
     return;
   }
-  if (tid == 256) *scale = (uint8_t)(e + 127);
+  if (tid == kHalf) *scale = (uint8_t)(e + 127);
 #pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const int piece = (tid & 255) + 256 * n;
+  for (int n = 0; n < T; ++n) {
+    const int piece = tid % kHalf + kHalf * n;
     const int t0 = ((piece >> 6) & 1) * 8 + ((piece >> 5) & 1) * 4;  // its tokens: 16 s + t0 .. + 3, s = 0..3
     u32x4* at = reinterpret_cast<u32x4*>(codes + piece * 16);
     const u32x4 fresh = *reinterpret_cast<const u32x4*>(&vt[v_lds(piece * 16)]);
-    if (lo == 0 && hi == kKv8Block) {
+    if (whole) {
       *at = fresh;
       continue;
     }
@@ -272,13 +356,115 @@ __global__ __launch_bounds__(512) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Prep p) 
       any |= take[s] | keep[s];
     }
     if (!any) continue;
-    u32x4 o = *at;
+    u32x4 o = old[n];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const uint32_t moved = keep[s] ? (uint32_t)rescale_e4m3((int)o[s], shift) : 0;
       o[s] = (o[s] & ~(take[s] | keep[s])) | (fresh[s] & take[s]) | (moved & keep[s]);
     }
     *at = o;
+  }
+}
+
+// One row: a block per head. Every wave holds the whole row (K 16 dims in each of 16
+// lanes, V four a lane) and so both powers of two; the first one writes it, and
+// where a power of two has risen all of them rescale the rows before it. What bounds it is one
+// trip to memory and the fetch of its code: 2.6 us, where the kernel above takes 6.4
+// (prepare: 4.3 and more than 10).
+template <bool PREP>
+__global__ __launch_bounds__(512) void k_kv8_write_one(Kv8 c, Kv8Rows r, Kv8Prep p) {
+  __shared__ double2 cs[PREP ? 32 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, chunk = tid & 15, head = blockIdx.x;
+  float gain[16];
+  if (PREP && head >= c.heads) {
+    const int at = (head - c.heads) * 32 + (tid >> 4);
+    float2* qcs = reinterpret_cast<float2*>(cs);
+    if (tid < 32) qcs[tid] = angle_cs(r.position, p.inv_freq[tid]);
+    load16(p.q_gain + chunk * 16, gain);
+    __syncthreads();
+    if (at < p.q_heads) prepare_query(p, at, gain, qcs, chunk);
+    return;
+  }
+  const int t = r.position % kKv8Block;
+  const size_t store = (size_t)head * c.blocks + r.position / kKv8Block;
+  uint8_t *kcodes = c.k + store * kBlockBytes, *vcodes = c.v + store * kBlockBytes;
+  const u32x4* k = reinterpret_cast<const u32x4*>(r.k + (int64_t)head * r.head_stride + chunk * 16);
+  const u32x4 k0 = k[0], k1 = k[1];
+  const uint2 v = *reinterpret_cast<const uint2*>(r.v + (int64_t)head * r.head_stride + lane * 4);
+  int kbefore = 255, vbefore = 255;  // 255: the block holds none
+  if (t > 0) {
+    kbefore = c.k_scale[store];
+    vbefore = c.v_scale[store];
+  }
+  if (PREP) load16(p.k_gain + chunk * 16, gain);
+  if (PREP && tid < 32) cs[tid] = angle_cs64(r.position, p.inv_freq[tid]);
+  issue_fence();
+  __syncthreads();  // all have read the powers of two (and the angles are there)
+  float x[16], y[4] = {bf_lo(v.x), bf_hi(v.x), bf_lo(v.y), bf_hi(v.y)};
+  unpack16(k0, k1, x);
+  if (PREP) prepare_key(x, gain, cs, chunk);
+  bool bad = false;
+  float kmost = 0.0f, vmost = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    bad |= !finite(x[j]);
+    x[j] = finite(x[j]) ? x[j] : 0.0f;
+    kmost = fmaxf(kmost, fabsf(x[j]));
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    bad |= !finite(y[j]);
+    y[j] = finite(y[j]) ? y[j] : 0.0f;
+    vmost = fmaxf(vmost, fabsf(y[j]));
+  }
+  bad = __any(bad);
+  int ke = scale_exponent(row16_max(kmost), -127), ve = scale_exponent(wave_max(vmost), -127);
+  const int kshift = kbefore == 255 ? 0 : max(ke + 127 - kbefore, 0), vshift = vbefore == 255 ? 0 : max(ve + 127 - vbefore, 0);
+  if (kbefore != 255) ke = max(ke, kbefore - 127);
+  if (vbefore != 255) ve = max(ve, vbefore - 127);
+  if (kshift > 0) {
+    for (int n = 0; n < 2; ++n) {
+      const int token = (tid >> 4) + 32 * n;
+      if (token >= t) break;
+      u32x4* at = reinterpret_cast<u32x4*>(kcodes + k_piece(token, chunk));
+      u32x4 o = *at;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = (uint32_t)rescale_e4m3((int)o[j], kshift);
+      *at = o;
+    }
+  }
+  if (vshift > 0) {
+    for (int n = 0; n < 2; ++n) {
+      const int piece = tid + 512 * n, first = ((piece >> 6) & 1) * 8 + ((piece >> 5) & 1) * 4;
+      uint32_t* at = reinterpret_cast<uint32_t*>(vcodes + piece * 16);
+      const u32x4 w = *reinterpret_cast<const u32x4*>(at);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int left = t - first - 16 * s;  // tokens of these four before the row's
+        const uint32_t o = (uint32_t)rescale_e4m3((int)w[s], vshift);
+        if (left >= 4)
+          at[s] = o;
+        else
+          for (int b = 0; b < left; ++b) reinterpret_cast<uint8_t*>(at + s)[b] = (uint8_t)(o >> (8 * b));
+      }
+    }
+  }
+  if (tid >= 64) return;
+  if (lane < 16) {
+    const float power = __uint_as_float((uint32_t)(ke + 127) << 23);
+    u32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] = bad ? 0x01010101u * kNanCode : (uint32_t)pack_e4m3(power, x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+    *reinterpret_cast<u32x4*>(kcodes + k_piece(t, chunk)) = o;
+  }
+  const uint32_t o = (uint32_t)pack_e4m3(__uint_as_float((uint32_t)(ve + 127) << 23), y[0], y[1], y[2], y[3]);
+  uint8_t* at = vcodes + v_piece(t, lane * 4) + (t >> 4) * 4 + (t & 3);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) at[16 * j] = (uint8_t)(o >> (8 * j));
+  if (lane == 0) {
+    c.k_scale[store] = (uint8_t)(ke + 127);
+    c.v_scale[store] = (uint8_t)(ve + 127);
   }
 }
 
@@ -780,7 +966,6 @@ __device__ __forceinline__ void wait_vmcnt() {
 // all keys each, the same steps interleaved within a wave, took 3530 cycles; eight
 // with 16 queries, both parts as columns of one product, 3560.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short i16x2 __attribute__((ext_vector_type(2)));
 constexpr int kRowPairs = 128, kRowDma = 3;      // DMA instructions of a wave for a block's K (or V)
 constexpr int kKStages = 3, kVStages = 4;
 // LDS: the queries' lower parts, 64 dims of their upper ones, K, V
@@ -1064,13 +1249,21 @@ size_t kv8_attn_scratch_bytes(int q_heads, int kv_heads, int rows) {
 
 hipError_t launch_kv8_write(const Kv8& c, const Kv8Rows& r, hipStream_t s) {
   const int nblk = (r.position + r.rows - 1) / kKv8Block - r.position / kKv8Block + 1;
+  if (r.rows == 1) {
+    hipLaunchKernelGGL(k_kv8_write_one<false>, dim3(c.heads), dim3(512), 0, s, c, r, Kv8Prep{});
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL(k_kv8_write<false>, dim3(nblk * c.heads), dim3(512), 0, s, c, r, Kv8Prep{});
   return hipGetLastError();
 }
 
 hipError_t launch_kv8_prepare(const Kv8& c, const Kv8Rows& r, const Kv8Prep& p, hipStream_t s) {
   const int nblk = (r.position + r.rows - 1) / kKv8Block - r.position / kKv8Block + 1;
-  hipLaunchKernelGGL(k_kv8_write<true>, dim3(nblk * c.heads + (r.rows + 7) / 8), dim3(512), 0, s, c, r, p);
+  if (r.rows == 1) {
+    hipLaunchKernelGGL(k_kv8_write_one<true>, dim3(c.heads + (p.q_heads + 31) / 32), dim3(512), 0, s, c, r, p);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(k_kv8_write<true>, dim3(nblk * c.heads + (r.rows + 7) / 8), dim3(1024), 0, s, c, r, p);
   return hipGetLastError();
 }
 

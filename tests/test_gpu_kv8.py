@@ -125,6 +125,24 @@ def test_a_row_with_a_nan_or_infinity_reads_back_as_nan(bad):
     same_memory(cache, plain)
 
 
+@pytest.mark.parametrize("bad", [None, np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("scale", [0.0, 1e-40, 1e-36, 1.0, 1e30, 3e38])
+def test_rows_one_by_one(scale, bad):
+    """Single rows, each larger or smaller than those before it, over two blocks."""
+    r = rng(30)
+    x = (np.clip(r.normal(0, 0.2, (80, 3, DIM)), -1, 1) * np.exp2(r.integers(-20, 1, (80, 3, 1))) * scale).astype(np.float32)
+    y = np.roll(x[::-1], 7, 2)
+    if bad is not None:
+        x[5, 0, 3] = x[63, 1, 255] = y[40, 1, 200] = y[64, 2, 0] = bad
+    k, v = bf16(x), bf16(y)
+    cache, plain = kv8.new_cache(3, 128), kv8.Plain(3, 128)
+    for i in range(80):
+        kv8.write(cache, k[i:i + 1], v[i:i + 1], i)
+        plain.write(f64(k[i:i + 1]), f64(v[i:i + 1]), i)
+    same_memory(cache, plain)
+    same_values(cache, plain, 0, 80)
+
+
 @pytest.mark.parametrize("row_stride,head_stride", [(1024, 256), (512 + 8, 256), (256, 80 * 256), (264, 8 * 2680), (2000, 768)])
 def test_strides(row_stride, head_stride):
     r = rng(9)
@@ -220,6 +238,26 @@ def test_prepare(hq, hk, position, rows):
     if held is not None:
         for x, y in zip(kv8.read(cache, base, position - base), before):
             assert (np.abs(f64(x) - f64(y)) <= 2.0 ** -4 * np.abs(f64(y)) + 2.0 ** -10 * np.abs(f64(y)).max() / 224).all()
+
+
+@pytest.mark.parametrize("hq,hk", [(8, 2), (5, 5), (40, 1), (70, 10)])
+def test_prepare_one_by_one(hq, hk):
+    """The same queries, bit for bit; K and V within what later powers of two round again."""
+    r = rng(31)
+    q, k, v, qg, kg = projections(r, 70, hq, hk)
+    whole, single = kv8.new_cache(hk, 100), kv8.new_cache(hk, 100)
+    want = prepare(whole, q, k, v, qg, kg, 30)
+    got = [prepare(single, q[i:i + 1], k[i:i + 1], v[i:i + 1], qg, kg, 30 + i) for i in range(70)]
+    assert np.array_equal(np.concatenate(got), want)
+    assert np.array_equal(whole.k_scale.numpy(np.uint8), single.k_scale.numpy(np.uint8))
+    assert np.array_equal(whole.v_scale.numpy(np.uint8), single.v_scale.numpy(np.uint8))
+    power = whole.k_scale.numpy(np.uint8).max(), whole.v_scale.numpy(np.uint8).max()
+    for a, b, e in zip(kv8.read(whole, 30, 70), kv8.read(single, 30, 70), power):
+        a, b = f64(a), f64(b)
+        # half a step each: of the value, or of the subnormals (2^-9) at the power of two; the single ones
+        # twice where theirs has risen in between, more than once only below half a step
+        assert (np.abs(a - b) <= 4 * (2.0 ** -4 * np.abs(a) + 2.0 ** -10 * 2.0 ** (int(e) - 127))).all()
+        assert (a != b).mean() < 0.25
 
 
 def test_prepare_of_a_row_with_nan():
