@@ -916,6 +916,41 @@ __global__ __launch_bounds__(256) void k_kv8_attn_join(Kv8Attn a) {
   a.out[at * 256 + d0 + t] = (uint16_t)f2bf(y);
 }
 
+// The same of many: a wave each, four dims a lane.
+__global__ __launch_bounds__(256) void k_kv8_attn_join_rows(Kv8Attn a) {
+  const int lane = threadIdx.x & 63;
+  const size_t at = (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (at >= (size_t)a.rows * a.q_heads) return;
+  const float* part = a.part + at * a.splits * kKv8PartFloats;
+  const float2 md = lane < a.splits ? *reinterpret_cast<const float2*>(part + (size_t)lane * kKv8PartFloats + 256)
+                                    : make_float2(kNone, 0.0f);
+  const float f = __builtin_amdgcn_exp2f(md.x - wave_max(md.x)), total = tree64(md.y * f);
+  f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < a.splits; s += 4) {
+    f32x4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = *reinterpret_cast<const f32x4*>(part + (size_t)min(s + i, a.splits - 1) * kKv8PartFloats + lane * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s + i >= a.splits) break;
+      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s + i));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = fmaf(x[i][k], w, o[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] /= total;
+  if (a.gate) {
+    const uint2 gate = *reinterpret_cast<const uint2*>(a.gate + at * 512 + 256 + lane * 4);
+    o[0] *= sigmoid(bf_lo(gate.x));
+    o[1] *= sigmoid(bf_hi(gate.x));
+    o[2] *= sigmoid(bf_lo(gate.y));
+    o[3] *= sigmoid(bf_hi(gate.y));
+  }
+  *reinterpret_cast<uint2*>(a.out + at * 256 + lane * 4) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+}
+
 // DMA into LDS: 16 bytes a lane from `uniform` + `lane` of a buffer, piece I of
 // 1024 bytes behind each other, to LDS `to`; or one byte of a buffer to each dword of
 // the 64 at `to`. In assembly, so that the compiler's waits before it reads LDS do
@@ -977,11 +1012,13 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
   __shared__ float scaled[kRowPairs], most[2][kRowPairs], sums[2][kRowPairs];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), upper = wave >> 2, mine = (wave & 3) * 32 + r;
-  // heads in turn, so that an XCD's blocks share a head's keys where the heads
-  // divide the XCDs; the longest ranges of keys first
-  const int head = (int)blockIdx.x % c.heads, tile = a.tiles - 1 - (int)blockIdx.x / c.heads;
+  // heads in turn, then ranges of keys, so that an XCD's blocks share keys where
+  // heads and ranges divide the XCDs; the tiles with most keys first
+  const int head = (int)blockIdx.x % c.heads, rest = (int)blockIdx.x / c.heads;
+  const int split = rest % a.splits, tile = a.tiles - 1 - rest / a.splits;
   const int pairs = a.rows * a.group, end = a.position + a.rows, pair0 = tile * kRowPairs;
-  const int nblk = (a.position + divide(min(pair0 + kRowPairs - 1, pairs - 1), a.group, a.inv_group).x) / kKv8Block + 1;
+  const int all = (a.position + divide(min(pair0 + kRowPairs - 1, pairs - 1), a.group, a.inv_group).x) / kKv8Block + 1;
+  const int b0 = split * all / a.splits, nblk = (split + 1) * all / a.splits - b0;  // the block's own: b0 + 0 .. nblk - 1
   const size_t store = (size_t)head * c.blocks;
   const auto kbuf = buffer_of(c.k + store * kBlockBytes), vbuf = buffer_of(c.v + store * kBlockBytes);
   const auto kscale = buffer_of(c.k_scale + store), vscale = buffer_of(c.v_scale + store);
@@ -991,7 +1028,7 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
   // K and V of block b. One behind the last is fetched as the last, into the stage of
   // a block that is done with, so that every phase's wait counts the same instructions.
   auto issue = [&](int b) {
-    const uint32_t at = min(b, nblk - 1), k = kstage(b), v = vstage(b), to = lds_address(lds) + kRowStages + part;
+    const uint32_t at = b0 + min(b, nblk - 1), k = kstage(b), v = vstage(b), to = lds_address(lds) + kRowStages + part;
     dma16<0>(kbuf, part + lane * 16, at * kBlockBytes, to + k * kBlockBytes);
     dma16<1>(kbuf, part + lane * 16, at * kBlockBytes, to + k * kBlockBytes);
     dma1(kscale, at, lds_address(exponent) + k * 256);
@@ -1078,8 +1115,8 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
       if (t == 4) qh[3] = read(kRowLast + (wave & 3) * 2048);
       if (t % 2 == 0 && t > 0 && t < 8) ql[t / 2] = read(lower + t * 1024);
     }
-    if (b * 64 + 63 > a.position) {  // the causal border
-      const int left = last - b * 64 - 4 * h;
+    if ((b0 + b) * 64 + 63 > a.position) {  // the causal border
+      const int left = last - (b0 + b) * 64 - 4 * h;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1145,7 +1182,7 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
     lds_barrier();
     issue(p + 2);
     issue_fence();
-    if (p == nblk - 1 && nblk * 64 > end) {  // bytes behind the last key may be anything
+    if (p == nblk - 1 && (b0 + nblk) * 64 > end) {  // bytes behind the last key may be anything
       wait_vmcnt<4 * kRowDma>();             // V of the phase's block: each wave clears what it fetched
       int own = lane;
       asm volatile("" : "+v"(own));  // masks are no registers of the loop's
@@ -1155,7 +1192,7 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
         i32x4 w = *at;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int left = end - p * 64 - (16 * k + 8 * i + 4 * (own >> 5));
+          const int left = end - (b0 + p) * 64 - (16 * k + 8 * i + 4 * (own >> 5));
           w[k] &= (int)((1ull << (8 * min(max(left, 0), 4))) - 1);
         }
         *at = w;
@@ -1191,7 +1228,8 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
   lds_barrier();
   const float other = most[1 - upper][mine], ref = fmaxf(m, other);
   float f = __builtin_amdgcn_exp2f(m - ref), fo = __builtin_amdgcn_exp2f(other - ref);
-  const float inv = 16.0f / fmaf(sums[upper][mine], f, sums[1 - upper][mine] * fo);  // 2^kShift
+  const float total = fmaf(sums[0][mine], upper ? fo : f, sums[1][mine] * (upper ? f : fo)) * 0.0625f;  // 2^-kShift
+  const float inv = a.splits > 1 ? 1.0f : 1.0f / total;
   f *= inv;
   fo *= inv;
   const size_t row = (size_t)rq.x * a.q_heads + head * a.group + rq.y;
@@ -1216,6 +1254,15 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
         y[k] = __uint_as_float(w[0]);
         y[4 + k] = __uint_as_float(w[1]);
       }
+      if (a.splits > 1) {
+        float* part = a.part + (row * a.splits + split) * kKv8PartFloats;
+        if (pair0 + mine < pairs) {
+          *reinterpret_cast<f32x4*>(part + upper * 128 + 32 * i + 16 * j + 8 * h) = f32x4{y[0], y[1], y[2], y[3]};
+          *reinterpret_cast<f32x4*>(part + upper * 128 + 32 * i + 16 * j + 8 * h + 4) = f32x4{y[4], y[5], y[6], y[7]};
+          if (i + j + h + upper == 0) *reinterpret_cast<float2*>(part + 256) = make_float2(ref, total);
+        }
+        continue;
+      }
       if (a.gate) {
         const u32x4 gate = *reinterpret_cast<const u32x4*>(a.gate + row * 512 + 256 + upper * 128 + 32 * i + 16 * j + 8 * h);
 #pragma unroll
@@ -1229,21 +1276,61 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
     }
 }
 
-// Whether 128 pairs a block, all keys each, fill enough of the chip's 256 CUs: with
-// 160 full blocks' worth. (At 128 of them, 2048 rows behind 30000 and 2 heads, the
-// form with ranges takes 582 us and this 659; at 176, 700 rows behind 20000 and 8
-// heads, 586 and 443; at 256, 4096 rows behind 28672 and 2 heads, 1145 and 853.)
-bool many(int pairs, int heads) { return (int64_t)pairs * heads >= 160 * kRowPairs; }
 // 16-query tiles of a block: as many as the pairs fill, two at most.
 int few_nt(int pairs) { return pairs <= 16 ? 1 : 2; }
 int few_tiles(int pairs) { return (pairs + 16 * few_nt(pairs) - 1) / (16 * few_nt(pairs)); }
 // Ranges of keys of one call: enough blocks for the chip's 256 CUs.
 int few_ranges(int heads, int tiles) { return max(1, 256 / (heads * tiles)); }
 
+// 128-pair blocks: of one call and one range of keys, and the ranges that scratch is
+// for (three rounds of blocks on the chip's 256 CUs).
+int row_tiles(int pairs) { return (pairs + kRowPairs - 1) / kRowPairs; }
+int row_ranges_most(int tiles) { return tiles >= 256 ? 1 : min(256, 768 / tiles); }
+constexpr int kRowLeast = 96;  // pairs of a head from which on 128-pair blocks come into question
+
+// Estimates in us by which a call takes the one form or the other, fitted to calls of
+// 1000 to 8192 rows at 0 to 60000, 2 to 8 KV heads:
+//   few: 0.575 for 64 keys of a tile of 32 pairs, and 8 for each round of blocks
+//   rows: 1.28 for 64 keys of a tile of 128 with a CU of its own, up to 1.6 when all CUs
+//     are at it (the clock falls), 10 a round; with ranges, writing and joining them
+// (2048 rows behind 30000, 2 KV heads: few 568 us, rows 663 with one range, 435 with
+// two; 128 rows behind 28672: few 49, rows 57 with 32 ranges; 700 rows behind 20000,
+// 8 KV heads: 557, 444 with one, 430 with four; 4096 rows behind none: 111, 107.)
+float few_us(int heads, int pairs, float keys) {
+  const float tiles = (float)few_tiles(pairs) * heads;
+  return tiles * keys / 256 * 0.575f + 8 * ceilf(tiles / 256);
+}
+// most and least: blocks of keys of the last tile and the first
+float rows_us(int tiles, int ranges, int least, int most) {
+  const int n = tiles * ranges, rounds = (n + 255) / 256;
+  const float unit = 1.28f + 0.32f * min(1.0f, n / 256.0f);
+  if (ranges > 1) return rounds * ((float)((most + ranges - 1) / ranges) * unit + 10) + 4 + n * 0.054f;
+  const float mean = 0.5f * (least + most);
+  // with two rounds, as the longest come first, two of the length in the middle follow each other
+  const float keys = rounds == 1 ? most : rounds == 2 ? max((float)most, 2 * (most - (most - least) * 256.0f / n))
+                                                      : max((float)most, mean * n / 256 * (1 + 0.5f / rounds));
+  return keys * unit + 10 * rounds;
+}
+
+// After a launch with ranges of keys. A wave for each output fills the chip from about
+// 1024 on (with 1600 outputs a call takes 21.0 us and 23.0 with blocks, with 800 17.9 and
+// 17.4, with 320 18.6 and 13.8); it holds the weights of 64 ranges.
+hipError_t join(const Kv8Attn& a, hipStream_t s) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  const int outputs = a.rows * a.q_heads;
+  if (outputs >= 1024 && a.splits <= 64)
+    hipLaunchKernelGGL(k_kv8_attn_join_rows, dim3((outputs + 3) / 4), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(k_kv8_attn_join, dim3(outputs * 4), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 size_t kv8_attn_scratch_bytes(int q_heads, int kv_heads, int rows) {
-  const int pairs = rows * (q_heads / kv_heads), most = many(pairs, kv_heads) ? 1 : few_ranges(kv_heads, few_tiles(pairs));
+  const int pairs = rows * (q_heads / kv_heads), few = few_ranges(kv_heads, few_tiles(pairs));
+  const int most = pairs < kRowLeast ? few : max(few, row_ranges_most(row_tiles(pairs) * kv_heads));
   return most < 2 ? 0 : (size_t)rows * q_heads * most * kKv8PartFloats * sizeof(float);
 }
 
@@ -1277,10 +1364,22 @@ hipError_t launch_kv8_read(const Kv8& c, int position, int rows, uint16_t* k, ui
 
 hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
   a.inv_group = 1.0f / (float)a.group;
-  if (many(a.rows * a.group, c.heads)) {
-    a.tiles = (a.rows * a.group + kRowPairs - 1) / kRowPairs;
-    hipLaunchKernelGGL(k_kv8_attn_rows, dim3(a.tiles * c.heads), dim3(512), 0, s, c, a);
-    return hipGetLastError();
+  const int pairs = a.rows * a.group, all = row_tiles(pairs) * c.heads;
+  const int least = a.position / kKv8Block + 1, most = (a.position + a.rows - 1) / kKv8Block + 1;
+  float best = few_us(c.heads, pairs, 0.5f * (least + most));
+  a.splits = 0;
+  for (int rounds = 0; rounds < 4 && pairs >= kRowLeast; ++rounds) {
+    const int ranges = rounds == 0 ? 1 : min(min(256 * rounds / all, row_ranges_most(all)), least);  // none of no keys
+    const float us = ranges > 0 ? rows_us(all, ranges, least, most) : best;
+    if (us < best) {
+      best = us;
+      a.splits = ranges;
+    }
+  }
+  if (a.splits) {
+    a.tiles = row_tiles(pairs);
+    hipLaunchKernelGGL(k_kv8_attn_rows, dim3(all * a.splits), dim3(512), 0, s, c, a);
+    return join(a, s);
   }
   const int tiles = few_tiles(a.rows * a.group), nblk = (a.position + a.rows - 1) / kKv8Block + 1;
   const int ranges = few_ranges(c.heads, tiles);
@@ -1291,10 +1390,7 @@ hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
                        ? (g == 4 ? k_kv8_attn_few<1, 4> : g == 2 ? k_kv8_attn_few<1, 2> : k_kv8_attn_few<1, 1>)
                        : (g == 4 ? k_kv8_attn_few<2, 4> : g == 2 ? k_kv8_attn_few<2, 2> : k_kv8_attn_few<2, 1>);
   hipLaunchKernelGGL(few, dim3(a.splits, tiles, c.heads), dim3(256 * g), 0, s, c, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL(k_kv8_attn_join, dim3(a.rows * a.q_heads * 4), dim3(256), 0, s, a);
-  return hipGetLastError();
+  return join(a, s);
 }
 
 }  // namespace es

@@ -391,10 +391,11 @@ def test_growing_scores_move_the_maximum_in_every_block(rows):
     kv8.check_attention(kv8.attend(cache, q, n - rows), q, k, v, n - rows, spread=False)
 
 
-def same_as_in_parts(got, cache, q, position, g=None, rows=48):
+def same_as_in_parts(got, cache, q, position, g=None):
     """Many rows and the same ones some at a time, which other kernels compute:
     NaN in the same places, and each output's error of 2^-8 at most (root mean square) on
     either side, so one vector of another row would be seen among 20000."""
+    rows = max(1, 64 * cache.heads // q.shape[1])
     parts = [kv8.attend(cache, q[i:i + rows], position + i, None if g is None else g[i:i + rows])
              for i in range(0, len(q), rows)]
     a, b = f64(got), f64(np.concatenate(parts))
@@ -413,7 +414,10 @@ def check_some_rows(got, q, k, v, position, group, g=None, heads=(0, -1)):
 
 
 MANY = [(32, 8, 640, 0), (32, 8, 651, 64), (8, 2, 2570, 100), (28, 4, 740, 37), (256, 256, 80, 0), (256, 256, 81, 64),
-        (200, 200, 129, 5), (8, 1, 2600, 191), (16, 4, 1300, 700)]
+        (200, 200, 129, 5), (8, 1, 2600, 191), (16, 4, 1300, 700),
+        # ranges of keys as well
+        (8, 2, 33, 30000), (8, 2, 300, 20000), (1, 1, 97, 60001), (28, 4, 250, 9000), (5, 5, 700, 12345), (16, 4, 1000, 6000),
+        (8, 2, 100, 4000), (12, 3, 1500, 5050)]
 
 
 @pytest.mark.parametrize("hq,hk,rows,position", MANY)
