@@ -357,8 +357,8 @@ int es_kv8_read(const es_kv8* cache, int position, int rows, uint16_t* k, uint16
  * RoPE(RMSNorm(q head) * q_gain) at its position, and the K and V rows written
  * as es_kv8_write does, K = RoPE(RMSNorm(k head) * k_gain). q_proj [rows,
  * q_heads, 512] (query|gate), k_proj, v_proj [rows, heads, 256], inv_freq 32
- * device floats. Computed in fp32 with one rounding at the end (to bf16 the
- * query, to the codes K), angles in double; eps 1e-6. Pointers 16-byte aligned,
+ * device floats. Queries in fp32 with one rounding to bf16 at the end, angles
+ * reduced in double; K in double up to its codes; eps 1e-6. Pointers 16-byte aligned,
  * rows * q_heads <= 2^22. */
 int es_attn_prepare_rows_kv8(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t* v_proj,
                              const uint16_t* q_gain, const uint16_t* k_gain, const float* inv_freq,

@@ -120,6 +120,7 @@ def attend(cache, query, position, gate=None, stream=None):
     need = int(E.lib().es_attn_kv8_scratch_bytes(hq, cache.heads, rows))
     scratch = E.DeviceBuffer(need + 64)
     scratch.fill(0xff)
+    E.synchronize()  # a stream of its own does not wait for the fills
     E.check(E.lib().es_attn_kv8(dq.ptr, hq, cache.struct, position, rows, dg.ptr if dg else None,
                                 scratch.ptr if need else None, need, out.ptr, stream))
     E.synchronize()

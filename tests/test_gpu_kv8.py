@@ -193,6 +193,7 @@ def prepare(cache, q_proj, k_proj, v_proj, q_gain, k_gain, position, stream=None
     d = [E.DeviceBuffer.from_numpy(x) for x in (q_proj, k_proj, v_proj, q_gain, k_gain, E.rope_inv_freq())]
     query = E.DeviceBuffer(rows * hq * DIM * 2 + 64)
     query.fill(0xa5)
+    E.synchronize()  # a stream of its own does not wait for the fill
     E.check(E.lib().es_attn_prepare_rows_kv8(*(b.ptr for b in d), position, rows, hq, query.ptr, cache.struct, stream))
     E.synchronize()
     got = query.numpy(np.uint16)
