@@ -600,7 +600,14 @@ __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
   __shared__ float scaled[NT * 16], most[G][NT * 16];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), group = __builtin_amdgcn_readfirstlane(tid >> 8);
-  const int split = blockIdx.x, tile = blockIdx.y, head = blockIdx.z;
+  int split = blockIdx.x, tile = blockIdx.y, head = blockIdx.z;
+  if (gridDim.y < (uint32_t)a.tiles) {  // all tiles of a range on one XCD: they share its keys in the L2
+    const int local = split >> 3, range = local / a.tiles * 8 + (split & 7);
+    tile = local % a.tiles;
+    head = range / a.splits;
+    split = range % a.splits;
+    if (head >= c.heads) return;
+  }
   const int pairs = a.rows * a.group, end = a.position + a.rows;  // keys that exist
   const int pair0 = tile * 16 * NT;
   const int tile_last = a.position + divide(min(pair0 + 16 * NT - 1, pairs - 1), a.group, a.inv_group).x;
@@ -1276,11 +1283,12 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
     }
 }
 
-// 16-query tiles of a block: as many as the pairs fill, two at most.
-int few_nt(int pairs) { return pairs <= 16 ? 1 : 2; }
-int few_tiles(int pairs) { return (pairs + 16 * few_nt(pairs) - 1) / (16 * few_nt(pairs)); }
+int few_tiles(int nt, int pairs) { return (pairs + 16 * nt - 1) / (16 * nt); }  // nt: 16-pair tiles of a block
+// Whether the tiles of a range of keys go to one XCD (whose L2 then fetches them
+// once): while groups of that many fill most of its 32 CUs.
+bool few_grouped(int tiles) { return tiles > 1 && tiles <= 10; }
 // Ranges of keys of one call: enough blocks for the chip's 256 CUs.
-int few_ranges(int heads, int tiles) { return max(1, 256 / (heads * tiles)); }
+int few_ranges(int heads, int tiles) { return max(1, few_grouped(tiles) ? 32 / tiles * 8 / heads : 256 / (heads * tiles)); }
 
 // 128-pair blocks: of one call and one range of keys, and the ranges that scratch is
 // for (three rounds of blocks on the chip's 256 CUs).
@@ -1288,23 +1296,25 @@ int row_tiles(int pairs) { return (pairs + kRowPairs - 1) / kRowPairs; }
 int row_ranges_most(int tiles) { return tiles >= 256 ? 1 : min(256, 768 / tiles); }
 constexpr int kRowLeast = 96;  // pairs of a head from which on 128-pair blocks come into question
 
-// Estimates in us by which a call takes the one form or the other, fitted to calls of
-// 1000 to 8192 rows at 0 to 60000, 2 to 8 KV heads:
-//   few: 0.575 for 64 keys of a tile of 32 pairs, and 8 for each round of blocks
-//   rows: 1.28 for 64 keys of a tile of 128 with a CU of its own, up to 1.6 when all CUs
-//     are at it (the clock falls), 10 a round; with ranges, writing and joining them
-// (2048 rows behind 30000, 2 KV heads: few 568 us, rows 663 with one range, 435 with
-// two; 128 rows behind 28672: few 49, rows 57 with 32 ranges; 700 rows behind 20000,
-// 8 KV heads: 557, 444 with one, 430 with four; 4096 rows behind none: 111, 107.)
-float few_us(int heads, int pairs, float keys) {
-  const float tiles = (float)few_tiles(pairs) * heads;
-  return tiles * keys / 256 * 0.575f + 8 * ceilf(tiles / 256);
+// Estimates in us by which a call takes one form or another, fitted to calls of 5 to
+// 8192 rows at 0 to 70000, 1 to 8 KV heads:
+//   few: for 64 keys of 16 pairs 0.42, of 32 together 0.575; for each round of blocks 8 and 13
+//   rows: 1.28 for 64 keys of 128 pairs with a CU of its own, up to 1.6 when all CUs are
+//     at it (the clock falls), 10 a round; with ranges, writing and joining them
+// Measured, 8 query and 2 KV heads where not said otherwise: 500 rows alone 8 us with 16 pairs
+// a block and 14 with 32; 1000 alone 21 and 16; 32 rows behind 70000 43 and 34, rows 47
+// with 128 ranges; 128 behind 28672 57, 49 and rows 57 with 32; 512 behind 28672 few 146,
+// rows 122 with eight; 2048 behind 30000 few 568, rows 663 with one, 435 with two; 700
+// behind 20000, 32 and 8 heads, 557, 444 with one; 4096 alone 111 and 107.
+float few_us(int nt, int heads, int pairs, float keys) {
+  const float tiles = (float)few_tiles(nt, pairs) * heads;
+  return tiles * keys / 256 * (nt == 1 ? 0.42f : 0.575f) + (nt == 1 ? 8 : 13) * ceilf(tiles / 256);
 }
 // most and least: blocks of keys of the last tile and the first
 float rows_us(int tiles, int ranges, int least, int most) {
   const int n = tiles * ranges, rounds = (n + 255) / 256;
   const float unit = 1.28f + 0.32f * min(1.0f, n / 256.0f);
-  if (ranges > 1) return rounds * ((float)((most + ranges - 1) / ranges) * unit + 10) + 4 + n * 0.054f;
+  if (ranges > 1) return rounds * ((float)((most + ranges - 1) / ranges) * unit + 10) + 8 + n * 0.054f;
   const float mean = 0.5f * (least + most);
   // with two rounds, as the longest come first, two of the length in the middle follow each other
   const float keys = rounds == 1 ? most : rounds == 2 ? max((float)most, 2 * (most - (most - least) * 256.0f / n))
@@ -1329,7 +1339,8 @@ hipError_t join(const Kv8Attn& a, hipStream_t s) {
 }  // namespace
 
 size_t kv8_attn_scratch_bytes(int q_heads, int kv_heads, int rows) {
-  const int pairs = rows * (q_heads / kv_heads), few = few_ranges(kv_heads, few_tiles(pairs));
+  const int pairs = rows * (q_heads / kv_heads);
+  const int few = max(few_ranges(kv_heads, few_tiles(1, pairs)), few_ranges(kv_heads, few_tiles(2, pairs)));
   const int most = pairs < kRowLeast ? few : max(few, row_ranges_most(row_tiles(pairs) * kv_heads));
   return most < 2 ? 0 : (size_t)rows * q_heads * most * kKv8PartFloats * sizeof(float);
 }
@@ -1366,7 +1377,9 @@ hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
   a.inv_group = 1.0f / (float)a.group;
   const int pairs = a.rows * a.group, all = row_tiles(pairs) * c.heads;
   const int least = a.position / kKv8Block + 1, most = (a.position + a.rows - 1) / kKv8Block + 1;
-  float best = few_us(c.heads, pairs, 0.5f * (least + most));
+  const float one = few_us(1, c.heads, pairs, 0.5f * (least + most)), two = few_us(2, c.heads, pairs, 0.5f * (least + most));
+  const int nt = one <= two ? 1 : 2;
+  float best = min(one, two);
   a.splits = 0;
   for (int rounds = 0; rounds < 4 && pairs >= kRowLeast; ++rounds) {
     const int ranges = rounds == 0 ? 1 : min(min(256 * rounds / all, row_ranges_most(all)), least);  // none of no keys
@@ -1381,15 +1394,16 @@ hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
     hipLaunchKernelGGL(k_kv8_attn_rows, dim3(all * a.splits), dim3(512), 0, s, c, a);
     return join(a, s);
   }
-  const int tiles = few_tiles(a.rows * a.group), nblk = (a.position + a.rows - 1) / kKv8Block + 1;
-  const int ranges = few_ranges(c.heads, tiles);
-  a.per = (nblk + ranges - 1) / ranges;
-  a.splits = (nblk + a.per - 1) / a.per;
+  const int tiles = few_tiles(nt, pairs), ranges = few_ranges(c.heads, tiles);
+  a.tiles = tiles;
+  a.per = (most + ranges - 1) / ranges;
+  a.splits = (most + a.per - 1) / a.per;
   const int g = a.per >= 4 ? 4 : a.per >= 2 ? 2 : 1;
-  const auto few = few_nt(a.rows * a.group) == 1
+  const auto few = nt == 1
                        ? (g == 4 ? k_kv8_attn_few<1, 4> : g == 2 ? k_kv8_attn_few<1, 2> : k_kv8_attn_few<1, 1>)
                        : (g == 4 ? k_kv8_attn_few<2, 4> : g == 2 ? k_kv8_attn_few<2, 2> : k_kv8_attn_few<2, 1>);
-  hipLaunchKernelGGL(few, dim3(a.splits, tiles, c.heads), dim3(256 * g), 0, s, c, a);
+  const dim3 grid = few_grouped(tiles) ? dim3((a.splits * c.heads + 7) / 8 * 8 * tiles) : dim3(a.splits, tiles, c.heads);
+  hipLaunchKernelGGL(few, grid, dim3(256 * g), 0, s, c, a);
   return join(a, s);
 }
 
