@@ -1396,7 +1396,9 @@ hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
   }
   const int tiles = few_tiles(nt, pairs), ranges = few_ranges(c.heads, tiles);
   a.tiles = tiles;
-  a.per = (most + ranges - 1) / ranges;
+  // Up to 12 blocks of keys one range: the second launch costs more than it saves (one
+  // token behind 100, 500, 750: 6.6, 7.6, 8.7 us, and 9.4 with a block to a range).
+  a.per = most <= 12 ? most : (most + ranges - 1) / ranges;
   a.splits = (most + a.per - 1) / a.per;
   const int g = a.per >= 4 ? 4 : a.per >= 2 ? 2 : 1;
   const auto few = nt == 1
