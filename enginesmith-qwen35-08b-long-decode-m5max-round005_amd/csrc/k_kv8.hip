@@ -193,9 +193,9 @@ __device__ __forceinline__ void prepare_query(const Kv8Prep& p, size_t at, const
 // rotation, two tokens a thread so that their 64-bit work spreads over more waves, and
 // further blocks make the queries, eight rows each.
 // Memory bounds it: 131072 rows of 2 heads, 403 MB, take 80 us (5.0 TB/s, what a
-// large copy reaches). Prepare of 4096 rows, 8 query and 2 KV heads: 63 MB in
-// 15.8 us (13.4 with all of K's arithmetic in 32 bits, 18.3 with four tokens a
-// thread).
+// large copy reaches). Prepare of 4096 rows, 8 query and 2 KV heads: 46 MB in
+// 15.5 us, K's 64-bit arithmetic on half of the CUs (13.4 with all of it in 32
+// bits, 18.3 with four tokens a thread).
 constexpr int kVPad = kBlockBytes + (kBlockBytes / 256) * 16;
 __device__ __forceinline__ int v_lds(int byte) { return byte + (byte >> 8) * 16; }
 
@@ -581,10 +581,10 @@ __device__ __forceinline__ void lds_barrier() {
 // So each byte of K and V enters one wave's registers once, straight from memory,
 // and the probabilities alone pass between waves (through LDS, one barrier a
 // block). What bounds a short context is how many bytes each CU must fetch
-// (measured 20 a cycle): one group of 64 tokens is enough work for a CU there. In
-// a long one 16 waves of a CU have 4 to 8 KB each on their way: the next block's K
-// is fetched as soon as this one's products have read it, its V likewise. A
-// group's waves share the exponent's reference of a query; it moves when a score
+// (measured 20 a cycle), a long one memory (131072 tokens, 2 heads: 134 MB in 25 us,
+// 5.3 TB/s), many queries the products and exponentials of four waves on a SIMD.
+// The next block's K is fetched as soon as this one's products have read it, its V
+// likewise: 32 KB of a group on their way. A group's waves share the exponent's reference of a query; it moves when a score
 // of any passes it by more than kSlack.
 // The bound of 1024 threads holds for every G: it keeps the compiler to the 128
 // vector registers of 16 waves a CU and off the accumulator registers.
@@ -1400,7 +1400,13 @@ hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
   // token behind 100, 500, 750: 6.6, 7.6, 8.7 us, and 9.4 with a block to a range).
   a.per = most <= 12 ? most : (most + ranges - 1) / ranges;
   a.splits = (most + a.per - 1) / a.per;
-  const int g = a.per >= 4 ? 4 : a.per >= 2 ? 2 : 1;
+  // Groups of four waves a block. Where one tile reads its keys alone memory sets the time
+  // and one group fetches as fast as four, with nothing to join; many tiles of a range, or the
+  // one range of a short context, have work for all 16 waves. (4, 2 and 1 groups, 2 KV heads:
+  // one token behind 16000 10.4, 9.8, 8.9 us; 6 rows behind 32000, two tiles, 13.2, 12.3,
+  // 12.8; 40 behind 20000, ten, 20.4, 21.8, 25.5; 1000 rows alone 16.2, 17.2, 21.9.)
+  const int most_groups = a.splits == 1 || tiles > 5 ? 4 : tiles > 1 ? 2 : 1;
+  const int g = min(most_groups, a.per >= 4 ? 4 : a.per >= 2 ? 2 : 1);
   const auto few = nt == 1
                        ? (g == 4 ? k_kv8_attn_few<1, 4> : g == 2 ? k_kv8_attn_few<1, 2> : k_kv8_attn_few<1, 1>)
                        : (g == 4 ? k_kv8_attn_few<2, 4> : g == 2 ? k_kv8_attn_few<2, 2> : k_kv8_attn_few<2, 1>);
