@@ -359,20 +359,22 @@ int es_kv8_read(const es_kv8* cache, int position, int rows, uint16_t* k, uint16
  * q_heads, 512] (query|gate), k_proj, v_proj [rows, heads, 256], inv_freq 32
  * device floats. Queries in fp32 with one rounding to bf16 at the end, angles
  * reduced in double; K in double up to its codes; eps 1e-6. Pointers 16-byte aligned,
- * rows * q_heads <= 2^22. */
+ * query apart from the projections, rows * q_heads <= 2^22. */
 int es_attn_prepare_rows_kv8(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t* v_proj,
                              const uint16_t* q_gain, const uint16_t* k_gain, const float* inv_freq,
                              int position, int rows, int q_heads, uint16_t* query, const es_kv8* cache,
                              void* stream);
 
 /* Scratch bytes of es_attn_kv8 for these heads and this number of rows, at any
- * position and capacity (0 where it needs none, or for bad arguments). */
+ * position and capacity (0 where it needs none, or for bad arguments). More
+ * rows can need less: a buffer for several numbers takes the largest. */
 size_t es_attn_kv8_scratch_bytes(int q_heads, int kv_heads, int rows);
 
 /* Causal attention of `rows` queries at positions position .. position+rows-1
  * over this cache, one token or many: row r attends to positions 0 ..
  * position+r; o = softmax(q.K^T / 16) V in fp32 (queries exact, probabilities
- * to 8 significant bits, products on 8-bit matrix instructions), out [rows,
+ * to 8 significant bits, products on 8-bit matrix instructions, sums of values
+ * times up to 2^8 in fp32), out [rows,
  * q_heads, 256] = bf16(o), or with gate (q_proj rows [rows, q_heads, 512],
  * optional) bf16(o * sigmoid(gate)), gate the second half of each head. query
  * [rows, q_heads, 256] bf16. Pointers 16-byte aligned, rows * q_heads <= 2^22.

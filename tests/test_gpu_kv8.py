@@ -497,6 +497,59 @@ def test_far_behind_in_a_long_cache():
     kv8.check_attention(kv8.attend(cache, q, n - 1), q, *(f64(x) for x in kv8.read(cache, 0, n)), n - 1)
 
 
+@pytest.mark.parametrize("rows,hq", [(1, 6), (7, 15), (200, 6)])
+def test_all_keys_of_a_long_cache(rows, hq):
+    """2^22 keys of three heads, in blocks beyond 2^31 bytes. Keys of zeros weigh all
+    values alike: one row everywhere but for the last ones, which are of their own."""
+    cache = kv8.new_cache(3, 1 << 22, 0xff)
+    r = rng(32)
+    n = 1 << 22
+    k, v = np.zeros((1, 3, DIM), np.uint16), kv8.keys(r, 1, 3)
+    dk, dv = E.DeviceBuffer.from_numpy(k), E.DeviceBuffer.from_numpy(v)
+    E.check(E.lib().es_kv8_write(cache.struct, dk.ptr, dv.ptr, 0, DIM, 0, n, None))
+    E.synchronize()
+    last = bf16(f32(kv8.keys(r, 300, 3)) * 2.0 ** 14)
+    kv8.write(cache, np.zeros((300, 3, DIM), np.uint16), last, n - 300)
+    first, last = (f64(kv8.read(cache, at, m)[1]) for at, m in ((0, 1), (n - 300, 300)))
+    got = f64(kv8.attend(cache, kv8.keys(r, rows, hq), n - rows))
+    # the block of rows before the last 300 has their power of two, and reads back smaller values
+    edge = f64(kv8.read(cache, n - 320, 20)[1])
+    total = first[0] * (n - 320) + edge.sum(0)
+    for i in range(rows):
+        seen = 300 - rows + 1 + i
+        want = (total + last[:seen].sum(0)) / (n - 300 + seen)
+        size = (np.abs(first[0]) * (n - 320) + np.abs(edge).sum(0) + np.abs(last[:seen]).sum(0)) / n
+        # 2^16 blocks added up in 32 bits at most, addends aligned to 2^-12 of the largest, bf16
+        off = (2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -12) * size).repeat(hq // 3, 0)
+        assert (np.abs(got[i] - want.repeat(hq // 3, 0)) <= off).all(), i
+
+
+def test_outputs_to_the_last_of_two_gigabytes():
+    """rows * q_heads = 2^22: every head has the same keys, so a few rows of a few heads say it all."""
+    torch.manual_seed(4)
+    heads, rows = 256, 16384
+    cache = E.DeviceKV8(heads, rows)
+    r = rng(33)
+    k, v = kv8.keys(r, rows, 1), kv8.keys(r, rows, 1)
+    dk, dv = E.DeviceBuffer.from_numpy(k), E.DeviceBuffer.from_numpy(v)
+    E.check(E.lib().es_kv8_write(cache.struct, dk.ptr, dv.ptr, DIM, 0, 0, rows, None))
+    q = torch.randn(rows, heads, DIM, device="cuda", dtype=torch.bfloat16)
+    out = torch.full((rows + 1, heads, DIM), 7.0, device="cuda", dtype=torch.bfloat16)
+    need = int(E.lib().es_attn_kv8_scratch_bytes(heads, heads, rows))
+    scratch = torch.empty(max(need, 16), device="cuda", dtype=torch.uint8)
+    torch.cuda.synchronize()
+    E.check(E.lib().es_attn_kv8(q.data_ptr(), heads, cache.struct, 0, rows, None, scratch.data_ptr(), need, out.data_ptr(),
+                                None))
+    torch.cuda.synchronize()
+    assert (out[rows] == 7.0).all()
+    assert bool(torch.isfinite(out).all())
+    k, v = (f64(x)[:, :1] for x in kv8.read(cache, 0, rows))
+    for i in (0, 63, 8191, rows - 1):
+        for h in (0, 101, 255):
+            a, b = (x[i:i + 1, h:h + 1].contiguous().view(torch.int16).cpu().numpy().view(np.uint16) for x in (out, q))
+            kv8.check_attention(a, b, k[:i + 1], v[:i + 1], i)
+
+
 # --------------------------------------------------------------- together
 def test_a_prompt_and_tokens_after_it():
     """Prompt chunks and single tokens, prepared and attended in order on a stream
@@ -561,5 +614,41 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         got = out.clone()
         step(other, eager, None)
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager)
+
+
+@pytest.mark.parametrize("hq,hk,rows,n", [(32, 8, 660, 0), (8, 2, 300, 20000), (8, 2, 9, 30000), (8, 2, 1, 5000)])
+def test_attention_captured_and_replayed(hq, hk, rows, n):
+    """Each form of the kernels, ranges and their joining: replays on new queries, among
+    eager calls that use another scratch, equal the eager results."""
+    torch.manual_seed(5)
+    lib = E.lib()
+
+    def bf(*shape):
+        return torch.randn(*shape, device="cuda").to(torch.bfloat16)
+
+    cache = E.DeviceKV8(hk, n + rows)
+    k, v = bf(n + rows, hk, 256), bf(n + rows, hk, 256)
+    torch.cuda.synchronize()
+    E.check(lib.es_kv8_write(cache.struct, k.data_ptr(), v.data_ptr(), hk * 256, 256, 0, n + rows, None))
+    E.synchronize()
+    size = int(lib.es_attn_kv8_scratch_bytes(hq, hk, rows))
+    scratch, other = (torch.empty(max(size, 16), dtype=torch.uint8, device="cuda") for _ in range(2))
+    q, out, eager = bf(rows, hq, 256), bf(rows, hq, 256), bf(rows, hq, 256)
+
+    def attend(work, to, stream):
+        E.check(lib.es_attn_kv8(q.data_ptr(), hq, cache.struct, n, rows, None, work.data_ptr(), size, to.data_ptr(), stream))
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(scratch, out, torch.cuda.current_stream().cuda_stream)
+    for _ in range(4):
+        q.copy_(torch.randn_like(q, dtype=torch.float32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        attend(other, eager, None)
         torch.cuda.synchronize()
         assert torch.equal(got, eager)
