@@ -963,13 +963,14 @@ __global__ __launch_bounds__(256) void k_kv8_attn_join_rows(Kv8Attn a) {
 // the 64 at `to`. In assembly, so that the compiler's waits before it reads LDS do
 // not count these (the kernel's own do); a buffer spans all 32-bit offsets: what is
 // in range is the caller's affair.
-typedef __attribute__((address_space(3))) void* lptr_t;
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 __device__ __forceinline__ u32x4 buffer_of(const uint8_t* base) {
   return u32x4{(uint32_t)(uintptr_t)base, (uint32_t)((uintptr_t)base >> 32), 0xffffffffu, 0x00020000u};
 }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved, and clobbered here
 template <int I>
 __device__ __forceinline__ void dma16(u32x4 from, uint32_t lane, uint32_t uniform, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen offset:%4 lds"
@@ -983,6 +984,7 @@ __device__ __forceinline__ void dma1(u32x4 from, uint32_t uniform, uint32_t to) 
                : "s"(to), "s"(from), "s"(uniform)
                : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
