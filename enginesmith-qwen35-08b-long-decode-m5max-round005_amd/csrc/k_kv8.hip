@@ -192,7 +192,7 @@ __device__ __forceinline__ void prepare_query(const Kv8Prep& p, size_t at, const
 // other byte changes. Prepare (PREP) makes the K rows from projections by norm and
 // rotation, two tokens a thread so that their 64-bit work spreads over more waves, and
 // further blocks make the queries, eight rows each.
-// Memory bounds it: 131072 rows of 2 heads, 403 MB, take 80 us (5.0 TB/s, what a
+// Memory bounds it: 131072 rows of 2 heads, 403 MB, take 77 us (5.2 TB/s, what a
 // large copy reaches). Prepare of 4096 rows, 8 query and 2 KV heads: 46 MB in
 // 15.5 us, K's 64-bit arithmetic on half of the CUs (13.4 with all of it in 32
 // bits, 18.3 with four tokens a thread).
@@ -237,8 +237,8 @@ __global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Pre
     const int t = min(max(is_v ? T * g + i : 64 / T * i + g, lo), hi - 1);
     const u32x4* from = reinterpret_cast<const u32x4*>((is_v ? r.v : r.k) + (int64_t)(base + t - r.position) * r.row_stride +
                                                        (int64_t)head * r.head_stride + chunk * 16);
-    row[i][0] = from[0];
-    row[i][1] = from[1];
+    row[i][0] = __builtin_nontemporal_load(from);  // read once
+    row[i][1] = __builtin_nontemporal_load(from + 1);
   }
   const bool whole = lo == 0 && hi == kKv8Block;
   int before = 255;  // 255: the block holds none
@@ -254,7 +254,14 @@ __global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Pre
       cs[lo + (i >> 5)][i & 31] = angle_cs64(base + lo + (i >> 5), p.inv_freq[i & 31]);
     __syncthreads();
   }
-  float x[T][16];
+  // The rows stay as bf16 (84 registers and three blocks a CU instead of 107 and two: 77 us
+  // instead of 85 for the 131072 above), prepared ones become fp32.
+  float x[PREP ? T : 1][16];
+  auto value = [&](int i, int j) {
+    if constexpr (PREP) return x[i][j];
+    const uint32_t u = row[i][j >> 3][(j >> 1) & 3];
+    return j & 1 ? bf_hi(u) : bf_lo(u);
+  };
   float largest = 0.0f;
   float gain[16];
   uint64_t own_bad[T];
@@ -263,20 +270,25 @@ __global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Pre
   for (int i = 0; i < T; ++i) {
     const int t = is_v ? T * g + i : 64 / T * i + g;
     const bool in = t >= lo && t < hi;
-    unpack16(row[i][0], row[i][1], x[i]);
-    if (PREP && !is_v) prepare_key(x[i], gain, cs[min(max(t, lo), hi - 1)], chunk);
+    if (PREP) unpack16(row[i][0], row[i][1], x[PREP ? i : 0]);
+    if (PREP && !is_v) prepare_key(x[PREP ? i : 0], gain, cs[min(max(t, lo), hi - 1)], chunk);
     // magnitudes compare as integers, a NaN or infinity above every number
     uint32_t most = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) most = max(most, __float_as_uint(x[i][j]) & 0x7fffffffu);
+    for (int j = 0; j < 16; ++j) most = max(most, __float_as_uint(value(i, j)) & 0x7fffffffu);
     most = in ? most : 0;
     own_bad[i] = __ballot(most >= 0x7f800000u);
     if (own_bad[i]) {
       most = 0;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        x[i][j] = finite(x[i][j]) ? x[i][j] : 0.0f;
-        most = max(most, __float_as_uint(x[i][j]) & 0x7fffffffu);
+        if (!finite(value(i, j))) {
+          if constexpr (PREP)
+            x[i][j] = 0.0f;
+          else
+            row[i][j >> 3][(j >> 1) & 3] &= j & 1 ? 0xffffu : 0xffff0000u;
+        }
+        most = max(most, __float_as_uint(value(i, j)) & 0x7fffffffu);
       }
       most = in ? most : 0;
     }
@@ -301,7 +313,7 @@ __global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Pre
 #pragma unroll
     for (int j = 0; j < 16; ++j) {  // piece of dim 16 chunk + j, dword token / 16
       uint8_t* const to = &vt[v_lds(v_piece(T * g, chunk * 16 + j)) + (T * g >> 4) * 4];
-      const int w = pack_e4m3(power, x[0][j], x[1][j], x[T - 2][j], x[T - 1][j]);
+      const int w = pack_e4m3(power, value(0, j), value(1, j), value(T - 2, j), value(T - 1, j));
       if constexpr (T == 4)
         *reinterpret_cast<int*>(to) = w;
       else
@@ -318,7 +330,7 @@ __global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Pre
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           o[j] = lanes & 0xffff ? 0x01010101u * kNanCode
-                                : (uint32_t)pack_e4m3(power, x[i][4 * j], x[i][4 * j + 1], x[i][4 * j + 2], x[i][4 * j + 3]);
+                                : (uint32_t)pack_e4m3(power, value(i, 4 * j), value(i, 4 * j + 1), value(i, 4 * j + 2), value(i, 4 * j + 3));
         *at = o;
       } else if (t < lo && shift > 0) {
 #pragma unroll
