@@ -1304,22 +1304,27 @@ bool few_grouped(int tiles) { return tiles > 1 && tiles <= 10; }
 // Ranges of keys of one call: enough blocks for the chip's 256 CUs.
 int few_ranges(int heads, int tiles) { return max(1, few_grouped(tiles) ? 32 / tiles * 8 / heads : 256 / (heads * tiles)); }
 
-// 128-pair blocks: of one call and one range of keys, and the ranges that scratch is
-// for (three rounds of blocks on the chip's 256 CUs).
+// 128-pair blocks of a head; and of all heads' the ranges of keys that fill `rounds`
+// rounds of blocks on the chip's 256 CUs, 1 if they end no sooner than whole rounds do.
 int row_tiles(int pairs) { return (pairs + kRowPairs - 1) / kRowPairs; }
-int row_ranges_most(int tiles) { return tiles >= 256 ? 1 : min(256, 768 / tiles); }
+constexpr int kRowRounds = 4;
+int row_ranges(int tiles, int rounds) {
+  const int ranges = min(256, 256 * rounds / tiles);
+  return ranges > 1 && (tiles * ranges + 255) / 256 < (tiles + 255) / 256 * ranges ? ranges : 1;
+}
 constexpr int kRowLeast = 96;  // pairs of a head from which on 128-pair blocks come into question
 
 // Estimates in us by which a call takes one form or another, fitted to calls of 5 to
 // 8192 rows at 0 to 70000, 1 to 8 KV heads:
 //   few: for 64 keys of 16 pairs 0.42, of 32 together 0.575; for each round of blocks 8 and 13
 //   rows: 1.28 for 64 keys of 128 pairs with a CU of its own, up to 1.6 when all CUs are
-//     at it (the clock falls), 10 a round; with ranges, writing and joining them
+//     at it (the clock falls), 10 a round; with ranges 6, and writing and joining them
 // Measured, 8 query and 2 KV heads where not said otherwise: 500 rows alone 8 us with 16 pairs
 // a block and 14 with 32; 1000 alone 21 and 16; 32 rows behind 70000 43 and 34, rows 47
 // with 128 ranges; 128 behind 28672 57, 49 and rows 57 with 32; 512 behind 28672 few 146,
-// rows 122 with eight; 2048 behind 30000 few 568, rows 663 with one, 435 with two; 700
-// behind 20000, 32 and 8 heads, 557, 444 with one; 4096 alone 111 and 107.
+// rows 119 with eight; 2048 behind 30000 few 568, rows 663 with one, 435 with two; 4200
+// behind 28672 few 1273, rows 1304 with one and 1010 with three; 700 behind 20000, 32 and
+// 8 heads, 557, 444 with one; 4096 alone 111 and 107.
 float few_us(int nt, int heads, int pairs, float keys) {
   const float tiles = (float)few_tiles(nt, pairs) * heads;
   return tiles * keys / 256 * (nt == 1 ? 0.42f : 0.575f) + (nt == 1 ? 8 : 13) * ceilf(tiles / 256);
@@ -1327,12 +1332,12 @@ float few_us(int nt, int heads, int pairs, float keys) {
 // most and least: blocks of keys of the last tile and the first
 float rows_us(int tiles, int ranges, int least, int most) {
   const int n = tiles * ranges, rounds = (n + 255) / 256;
-  const float unit = 1.28f + 0.32f * min(1.0f, n / 256.0f);
-  if (ranges > 1) return rounds * ((float)((most + ranges - 1) / ranges) * unit + 10) + 8 + n * 0.054f;
+  const float unit = 1.28f + 0.32f * fminf(1.0f, n / 256.0f);
   const float mean = 0.5f * (least + most);
+  if (ranges > 1) return rounds * (ceilf((rounds == 1 ? most : mean) / ranges) * unit + 6) + 4 + n * 0.054f;
   // with two rounds, as the longest come first, two of the length in the middle follow each other
-  const float keys = rounds == 1 ? most : rounds == 2 ? max((float)most, 2 * (most - (most - least) * 256.0f / n))
-                                                      : max((float)most, mean * n / 256 * (1 + 0.5f / rounds));
+  const float keys = rounds == 1 ? most : rounds == 2 ? fmaxf(most, 2 * (most - (most - least) * 256.0f / n))
+                                                      : fmaxf(most, mean * n / 256 * (1 + 0.5f / rounds));
   return keys * unit + 10 * rounds;
 }
 
@@ -1355,7 +1360,9 @@ hipError_t join(const Kv8Attn& a, hipStream_t s) {
 size_t kv8_attn_scratch_bytes(int q_heads, int kv_heads, int rows) {
   const int pairs = rows * (q_heads / kv_heads);
   const int few = max(few_ranges(kv_heads, few_tiles(1, pairs)), few_ranges(kv_heads, few_tiles(2, pairs)));
-  const int most = pairs < kRowLeast ? few : max(few, row_ranges_most(row_tiles(pairs) * kv_heads));
+  int most = few;
+  for (int rounds = 1; rounds <= kRowRounds && pairs >= kRowLeast; ++rounds)
+    most = max(most, row_ranges(row_tiles(pairs) * kv_heads, rounds));
   return most < 2 ? 0 : (size_t)rows * q_heads * most * kKv8PartFloats * sizeof(float);
 }
 
@@ -1393,11 +1400,11 @@ hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
   const int least = a.position / kKv8Block + 1, most = (a.position + a.rows - 1) / kKv8Block + 1;
   const float one = few_us(1, c.heads, pairs, 0.5f * (least + most)), two = few_us(2, c.heads, pairs, 0.5f * (least + most));
   const int nt = one <= two ? 1 : 2;
-  float best = min(one, two);
+  float best = fminf(one, two);
   a.splits = 0;
-  for (int rounds = 0; rounds < 4 && pairs >= kRowLeast; ++rounds) {
-    const int ranges = rounds == 0 ? 1 : min(min(256 * rounds / all, row_ranges_most(all)), least);  // none of no keys
-    const float us = ranges > 0 ? rows_us(all, ranges, least, most) : best;
+  for (int rounds = 0; rounds <= kRowRounds && pairs >= kRowLeast; ++rounds) {
+    const int ranges = rounds == 0 ? 1 : min(row_ranges(all, rounds), least);  // none of no keys
+    const float us = rows_us(all, ranges, least, most);
     if (us < best) {
       best = us;
       a.splits = ranges;
