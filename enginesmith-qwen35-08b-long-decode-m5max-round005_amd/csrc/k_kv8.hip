@@ -546,7 +546,7 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8 c, int position, int rows,
 // ---- attention ----
 constexpr float kLog2e = 1.44269504088896341f;
 // Four values (at most 448, of eight significant bits) in two parts: the nearest
-// codes, and the codes of 16 times the rest.
+// codes, and the codes of 16 times the rest (which below 2^-6 rounds by 2^-14 at most).
 __device__ __forceinline__ int2 split_e4m3(float a, float b, float c, float d) {
   const int h = pack_e4m3(a, b, c, d);
   const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), v = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);

@@ -372,9 +372,9 @@ size_t es_attn_kv8_scratch_bytes(int q_heads, int kv_heads, int rows);
 
 /* Causal attention of `rows` queries at positions position .. position+rows-1
  * over this cache, one token or many: row r attends to positions 0 ..
- * position+r; o = softmax(q.K^T / 16) V in fp32 (queries exact, probabilities
- * to 8 significant bits, products on 8-bit matrix instructions, sums of values
- * times up to 2^8 in fp32), out [rows,
+ * position+r; o = softmax(q.K^T / 16) V in fp32 (queries exact to 2^-21 of a
+ * head's largest magnitude, probabilities to 8 significant bits, products on
+ * 8-bit matrix instructions, sums of values times up to 2^8), out [rows,
  * q_heads, 256] = bf16(o), or with gate (q_proj rows [rows, q_heads, 512],
  * optional) bf16(o * sigmoid(gate)), gate the second half of each head. query
  * [rows, q_heads, 256] bf16. Pointers 16-byte aligned, rows * q_heads <= 2^22.
