@@ -151,7 +151,8 @@ __device__ __forceinline__ double2 angle_cs64(int position, float inv) {
   const int q = (int)((long long)k & 3);
   return make_double2(q == 0 ? cs : q == 1 ? -sn : q == 2 ? -cs : sn, q == 0 ? sn : q == 1 ? cs : q == 2 ? -sn : -cs);
 }
-__device__ __forceinline__ void prepare_key(float* x, const float* gain, const double2* cs, int c) {
+// cs: 32 (cos, sin) of the token, then somewhere 16 of angle 0 for the lanes that hold no pair.
+__device__ __forceinline__ void prepare_key(float* x, const float* gain, const double2* cs, const double2* none, int c) {
   double ss = 0.0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) ss = fma((double)x[i], (double)x[i], ss);
@@ -160,13 +161,13 @@ __device__ __forceinline__ void prepare_key(float* x, const float* gain, const d
   ss += dpp64<0x141>(ss);
   ss += dpp64<0x140>(ss);
   ss = fma(ss, 1.0 / 256.0, 1e-6);
-  double inv = 1.0f / sqrtf((float)ss);
+  double inv = __builtin_amdgcn_rsq(ss);
   inv = fma(0.5 * inv, fma(-ss * inv, inv, 1.0), inv);
+  const double2* t = c < 4 ? cs + (c & 1) * 16 : none;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const double y = (double)(x[i] * gain[i]) * inv, other = dpp64<0x4E>(y);
-    const double2 t = cs[(c & 1) * 16 + i];
-    x[i] = to_odd(c < 2 ? fma(y, t.x, -(other * t.y)) : c < 4 ? fma(other, t.y, y * t.x) : y);
+    x[i] = to_odd(fma(y, t[i].x, (c < 2 ? -other : other) * t[i].y));
   }
 }
 // One (row, query head): 16 lanes, 16 dims in each.
@@ -194,8 +195,8 @@ __device__ __forceinline__ void prepare_query(const Kv8Prep& p, size_t at, const
 // further blocks make the queries, eight rows each.
 // Memory bounds it: 131072 rows of 2 heads, 403 MB, take 77 us (5.2 TB/s, what a
 // large copy reaches). Prepare of 4096 rows, 8 query and 2 KV heads: 46 MB in
-// 15.5 us, K's 64-bit arithmetic on half of the CUs (13.4 with all of it in 32
-// bits, 18.3 with four tokens a thread).
+// 15 us (alone the queries 10.4, the keys with their 64-bit arithmetic on half of the
+// CUs 12).
 constexpr int kVPad = kBlockBytes + (kBlockBytes / 256) * 16;
 __device__ __forceinline__ int v_lds(int byte) { return byte + (byte >> 8) * 16; }
 
@@ -203,7 +204,7 @@ template <bool PREP, int T = PREP ? 2 : 4>
 __global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Prep p) {
   constexpr int kHalf = 1024 / T, kWaves = kHalf / 64;  // threads and waves of K (of V)
   __shared__ __attribute__((aligned(16))) uint8_t vt[kVPad];
-  __shared__ double2 cs[PREP ? 64 : 1][32];
+  __shared__ double2 cs[PREP ? 64 : 1][32], none[PREP ? 16 : 1];
   __shared__ float top[2 * kWaves];       // the waves' largest magnitudes
   __shared__ uint64_t bad[2 * kWaves][T];  // and their lanes with a NaN or infinity, of their T tokens each
   const int tid = threadIdx.x, chunk = tid & 15;
@@ -252,6 +253,7 @@ __global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Pre
   if (PREP) {
     for (int i = tid; i < (hi - lo) * 32; i += 2 * kHalf)
       cs[lo + (i >> 5)][i & 31] = angle_cs64(base + lo + (i >> 5), p.inv_freq[i & 31]);
+    if (tid < 16) none[tid] = make_double2(1.0, 0.0);
     __syncthreads();
   }
   // The rows stay as bf16 (84 registers and three blocks a CU instead of 107 and two: 77 us
@@ -271,7 +273,7 @@ __global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Pre
     const int t = is_v ? T * g + i : 64 / T * i + g;
     const bool in = t >= lo && t < hi;
     if (PREP) unpack16(row[i][0], row[i][1], x[PREP ? i : 0]);
-    if (PREP && !is_v) prepare_key(x[PREP ? i : 0], gain, cs[min(max(t, lo), hi - 1)], chunk);
+    if (PREP && !is_v) prepare_key(x[PREP ? i : 0], gain, cs[min(max(t, lo), hi - 1)], none, chunk);
     // magnitudes compare as integers, a NaN or infinity above every number
     uint32_t most = 0;
 #pragma unroll
@@ -382,10 +384,10 @@ __global__ __launch_bounds__(2048 / T) void k_kv8_write(Kv8 c, Kv8Rows r, Kv8Pre
 // lanes, V four a lane) and so both powers of two; the first one writes it, and
 // where a power of two has risen all of them rescale the rows before it. What bounds it is one
 // trip to memory and the fetch of its code: 2.6 us, where the kernel above takes 6.4
-// (prepare: 4.3 and more than 10).
+// (prepare: 3.9 and more than 10).
 template <bool PREP>
 __global__ __launch_bounds__(512) void k_kv8_write_one(Kv8 c, Kv8Rows r, Kv8Prep p) {
-  __shared__ double2 cs[PREP ? 32 : 1];
+  __shared__ double2 cs[PREP ? 32 : 1], none[PREP ? 16 : 1];
   const int tid = threadIdx.x, lane = tid & 63, chunk = tid & 15, head = blockIdx.x;
   float gain[16];
   if (PREP && head >= c.heads) {
@@ -410,11 +412,12 @@ __global__ __launch_bounds__(512) void k_kv8_write_one(Kv8 c, Kv8Rows r, Kv8Prep
   }
   if (PREP) load16(p.k_gain + chunk * 16, gain);
   if (PREP && tid < 32) cs[tid] = angle_cs64(r.position, p.inv_freq[tid]);
+  if (PREP && tid < 16) none[tid] = make_double2(1.0, 0.0);
   issue_fence();
   __syncthreads();  // all have read the powers of two (and the angles are there)
   float x[16], y[4] = {bf_lo(v.x), bf_hi(v.x), bf_lo(v.y), bf_hi(v.y)};
   unpack16(k0, k1, x);
-  if (PREP) prepare_key(x, gain, cs, chunk);
+  if (PREP) prepare_key(x, gain, cs, none, chunk);
   bool bad = false;
   float kmost = 0.0f, vmost = 0.0f;
 #pragma unroll

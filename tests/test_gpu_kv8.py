@@ -261,6 +261,22 @@ def test_prepare_one_by_one(hq, hk):
         assert (a != b).mean() < 0.25
 
 
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("scale", [1e-30, 1e-3, 1e15, 1e30])
+def test_prepare_of_large_and_small_keys(rows, scale):
+    """K's norm in 64 bits: of any magnitude the same keys but for the epsilon."""
+    r = rng(34)
+    q, k, v, qg, kg = projections(r, rows, 8, 2)
+    k = bf16(f32(k) * np.float32(scale))
+    cache = kv8.new_cache(2, rows)
+    prepare(cache, q, k, v, qg, kg, 0)
+    got = f64(kv8.read(cache, 0, rows)[0])
+    want = rotated(k, kg, 0, E.rope_inv_freq())
+    power = np.exp2(cache.k_scale.numpy(np.uint8).reshape(2, -1).astype(float) - 127).repeat(64, 1)[:, :rows].T[:, :, None]
+    # half a step of the code, or of the subnormals' at the block's power of two
+    assert (np.abs(got - want) <= 2.0 ** -4 * np.abs(want) * (1 + 2.0 ** -20) + 2.0 ** -10 * power).all()
+
+
 def test_prepare_of_a_row_with_nan():
     r = rng(4)
     q, k, v, qg, kg = projections(r, 5, 8, 2)
