@@ -1235,7 +1235,10 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
     phase(b + 1);
     values(b);
   }
-  if ((nblk & 1) == upper) lds_barrier();
+  if ((nblk & 1) == upper) {  // the half without the last block: its part of that block's V, which the other half reads
+    wait_vmcnt<3 * kRowDma>();
+    lds_barrier();
+  }
   wait_vmcnt<0>();  // no DMA outlives this
   // Both halves: each wave finishes half of the dims.
   const float2 t = rows_xor32(l);
