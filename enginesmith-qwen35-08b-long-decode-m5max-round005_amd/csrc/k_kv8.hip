@@ -19,8 +19,9 @@
 //
 // A bf16 has eight significant bits and is the exact sum of two e4m3 of four
 // bits each (and a signed rest): x = hi + lo, hi the nearest e4m3, lo = x - hi.
-// Queries and probabilities enter the 8-bit products in these two parts, which
-// loses nothing against bf16 products (the matrix cores align the addends of an
+// Queries and probabilities enter the 8-bit products in these two parts, a query at
+// a power of two of its own, probabilities at one for each 32 keys (shift_of below), so that
+// what bf16 products would take is kept (the matrix cores align the addends of an
 // 8-bit product to about 2^-13 of the largest: measured rms 1e-5 of it).
 #include "es_kernels.hpp"
 
@@ -561,10 +562,45 @@ __device__ __forceinline__ uint32_t finite_bits(uint32_t x) {
   return x < 0x7f800000u ? x : 0;
 }
 
-// Most that the scores may pass the exponent's reference before it moves (base
-// 2): e^-reference is at most 2^kSlack, and 2^(kSlack + kShift) is below 448.
+// The reference m of a query's exponents lies kShift below the largest score at which
+// it was set, and moves when a score passes m + kShift by more than kSlack (base 2).
 constexpr float kSlack = 4.0f, kShift = 4.0f;
 constexpr int kOne = 127, kLo = 127 - 4, kProb = 127 - 4;  // scale operands, 2^(byte - 127)
+
+// A probability enters its product as the sum of two e4m3, the lower one 2^5 times
+// too large, at a power of two that 32 keys of a query share: a lane's scale operand covers
+// 16 bytes of several lanes, which are of a block the tokens 16 j + 0 .. 7, or 16 j + 8 .. 15. The
+// largest of the 32 is brought to 2^7 .. 2^8. So each has eight significant bits down to 2^-13 of
+// that one, and an error of 2^-15, 2^-22 of it, below; a long flat rest keeps its weight
+// however far it lies below a single key elsewhere. (At one power for all keys, and the lower part
+// at the upper's, 131072 keys 10 nats below a first one lost 0.8 %, 16384 of 128 heads half.)
+// For the rest of those 32 themselves: where their largest outweighs the other three of its four
+// eights by 2^kAlone, what is at most the largest of these takes a product of its
+// own, at a power of two by that one. (For every block with a key 2^18 below its largest a
+// prompt chunk took 4 % longer at scores of unit deviation and 24 % at a deviation of two, so 2 and 3 %.)
+constexpr float kRest = 0.03125f, kMostShift = kProb - 5, kNoShift = -2.0f, kMostRef = 0x1p18f, kAlone = 13.0f;
+constexpr int kRestScale = -5, kNever = 500;
+// Exponent of a power of two by the logarithm, less m, of what comes to 2^7 .. 2^8: the most where there
+// is no key (-inf), or far below m. A reference too large to take it off exactly keeps all at one power.
+__device__ __forceinline__ float shift_of(float x, float m) {
+  return fminf(floorf(8.0f - x), fabsf(m) < kMostRef ? kMostShift : kNoShift);
+}
+// Four probabilities in two parts.
+__device__ __forceinline__ int2 split_probabilities(const float* y) {
+  const int h = pack_e4m3(y[0], y[1], y[2], y[3]);
+  const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), w = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
+  return make_int2(h, pack_e4m3(kRest, y[0] - u[0], y[1] - u[1], y[2] - w[0], y[3] - w[1]));
+}
+// Moves those of y that times 2^up are at most 2^8 (as rounded) to z, so multiplied; kNever: none.
+__device__ __forceinline__ void take_small(float* y, float* z, int up) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = ldexpf(y[i], up);
+    const bool is = x <= 257.0f;
+    z[i] = is ? x : 0.0f;
+    y[i] = is ? 0.0f : y[i];
+  }
+}
 
 // the hardware's reciprocal, within 1 ulp
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
@@ -1014,7 +1050,7 @@ __device__ __forceinline__ void wait_vmcnt() {
 // Wave w holds the 32 pairs 32 (w % 4) ..; the lower four waves take the even blocks
 // of keys, the upper four the odd ones, and both halves are joined at the end.
 //   S^T[token, query] = K Q^T and O^T[d, query] += V^T P^T on 32x32x64, each query
-//   (probability) as the sum of two e4m3 numbers, the lower one 16 times too large
+//   (probability) as the sum of two e4m3 numbers, the lower one 16 (32) times too large
 //   and with a power of two of its own. Lane (r = lane % 32, h = lane / 32) gives K's
 //   bytes of token r (V's of dim r) and those of query r, and receives tokens (dims)
 //   8 i + 4 h .. + 3 of query r: the tokens whose probabilities it has to give next.
@@ -1023,10 +1059,10 @@ __device__ __forceinline__ void wait_vmcnt() {
 // matrix core while the other works on its softmax. K and V reach LDS by DMA, in the
 // order of the operands, two to three phases ahead; the queries' lower part stays in
 // LDS, as registers are full: 128 of sums, 24 of queries, 32 of scores, operands.
-// Measured: 4096 rows behind 28672, 8 query and 2 KV heads, 806 to 853 us (1.0e12
-// operations, 1.2e15 a second). A phase takes 3040 cycles, 2048 of them
-// of the matrix core (without the softmax 2660, without the DMA 3010), and with all
-// 256 CUs at it the clock falls from 2.4 to 1.9 GHz. Four waves with 32 queries and
+// Measured: 4096 rows behind 28672, 8 query and 2 KV heads, 832 to 870 us by the card (1.0e12
+// operations, 1.2e15 a second; 2 % less before the powers of two of 32 keys). A phase takes 3100
+// cycles, 2048 of them of the matrix core, and with all 256 CUs at it the clock falls from 2.4 to
+// 1.9 GHz. Four waves with 32 queries and
 // all keys each, the same steps interleaved within a wave, took 3530 cycles; eight
 // with 16 queries, both parts as columns of one product, 3560.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -1039,7 +1075,7 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[kRowBytes];
   __shared__ int exponent[kKStages + kVStages][64];  // each 64 times
   __shared__ float scaled[kRowPairs], most[2][kRowPairs], sums[2][kRowPairs];
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+  const int tid = threadIdx.x, lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), r = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), upper = wave >> 2, mine = (wave & 3) * 32 + r;
   // heads in turn, then ranges of keys, so that an XCD's blocks share keys where
   // heads and ranges divide the XCDs; the tiles with most keys first
@@ -1113,14 +1149,14 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
     for (int i = 0; i < 3; ++i) qhi[i] = read(upper_parts + (wave & 3) * 8192 + i * 2048);
   }
   const float cq = scaled[mine];
-  const int2 rq = divide(min(pair0 + mine, pairs - 1), a.group, a.inv_group);
-  const int last = a.position + rq.x;  // last key of the lane's query
+  const int last = a.position + divide(min(pair0 + mine, pairs - 1), a.group, a.inv_group).x;  // last key of the lane's query
   f32x16 o[8], s[2];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int k = 0; k < 16; ++k) o[i][k] = 0.0f;
   float m = kNone, l = 0.0f, cs = 0.0f;  // reference less kShift; the lane's part of the sum, times 2^kShift
+  float top32 = 0.0f, next32 = 0.0f;     // the largest of 32 scores, and of the other three eights of them
   auto scores = [&](int b) {
     const uint32_t from = kRowStages + kstage(b) * kBlockBytes, lower = (wave & 3) * 8192;
     const int ke = exponent[kstage(b)][lane];
@@ -1151,17 +1187,23 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) s[i][k] = 32 * i + 8 * (k >> 2) + (k & 3) <= left ? s[i][k] : -__builtin_inff();
     }
-    float tops[4];
+    float tops[4];  // of the lane's tokens 16 j + 0 .. 7 and 16 j + 8 .. 15, in either half of the block
 #pragma unroll
-    for (int k = 0; k < 4; ++k) tops[k] = s[k >> 1][8 * (k & 1)];
+    for (int k = 0; k < 4; ++k) tops[k] = s[k >> 1][4 * (k & 1)];
 #pragma unroll
     for (int k = 1; k < 8; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i)  // the larger; fmaxf would first quiet what a product gave
-        tops[i] = __builtin_amdgcn_fmed3f(tops[i], s[i >> 1][8 * (i & 1) + k], __builtin_inff());
-    float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        tops[i] = __builtin_amdgcn_fmed3f(tops[i], s[i >> 1][4 * (i & 1) + (k & 3) + 8 * (k >> 2)], __builtin_inff());
+    const float front = fmaxf(tops[0], tops[2]), back = fmaxf(tops[1], tops[3]);
+    // of the query's four eights of the first kind in the lower lanes, of the second in the upper: the two largest
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(front), __float_as_uint(back), false, false);
+    const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(fminf(tops[0], tops[2])), __float_as_uint(fminf(tops[1], tops[3])),
+                                                    false, false);
+    top32 = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    next32 = fmaxf(fminf(__uint_as_float(a[0]), __uint_as_float(a[1])), fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1])));
     cs = fmaxf(ldexpf(cq, ke - 127), 1e-37f);
-    top = top * cs - kShift;
+    const float top = fmaxf(front, back) * cs - kShift;
     if (__any(top > m + kSlack)) {
       const float2 u = rows_xor32(top);
       const float next = fmaxf(m, fmaxf(u.x, u.y)), f = __builtin_amdgcn_exp2f(m - next);
@@ -1179,29 +1221,61 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
     i32x8 v[8], phi, plo;
     // sums 0 .. 3 are of the wave's own half of the dims, 4 .. 7 of the other's
     auto fetch = [&](int t) { v[t] = read(t < 4 ? from + upper * 8192 + t * 2048 : from - upper * 8192 + t * 2048); };
-    float sum = 0.0f;
+    const float x = fmaf(top32, cs, -m), xnext = fmaf(next32, cs, -m);
+    const float shift = shift_of(x, m);
+    const float2 shifts = rows_xor32(shift);  // of the tokens 16 j + 0 .. 7, of the others
+    const float from_m[2] = {m - shifts.x, m - shifts.y};
+    const int scale = kProb - (int)shift;
+    int low_scale = 0;
+    float sum[2] = {0.0f, 0.0f};
+    auto probabilities = [&](int i, float* y) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float y[4];
+      for (int k = 0; k < 4; ++k) y[k] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][4 * (i & 3) + k], cs, -from_m[i & 1]));
+      sum[i & 1] += (y[0] + y[1]) + (y[2] + y[3]);
+    };
+    auto parts = [&](int i, const float* y, i32x8& upper, i32x8& lower) {
+      const int2 p = split_probabilities(y);
+      upper[(i & 1) * 4 + (i >> 1)] = p.x;
+      lower[(i & 1) * 4 + (i >> 1)] = p.y;
+    };
+    i32x8 low[2];  // the parts of those with a power of two of their own
+    const bool alone = x - xnext > kAlone && xnext > kNone;
+    const int lows = __any(alone) ? 2 : 0;
+    if (lows) {
+      const float own = shift_of(xnext, m);
+      const float2 ups = rows_xor32(alone ? own - shift : (float)kNever);
+      low_scale = kProb - (int)own;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) y[k] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][4 * (i & 3) + k], cs, -m));
-      sum += (y[0] + y[1]) + (y[2] + y[3]);
-      const int hi = pack_e4m3(y[0], y[1], y[2], y[3]);
-      const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), w = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-      i16x2 q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(i16x2{0, 0}, y[0] - u[0], y[1] - u[1], 0.0625f, false);
-      q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(q, y[2] - w[0], y[3] - w[1], 0.0625f, true);
-      phi[(i & 1) * 4 + (i >> 1)] = hi;
-      plo[(i & 1) * 4 + (i >> 1)] = __builtin_bit_cast(int, q);
+      for (int i = 0; i < 8; ++i) {
+        float y[4], z[4];
+        probabilities(i, y);
+        take_small(y, z, (int)(i & 1 ? ups.y : ups.x));
+        parts(i, y, phi, plo);
+        parts(i, z, low[0], low[1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float y[4];
+        probabilities(i, y);
+        parts(i, y, phi, plo);
+      }
     }
-    l += sum;
+    l += ldexpf(sum[0], -(int)shifts.x) + ldexpf(sum[1], -(int)shifts.y);
     fetch(0);
     fetch(1);
 #pragma unroll
     for (int t = 0; t < 9; ++t) {
       issue_fence();
-      if (t < 8) o[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v[t], phi, o[t], 0, 0, 0, ve, 0, kProb);
+      if (t < 8) o[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v[t], phi, o[t], 0, 0, 0, ve, 0, scale);
       if (t < 6) fetch(t + 2);
-      if (t > 0) o[t - 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v[t - 1], plo, o[t - 1], 0, 0, 0, ve, 0, kProb - 4);
+      if (t > 0) {
+        o[t - 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v[t - 1], plo, o[t - 1], 0, 0, 0, ve, 0, scale + kRestScale);
+#pragma unroll 1
+        for (int i = 0; i < lows; ++i)
+          o[t - 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v[t - 1], i ? low[1] : low[0], o[t - 1], 0, 0, 0, ve, 0,
+                                                                     low_scale + i * kRestScale);
+      }
     }
   };
   // K of the phase and V of the one before have arrived once all but the last three
@@ -1240,14 +1314,18 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
     lds_barrier();
   }
   wait_vmcnt<0>();  // no DMA outlives this
-  // Both halves: each wave finishes half of the dims.
+  // Both halves: each wave finishes half of the dims. The lane again, so that nothing of it takes registers in the loop.
+  int lane2 = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+  asm("" : "+v"(lane2));
+  const int h2 = lane2 >> 5, mine2 = (wave & 3) * 32 + (lane2 & 31);
+  const int2 rq = divide(min(pair0 + mine2, pairs - 1), a.group, a.inv_group);
   const float2 t = rows_xor32(l);
-  if (h == 0) {
-    most[upper][mine] = m;
-    sums[upper][mine] = t.x + t.y;
+  if (h2 == 0) {
+    most[upper][mine2] = m;
+    sums[upper][mine2] = t.x + t.y;
   }
   lds_barrier();
-  f32x4* const swap = reinterpret_cast<f32x4*>(lds) + lane;
+  f32x4* const swap = reinterpret_cast<f32x4*>(lds) + lane2;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1258,16 +1336,16 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
       swap[wave * 1024 + (4 * i + k) * 64] = x;
     }
   lds_barrier();
-  const float other = most[1 - upper][mine], ref = fmaxf(m, other);
+  const float other = most[1 - upper][mine2], ref = fmaxf(m, other);
   float f = __builtin_amdgcn_exp2f(m - ref), fo = __builtin_amdgcn_exp2f(other - ref);
-  const float total = fmaf(sums[0][mine], upper ? fo : f, sums[1][mine] * (upper ? f : fo)) * 0.0625f;  // 2^-kShift
+  const float total = fmaf(sums[0][mine2], upper ? fo : f, sums[1][mine2] * (upper ? f : fo)) * 0.0625f;  // 2^-kShift
   const float inv = a.splits > 1 ? 1.0f : 1.0f / total;
   f *= inv;
   fo *= inv;
   const size_t row = (size_t)rq.x * a.q_heads + head * a.group + rq.y;
   // a lane without a pair stores behind the end of the buffer, which drops it
   const auto out = __builtin_amdgcn_make_buffer_rsrc((void*)a.out, 0, (int)((uint32_t)a.rows * a.q_heads * 512u), 0x00020000);
-  const uint32_t to = pair0 + mine < pairs ? (uint32_t)row * 512u + upper * 256 + h * 16 : 0xfffff000u;
+  const uint32_t to = pair0 + mine2 < pairs ? (uint32_t)row * 512u + upper * 256 + h2 * 16 : 0xfffff000u;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1288,15 +1366,15 @@ __global__ __launch_bounds__(512, 1) void k_kv8_attn_rows(Kv8 c, Kv8Attn a) {
       }
       if (a.splits > 1) {
         float* part = a.part + (row * a.splits + split) * kKv8PartFloats;
-        if (pair0 + mine < pairs) {
-          *reinterpret_cast<f32x4*>(part + upper * 128 + 32 * i + 16 * j + 8 * h) = f32x4{y[0], y[1], y[2], y[3]};
-          *reinterpret_cast<f32x4*>(part + upper * 128 + 32 * i + 16 * j + 8 * h + 4) = f32x4{y[4], y[5], y[6], y[7]};
-          if (i + j + h + upper == 0) *reinterpret_cast<float2*>(part + 256) = make_float2(ref, total);
+        if (pair0 + mine2 < pairs) {
+          *reinterpret_cast<f32x4*>(part + upper * 128 + 32 * i + 16 * j + 8 * h2) = f32x4{y[0], y[1], y[2], y[3]};
+          *reinterpret_cast<f32x4*>(part + upper * 128 + 32 * i + 16 * j + 8 * h2 + 4) = f32x4{y[4], y[5], y[6], y[7]};
+          if (i + j + h2 + upper == 0) *reinterpret_cast<float2*>(part + 256) = make_float2(ref, total);
         }
         continue;
       }
       if (a.gate) {
-        const u32x4 gate = *reinterpret_cast<const u32x4*>(a.gate + row * 512 + 256 + upper * 128 + 32 * i + 16 * j + 8 * h);
+        const u32x4 gate = *reinterpret_cast<const u32x4*>(a.gate + row * 512 + 256 + upper * 128 + 32 * i + 16 * j + 8 * h2);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           y[2 * k] *= sigmoid(bf_lo(gate[k]));
