@@ -627,29 +627,37 @@ __device__ __forceinline__ void lds_barrier() {
 //   (n = lane % 16, g = lane / 16) gives K bytes of token n and Q bytes of query n
 //   and receives tokens 4 g .. 4 g + 3 of query n;
 //   O^T[d, query] += V^T P^T: wave w takes dims 64 w .. 64 w + 63; the 128 places along
-//   tokens hold the hi parts of the 64 probabilities and their lo parts,
+//   tokens hold the upper parts of the 64 probabilities and their lower parts,
 //   against V twice.
 // So each byte of K and V enters one wave's registers once, straight from memory,
-// and the probabilities alone pass between waves (through LDS, one barrier a
-// block). What bounds a short context is how many bytes each CU must fetch
-// (measured 20 a cycle), a long one memory (131072 tokens, 2 heads: 134 MB in 25 us,
-// 5.3 TB/s), many queries the products and exponentials of four waves on a SIMD.
+// and the largest scores and the probabilities alone pass between waves, through LDS with one
+// barrier a block: it publishes a block's largest scores, from which every wave takes the
+// powers of two of 32 keys and the reference, and the block before's probabilities. What bounds a
+// short context is how many bytes each CU must fetch (measured 20 a cycle), a long one memory
+// (131072 tokens, 2 heads: 134 MB in 25 us, 5.3 TB/s), many queries the products and
+// exponentials of four waves on a SIMD. (Probabilities before the barrier, at one power
+// of two, with 8 query and 2 KV heads: 1000 rows alone 14.3 us and 15.8 so, 128 behind 28672 45.6 and 50.2, one
+// behind 131071 28.4 and 28.9.)
 // The next block's K is fetched as soon as this one's products have read it, its V
-// likewise: 32 KB of a group on their way. A group's waves share the exponent's reference of a query; it moves when a score
-// of any passes it by more than kSlack.
+// likewise: 32 KB of a group on their way.
 // The bound of 1024 threads holds for every G: it keeps the compiler to the 128
 // vector registers of 16 waves a CU and off the accumulator registers.
 template <int NT, int G>
 __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
-  constexpr int kQueryBytes = NT * 8192, kProbBytes = NT * 4096;  // bytes: the queries' parts; a group's two buffers
+  // bytes: the queries' parts; a group's two buffers of probabilities, and of those with a power of two of their own
+  constexpr int kQueryBytes = NT * 8192, kProbBytes = NT * 4096, kLowBytes = NT * 4608;
   constexpr int kSumRow = 260, kSum = NT * 16 * kSumRow;  // floats: a query's row of sums; a group's sums
   // the queries and probabilities; at the end, in their place, the groups' sums
-  constexpr int kIn = kQueryBytes + G * kProbBytes, kOut = G > 1 ? G * kSum * 4 : 0;
+  constexpr int kLow = kQueryBytes + G * kProbBytes, kTops = kLow + G * kLowBytes, kTopBytes = NT * 16 * 32;  // largest scores: of a group, one buffer
+  constexpr int kIn = kTops + 2 * G * kTopBytes, kOut = G > 1 ? G * kSum * 4 : 0;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kIn > kOut ? kIn : kOut];
-  __shared__ __attribute__((aligned(16))) int moves[2][4 * G];
-  __shared__ __attribute__((aligned(16))) float tops[G][NT * 16][4];
-  __shared__ float scaled[NT * 16], most[G][NT * 16];
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  __shared__ __attribute__((aligned(16))) float sums[G][NT * 16][4];
+  __shared__ float most[G][NT * 16];
+  __shared__ struct {
+    float power;  // the query's power of two / 16, for base 2
+    int last;     // its last key
+  } of_query[NT * 16];
+  const int tid = threadIdx.x, lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), group = __builtin_amdgcn_readfirstlane(tid >> 8);
   int split = blockIdx.x, tile = blockIdx.y, head = blockIdx.z;
   if (gridDim.y < (uint32_t)a.tiles) {  // all tiles of a range on one XCD: they share its keys in the L2
@@ -665,22 +673,25 @@ __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
   const int nblk = tile_last / kKv8Block + 1;
   const int b0 = split * a.per, b1 = min(b0 + a.per, nblk), turns = max(0, (b1 - b0 + G - 1) / G);
   const size_t store = (size_t)head * c.blocks;
-  const uint8_t* kp = c.k + store * kBlockBytes + (wave >> 1) * 8192 + (wave & 1) * 256 + (g >> 1) * 2048 + (g & 1) * 512 + n * 16;
-  const uint8_t* vp = c.v + store * kBlockBytes + wave * 4096 + (g >> 1) * 1024 + (g & 1) * 512 + n * 16;
+  // the wave's part of the block and the lane's of that
+  const uint8_t* kp = c.k + store * kBlockBytes + (wave >> 1) * 8192 + (wave & 1) * 256 + 2048;  // all its offsets fit a load's
+  const uint8_t* vp = c.v + store * kBlockBytes + wave * 4096;
+  const uint32_t klane = (g >> 1) * 2048 + (g & 1) * 512 + n * 16, vlane = (g >> 1) * 1024 + (g & 1) * 512 + n * 16;
   i32x4 kr[4], vr[4];
   int ke = 0, ve = 0;
   auto fetch_k = [&](int b) {
     const uint8_t* at = kp + (size_t)b * kBlockBytes;
     ke = c.k_scale[store + b];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) kr[i] = *reinterpret_cast<const i32x4*>(at + (i >> 1) * 4096 + (i & 1) * 1024);
+    for (int i = 0; i < 4; ++i) kr[i] = *reinterpret_cast<const i32x4*>(at + ((i >> 1) * 4096 + (i & 1) * 1024 - 2048) + klane);
   };
   auto fetch_v = [&](int b) {
     const uint8_t* at = vp + (size_t)b * kBlockBytes;
     ve = c.v_scale[store + b];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vr[i] = *reinterpret_cast<const i32x4*>(at + (i >> 1) * 2048 + (i & 1) * 256);
+    for (int i = 0; i < 4; ++i) vr[i] = *reinterpret_cast<const i32x4*>(at + (i >> 1) * 2048 + (i & 1) * 256 + vlane);
   };
+  if (tid < 16 * NT) of_query[tid].last = a.position + divide(min(pair0 + tid, pairs - 1), a.group, a.inv_group).x;
   // queries: 16 lanes a query, 16 dims a lane; their loads go out before the first
   // keys' (loads return in order), which are on their way during the conversion
   {
@@ -710,7 +721,7 @@ __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
       for (int i = 0; i < 8; ++i)
         top = max(top, max(finite_bits(x[i >> 2][i & 3] << 16), finite_bits(x[i >> 2][i & 3] & 0xffff0000u)));
       const int e = scale_exponent(row16_max(__uint_as_float(top)), -100);
-      if (chunk == 0) scaled[q] = ldexpf(kLog2e / 16.0f, e);
+      if (chunk == 0) of_query[q].power = ldexpf(kLog2e / 16.0f, e);
       i32x4 hi, lo;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -727,36 +738,45 @@ __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
   }
   lds_barrier();
   f32x4 o[NT][4];
-  float m[NT], l[NT], cq[NT];  // the reference, less kShift; the lane's part of the sum, times 2^kShift
-  int last[NT];                // last key of the lane's query
+  float m[NT], l[NT];  // the reference, less kShift; the lane's part of the sum, times 2^kShift
 #pragma unroll
   for (int q = 0; q < NT; ++q) {
     m[q] = kNone;
     l[q] = 0.0f;
-    cq[q] = scaled[16 * q + n];
-    last[q] = a.position + divide(min(pair0 + 16 * q + n, pairs - 1), a.group, a.inv_group).x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[q][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  int* const prob = reinterpret_cast<int*>(lds + kQueryBytes + group * kProbBytes);
+  // of a turn's buffer and a tile: upper parts, lower parts
+  auto prob_of = [&](int turn, int q) {
+    return reinterpret_cast<int*>(lds + kQueryBytes + group * kProbBytes) + ((turn & 1) * NT + q) * 512;
+  };
+  // the same of those with a power of two of their own, then the lanes' scale operands
+  auto low_of = [&](int turn, int q) { return reinterpret_cast<int*>(lds + kLow + group * kLowBytes) + ((turn & 1) * NT + q) * 576; };
   // hi of dims 0 .. 127 and 128 .. 255, lo of both
-  auto queries = [&](int q, i32x8* w) {
+  auto queries = [&](int q, i32x8* w, int from) {
     const i32x4* at = reinterpret_cast<const i32x4*>(lds + q * 8192) + lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __builtin_shufflevector(at[i * 128], at[i * 128 + 64], 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int i = from; i < 4; ++i) w[i] = __builtin_shufflevector(at[i * 128], at[i * 128 + 64], 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  i32x8 w[4];  // one tile's stay in registers (40 rows behind 20000 19.9 us, 20.4 without)
-  if constexpr (NT == 1) queries(0, w);
-  auto block = [&](int turn, auto more) {
-    const int mine = b0 + group + turn * G, b = min(mine, b1 - 1), buf = turn & 1;
-    f32x4 s[NT];
+  // One tile's upper parts stay in registers, all of them before the lower parts were read again here:
+  // 40 rows behind 20000 18.2 us, 18.4 with half of them, 19.1 with none.
+  i32x8 w[4];
+  if constexpr (NT == 1) queries(0, w, 0);
+  // largest scores of a query in a block: [first or second 8 of every 16 tokens][wave]
+  auto top_of = [&](int turn, int q) {
+    return reinterpret_cast<float*>(lds + kTops + ((turn & 1) * G + group) * kTopBytes) + (q * 16 + n) * 8;
+  };
+  f32x4 s[NT];
+  int scales = 0;  // operands of the lane's parts of the probabilities, a byte each
+  auto scores = [&](int turn, auto more) {
+    const int mine = b0 + group + turn * G, b = min(mine, b1 - 1);
     {
       i32x8 k[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) k[h] = __builtin_shufflevector(kr[2 * h], kr[2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
       for (int q = 0; q < NT; ++q) {
-        if constexpr (NT > 1) queries(q, w);
+        queries(q, w, NT == 1 ? 2 : 0);
         const f32x4 zero = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         s[q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k[0], w[0], zero, 0, 0, 0, kOne, 0, kOne);
         f32x4 rest = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k[0], w[2], zero, 0, 0, 0, kOne, 0, kLo);
@@ -768,66 +788,87 @@ __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
     }
 #pragma unroll
     for (int q = 0; q < NT; ++q) asm volatile("" : "+v"(s[q]));  // the keys' registers are free
-    const float scale = ldexpf(1.0f, ke - 127);
+    const float power = ldexpf(1.0f, ke - 127);
     issue_fence();
     if constexpr (decltype(more)::value) fetch_k(min(mine + G, b1 - 1));
     issue_fence();
-    float top[NT], part[NT];
-    bool pass = false;
 #pragma unroll
     for (int q = 0; q < NT; ++q) {
-      const float cs = fmaxf(cq[q] * scale, 1e-37f);
-      const int left = (mine < b1 ? last[q] : -1) - (b * 64 + 16 * wave + 4 * g);
+      const auto own = of_query[16 * q + n];
+      const float cs = fmaxf(own.power * power, 1e-37f);
+      const int left = (mine < b1 ? own.last : -1) - (b * 64 + 16 * wave + 4 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[q][i] = i <= left ? s[q][i] * cs : -__builtin_inff();
-      top[q] = fmaxf(fmaxf(s[q][0], s[q][1]), fmaxf(s[q][2], s[q][3])) - kShift;
-      pass |= top[q] > m[q] + kSlack;
+      const float2 top = rows_xor16(fmaxf(fmaxf(s[q][0], s[q][1]), fmaxf(s[q][2], s[q][3])));
+      top_of(turn, q)[2 * (g & 2) + wave] = fmaxf(top.x, top.y);  // of two lanes each
     }
-    auto probabilities = [&]() {
-#pragma unroll
-      for (int q = 0; q < NT; ++q) {
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_exp2f(s[q][i] - m[q]);
-        const int h = pack_e4m3(y[0], y[1], y[2], y[3]);
-        const f32x2 u = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), w = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
-        int* to = prob + ((buf * NT + q) * 2) * 256 + lane * 4 + wave;
-        to[0] = h;
-        to[256] = pack_e4m3(y[0] - u[0], y[1] - u[1], y[2] - w[0], y[3] - w[1]);
-        part[q] = (y[0] + y[1]) + (y[2] + y[3]);
-      }
+  };
+  // A lane's own tokens are of the first or second kind by g / 2; its operand covers by g the upper parts of the
+  // first ones, of the second ones, the lower parts of the first ones, of the second ones.
+  auto operand = [&](float shift) {
+    const float2 both = rows_xor32(shift);
+    return (g & 2 ? kProb + kRestScale : kProb) - (int)(g & 1 ? both.y : both.x);
+  };
+  float limit = kMostShift;
+  bool low = false;  // whether the turn's have some with a power of two of their own
+  auto put = [&](const float* y, int* to) {
+    const int2 p = split_probabilities(y);
+    to[lane * 4 + wave] = p.x;
+    to[256 + lane * 4 + wave] = p.y;
+  };
+  auto probabilities = [&](int turn) {
+    float top[NT];
+    auto is_alone = [](float top, float next) { return top - next > kAlone && next > kNone; };
+    auto tops = [&](int q) { return *reinterpret_cast<const f32x4*>(top_of(turn, q) + 2 * (g & 2)); };  // of four eights
+    auto second = [](f32x4 t) {
+      return fmaxf(fminf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fminf(t[0], t[1]), fminf(t[2], t[3])));
     };
-    const bool move = __any(pass);
-    if (lane == 0) moves[buf][group * 4 + wave] = move;
-    if (!move) probabilities();
-    lds_barrier();
-    int moved = 0;
-    if (lane < G * 4) moved = moves[buf][lane];
-    if (__any(moved)) {
+    bool pass = false, alone = false;
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      const f32x4 t = tops(q);
+      top[q] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+      pass |= top[q] - m[q] > kShift + kSlack;
+      alone |= is_alone(top[q], second(t));
+    }
+    if (__any(pass)) {  // in all four waves or in none
+      bool large = false;
 #pragma unroll
       for (int q = 0; q < NT; ++q) {
-        const float2 x = rows_xor16(top[q]);
-        const float2 y = rows_xor32(fmaxf(x.x, x.y));
-        if (g == 0) tops[group][q * 16 + n][wave] = fmaxf(y.x, y.y);
-      }
-      lds_barrier();
-#pragma unroll
-      for (int q = 0; q < NT; ++q) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(tops[group][q * 16 + n]);
-        const float mn = fmaxf(m[q], fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-        const float f = __builtin_amdgcn_exp2f(m[q] - mn);
+        const float2 both = rows_xor32(top[q]);
+        const float mn = fmaxf(m[q], fmaxf(both.x, both.y) - kShift), f = __builtin_amdgcn_exp2f(m[q] - mn);
         m[q] = mn;
         l[q] *= f;
+        large |= mn != kNone && fabsf(mn) >= kMostRef;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int k = 0; k < 4; ++k) o[q][i][k] *= f;
       }
-      probabilities();
-      lds_barrier();
+      limit = __any(large) ? kNoShift : kMostShift;
     }
+    low = __any(alone);
 #pragma unroll
-    for (int q = 0; q < NT; ++q) l[q] += part[q];
+    for (int q = 0; q < NT; ++q) {
+      const float shift = fminf(floorf(8.0f - (top[q] - m[q])), limit);
+      scales = q == 0 ? operand(shift) : scales | operand(shift) << 8;
+      const float from = m[q] - shift;
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_exp2f(s[q][i] - from);
+      l[q] += ldexpf((y[0] + y[1]) + (y[2] + y[3]), -(int)shift);
+      if (low) {
+        const float next = second(tops(q)), own = fminf(floorf(8.0f - (next - m[q])), limit);
+        float z[4];
+        take_small(y, z, is_alone(top[q], next) ? (int)(own - shift) : kNever);
+        put(z, low_of(turn, q));
+        low_of(turn, q)[512 + lane] = operand(own);  // the same in all four waves
+      }
+      put(y, prob_of(turn, q));
+    }
+  };
+  auto values = [&](int turn, auto more) {
+    const int b = min(b0 + group + turn * G, b1 - 1);
     if (b * 64 + 64 > end) {  // bytes behind the last key may be anything
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -839,34 +880,59 @@ __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
     }
 #pragma unroll
     for (int q = 0; q < NT; ++q) {
-      const i32x4* at = reinterpret_cast<const i32x4*>(prob + ((buf * NT + q) * 2) * 256) + lane;
+      const i32x4* at = reinterpret_cast<const i32x4*>(prob_of(turn, q)) + lane;
       const i32x8 p = __builtin_shufflevector(at[0], at[64], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const i32x8 v = __builtin_shufflevector(vr[i], vr[i], 0, 1, 2, 3, 0, 1, 2, 3);
-        o[q][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, p, o[q][i], 0, 0, 0, ve, 0, kProb);
+        o[q][i] = q == 0 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, p, o[q][i], 0, 0, 0, ve, 0, scales)
+                         : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, p, o[q][i], 0, 0, 0, ve, 1, scales);
       }
     }
+    if (low) {
 #pragma unroll
-    for (int q = 0; q < NT; ++q)
+      for (int q = 0; q < NT; ++q) {
+        const i32x4* at = reinterpret_cast<const i32x4*>(low_of(turn, q)) + lane;
+        const i32x8 p = __builtin_shufflevector(at[0], at[64], 0, 1, 2, 3, 4, 5, 6, 7);
+        const int own = low_of(turn, q)[512 + lane];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(o[q][i]));
+        for (int i = 0; i < 4; ++i) {
+          const i32x8 v = __builtin_shufflevector(vr[i], vr[i], 0, 1, 2, 3, 0, 1, 2, 3);
+          o[q][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, p, o[q][i], 0, 0, 0, ve, 0, own);
+        }
+      }
+    }
     issue_fence();
-    if constexpr (decltype(more)::value) fetch_v(min(mine + G, b1 - 1));
+    if constexpr (decltype(more)::value) fetch_v(min(b0 + group + (turn + 1) * G, b1 - 1));
     issue_fence();
   };
-  // two bodies, so that the waits for loads count what is on its way in each
-  for (int turn = 0; turn + 1 < turns; ++turn) block(turn, std::true_type{});
-  if (turns > 0) block(turns - 1, std::false_type{});
+  // A turn's barrier publishes its largest scores and the probabilities of the turn before. The last
+  // one apart, so that the waits for loads count what is on its way in each.
+  for (int turn = 0; turn + 1 < turns; ++turn) {
+    scores(turn, std::true_type{});
+    lds_barrier();
+    if (turn > 0) values(turn - 1, std::true_type{});
+    probabilities(turn);
+  }
+  if (turns > 0) {
+    scores(turns - 1, std::false_type{});
+    lds_barrier();
+    if (turns > 1) values(turns - 2, std::true_type{});
+    probabilities(turns - 1);
+    lds_barrier();
+    values(turns - 1, std::false_type{});
+  }
+  // the lane again, so that nothing of it takes registers in the loop
+  const int lane2 = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), n2 = lane2 & 15, g2 = lane2 >> 4;
   // the lanes and waves of a query hold its tokens' parts of the sum
   __syncthreads();
 #pragma unroll
   for (int q = 0; q < NT; ++q) {
     const float2 x = rows_xor16(l[q]);
     const float2 y = rows_xor32(x.x + x.y);
-    if (g == 0) {
-      tops[group][q * 16 + n][wave] = (y.x + y.y) * (1.0f / 16.0f);
-      if (wave == 0) most[group][q * 16 + n] = m[q];
+    if (g2 == 0) {
+      sums[group][q * 16 + n2][wave] = (y.x + y.y) * (1.0f / 16.0f);
+      if (wave == 0) most[group][q * 16 + n2] = m[q];
     }
   }
   if constexpr (G > 1) {
@@ -875,26 +941,26 @@ __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
     for (int q = 0; q < NT; ++q)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(sum + (q * 16 + n) * kSumRow + wave * 64 + i * 16 + g * 4) = o[q][i];
+        *reinterpret_cast<f32x4*>(sum + (q * 16 + n2) * kSumRow + wave * 64 + i * 16 + g2 * 4) = o[q][i];
   }
   __syncthreads();
   // group k finishes tiles k, k + G, ..
 #pragma unroll
   for (int q = 0; q < NT; ++q) {
-    const int pair = pair0 + 16 * q + n, at = q * 16 + n;
+    const int pair = pair0 + 16 * q + n2, at = q * 16 + n2;
     if (q % G != group || pair >= pairs) continue;
     float ref = kNone, f[G], total = 0.0f;
 #pragma unroll
     for (int k = 0; k < G; ++k) ref = fmaxf(ref, most[k][at]);
 #pragma unroll
     for (int k = 0; k < G; ++k) {
-      const f32x4 t = *reinterpret_cast<const f32x4*>(tops[k][at]);
+      const f32x4 t = *reinterpret_cast<const f32x4*>(sums[k][at]);
       f[k] = __builtin_amdgcn_exp2f(most[k][at] - ref);
       total = fmaf((t[0] + t[1]) + (t[2] + t[3]), f[k], total);
     }
     const int2 to = divide(pair, a.group, a.inv_group);
     const size_t row = (size_t)to.x * a.q_heads + head * a.group + to.y;
-    const int d = wave * 64 + g * 4;
+    const int d = wave * 64 + g2 * 4;
     float* part = a.part + (row * a.splits + split) * kKv8PartFloats;
     const float inv = 1.0f / total;
 #pragma unroll
@@ -912,7 +978,7 @@ __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
       }
       if (a.splits > 1) {
         *reinterpret_cast<f32x4*>(part + d + 16 * i) = x;
-        if (i == 0 && wave == 0 && g == 0) *reinterpret_cast<float2*>(part + 256) = make_float2(ref, total);
+        if (i == 0 && wave == 0 && g2 == 0) *reinterpret_cast<float2*>(part + 256) = make_float2(ref, total);
         continue;
       }
 #pragma unroll
@@ -1405,7 +1471,7 @@ constexpr int kRowLeast = 96;  // pairs of a head from which on 128-pair blocks 
 
 // Estimates in us by which a call takes one form or another, fitted to calls of 5 to
 // 8192 rows at 0 to 70000, 1 to 8 KV heads:
-//   few: for 64 keys of 16 pairs 0.42, of 32 together 0.575; for each round of blocks 8 and 13
+//   few: for 64 keys of 16 pairs 0.42, of 32 together 0.6; for each round of blocks 8 and 13
 //   rows: 1.28 for 64 keys of 128 pairs with a CU of its own, up to 1.6 when all CUs are
 //     at it (the clock falls), 10 a round; with ranges 6, and writing and joining them
 // Measured, 8 query and 2 KV heads where not said otherwise: 500 rows alone 8 us with 16 pairs
@@ -1416,7 +1482,7 @@ constexpr int kRowLeast = 96;  // pairs of a head from which on 128-pair blocks 
 // 8 heads, 557, 444 with one; 4096 alone 111 and 107.
 float few_us(int nt, int heads, int pairs, float keys) {
   const float tiles = (float)few_tiles(nt, pairs) * heads;
-  return tiles * keys / 256 * (nt == 1 ? 0.42f : 0.575f) + (nt == 1 ? 8 : 13) * ceilf(tiles / 256);
+  return tiles * keys / 256 * (nt == 1 ? 0.42f : 0.6f) + (nt == 1 ? 8 : 13) * ceilf(tiles / 256);
 }
 // most and least: blocks of keys of the last tile and the first
 float rows_us(int tiles, int ranges, int least, int most) {
@@ -1510,16 +1576,18 @@ hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s) {
   // token behind 100, 500, 750: 6.6, 7.6, 8.7 us, and 9.4 with a block to a range).
   a.per = most <= 12 ? most : (most + ranges - 1) / ranges;
   a.splits = (most + a.per - 1) / a.per;
-  // Groups of four waves a block. Where one tile reads its keys alone memory sets the time
-  // and one group fetches as fast as four, with nothing to join; many tiles of a range, or the
-  // one range of a short context, have work for all 16 waves. (4, 2 and 1 groups, 2 KV heads:
-  // one token behind 16000 10.4, 9.8, 8.9 us; 6 rows behind 32000, two tiles, 13.2, 12.3,
-  // 12.8; 40 behind 20000, ten, 20.4, 21.8, 25.5; 1000 rows alone 16.2, 17.2, 21.9.)
-  const int most_groups = a.splits == 1 || tiles > 5 ? 4 : tiles > 1 ? 2 : 1;
-  const int g = min(most_groups, a.per >= 4 ? 4 : a.per >= 2 ? 2 : 1);
+  // Groups of four waves a block. Where one tile of 16 pairs reads its keys alone memory sets the time
+  // and one group fetches as fast as four, with nothing to join; more pairs of a range, or the
+  // one range of a short context, have work for all 16 waves, two tiles only where a range is
+  // long. (4 and 2 groups, 8 query and 2 KV heads: 8 rows behind 40000, two tiles of 16 pairs with ranges of
+  // 10 blocks of keys, 13.9 and 13.2 us; of 32 and 8 heads, with 20, 20.4 and 21.8; 16 rows behind 70000, four tiles,
+  // 21.7 and 25.1; 32 behind 70000, four tiles of 32, 34.2 and 41.0.) Tiles of 32 leave no registers to one group.
+  const int sixteens = tiles * nt;
+  const int most_groups = a.splits == 1 || sixteens > 2 ? 4 : sixteens == 1 ? 1 : a.per >= 20 ? 4 : 2;
+  const int g = min(most_groups, a.per >= 4 ? 4 : a.per >= 2 || nt == 2 ? 2 : 1);
   const auto few = nt == 1
                        ? (g == 4 ? k_kv8_attn_few<1, 4> : g == 2 ? k_kv8_attn_few<1, 2> : k_kv8_attn_few<1, 1>)
-                       : (g == 4 ? k_kv8_attn_few<2, 4> : g == 2 ? k_kv8_attn_few<2, 2> : k_kv8_attn_few<2, 1>);
+                       : (g == 4 ? k_kv8_attn_few<2, 4> : k_kv8_attn_few<2, 2>);
   const dim3 grid = few_grouped(tiles) ? dim3((a.splits * c.heads + 7) / 8 * 8 * tiles) : dim3(a.splits, tiles, c.heads);
   hipLaunchKernelGGL(few, grid, dim3(256 * g), 0, s, c, a);
   return join(a, s);

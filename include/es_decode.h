@@ -373,13 +373,17 @@ size_t es_attn_kv8_scratch_bytes(int q_heads, int kv_heads, int rows);
 /* Causal attention of `rows` queries at positions position .. position+rows-1
  * over this cache, one token or many: row r attends to positions 0 ..
  * position+r; o = softmax(q.K^T / 16) V in fp32 (queries exact to 2^-21 of a
- * head's largest magnitude, probabilities to 8 significant bits, products on
- * 8-bit matrix instructions, sums of values times up to 2^8), out [rows,
- * q_heads, 256] = bf16(o), or with gate (q_proj rows [rows, q_heads, 512],
- * optional) bf16(o * sigmoid(gate)), gate the second half of each head. query
- * [rows, q_heads, 256] bf16. Pointers 16-byte aligned, rows * q_heads <= 2^22.
- * out must not alias query or gate; scratch must not be used by two
- * calls at once. */
+ * head's largest magnitude, where that is at least 2^-92, probabilities to 8
+ * significant bits, products on 8-bit matrix instructions, sums of values times
+ * up to 2^8), out [rows, q_heads, 256] = bf16(o), or with gate (q_proj rows
+ * [rows, q_heads, 512], optional) bf16(o * sigmoid(gate)), gate the second half
+ * of each head. query [rows, q_heads, 256] bf16. Pointers 16-byte aligned, rows *
+ * q_heads <= 2^22. out must not alias query or gate; scratch must not be used by
+ * two calls at once.
+ * The 32 positions 16 j + 0 .. 7 of a block, and the 32 others, share a power of
+ * two: a probability below 2^-13 of the largest of its 32 is kept to 2^-22 of
+ * that one only, unless that one's eight alone outweighs the other 24 by 2^13:
+ * these then count by the largest among them. */
 int es_attn_kv8(const uint16_t* query, int q_heads, const es_kv8* cache, int position, int rows,
                 const uint16_t* gate, void* scratch, size_t scratch_bytes, uint16_t* out, void* stream);
 

@@ -115,3 +115,28 @@ def test_many_rows_with_scores_that_differ_and_sinks_with_values(group, heads, r
 def test_many_rows_with_a_rest_far_below(group, heads, rows, n, nats):
     """The rest keeps its eight bits however far it lies below, as far as the sink has no value."""
     check(Keys(n, nats, 0.0, 0.0), heads, group, rows)
+
+
+FEW = [(4, 2, 1, 700), (4, 2, 1, 1024), (8, 1, 1, 1024), (8, 1, 1, 4096), (4, 8, 1, 20011), (4, 2, 1, 131072), (1, 32, 1, 16384),
+       (1, 128, 1, 131072), (4, 2, 12, 4096), (4, 2, 40, 20040), (4, 2, 128, 28800), (8, 1, 100, 16384), (1, 256, 80, 80),
+       (4, 2, 30, 640)]
+
+
+@pytest.mark.parametrize("nats", NATS)
+@pytest.mark.parametrize("group,heads,rows,n", FEW)
+def test_few_rows_behind_a_sink_without_value(group, heads, rows, n, nats):
+    check(Keys(n, nats, 0.0, 0.0), heads, group, rows)
+
+
+@pytest.mark.parametrize("nats,spread,sink,at", SPREAD)
+@pytest.mark.parametrize("group,heads,rows,n", [(4, 2, 1, 1024), (4, 8, 1, 20011), (4, 2, 40, 20040), (1, 128, 2, 65536),
+                                                (4, 8, 20, 700)])
+def test_few_rows_with_scores_that_differ_and_sinks_with_values(group, heads, rows, n, nats, spread, sink, at):
+    check(Keys(n, nats, spread, sink, min(at, n - rows)), heads, group, rows)
+
+
+@pytest.mark.parametrize("nats", [22, 30, 38])
+@pytest.mark.parametrize("group,heads,rows,n", [(4, 2, 1, 128), (4, 2, 1, 4096), (4, 2, 130, 900)])
+def test_few_rows_with_a_rest_far_below(group, heads, rows, n, nats):
+    """The rest keeps its eight bits however far it lies below, as far as the sink has no value."""
+    check(Keys(n, nats, 0.0, 0.0), heads, group, rows)
