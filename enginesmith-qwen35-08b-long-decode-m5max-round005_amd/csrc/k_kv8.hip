@@ -121,7 +121,7 @@ __device__ __forceinline__ float2 angle_cs(int position, float inv) {
 // The same of a row of K, in 64 bits up to its e4m3: a code is decided by the last
 // bits of a value at a boundary between two (one in four million is within 32 bits'
 // rounding of one). The sum of squares, the root by one Newton step, a dim times its gain
-// (exact in 32 bits, eight significant ones each), the angles.
+// (which 32 bits do not always hold), the angles.
 template <int CTRL>
 __device__ __forceinline__ double dpp64(double v) {
   const i32x2 w = __builtin_bit_cast(i32x2, v);
@@ -167,7 +167,7 @@ __device__ __forceinline__ void prepare_key(float* x, const float* gain, const d
   const double2* t = c < 4 ? cs + (c & 1) * 16 : none;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const double y = (double)(x[i] * gain[i]) * inv, other = dpp64<0x4E>(y);
+    const double y = (double)x[i] * (double)gain[i] * inv, other = dpp64<0x4E>(y);
     x[i] = to_odd(fma(y, t[i].x, (c < 2 ? -other : other) * t[i].y));
   }
 }
