@@ -90,12 +90,23 @@ __device__ __forceinline__ void load16(const uint16_t* p, float* x) {
   unpack16(v[0], v[1], x);
 }
 
-// RMS norm of a 256-wide head in 32 bits, 16 dims in each lane of a row of 16.
+// RMS norm of a 256-wide head in 32 bits, 16 dims in each lane of a row of 16. Where
+// the sum of squares passes their range the head is taken times 2^-70, which leaves nothing of the epsilon.
 __device__ __forceinline__ void norm16(float* x, const float* gain) {
-  float ss = 0.0f;
+  auto mean = [&]() {
+    float ss = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
-  const float inv = 1.0f / sqrtf(tree16(ss) * (1.0f / 256.0f) + 1e-6f);
+    for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
+    return tree16(ss) * (1.0f / 256.0f);
+  };
+  float ms = mean() + 1e-6f;
+  if (__any(!finite(ms))) {
+    const float down = finite(ms) ? 1.0f : 0x1p-70f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] *= down;
+    ms = mean() + 1e-6f * down * down;
+  }
+  const float inv = 1.0f / sqrtf(ms);
 #pragma unroll
   for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * gain[i];
 }

@@ -50,3 +50,18 @@ def test_keys_of_any_magnitude(rows, kind, gain):
     power = np.exp2(cache.k_scale.numpy(np.uint8).reshape(2, -1).astype(float) - 127).repeat(64, 1)[:, :rows].T[:, :, None]
     # half a step of the code, or of the subnormals' at the block's power of two
     assert (np.abs(got - want) <= 2.0 ** -4 * np.abs(want) * (1 + 2.0 ** -20) + 2.0 ** -10 * power).all()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 70])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("gain", [1.0, 3.0])
+def test_queries_of_any_magnitude(rows, kind, gain):
+    r = rng(50 + rows)
+    _, k, v, qg, kg = projections(r, rows, 8, 2)
+    qg = bf16(f32(qg) * np.float32(gain))
+    q = large(r, rows, 8, 2 * DIM, kind)
+    got = f64(prepare(kv8.new_cache(2, rows), q, k, v, qg, kg, 0))
+    want = rotated(q[..., :DIM], qg, 0, E.rope_inv_freq())
+    # the output's rounding, and 32-bit arithmetic: sums of 256 squares, a dozen roundings, an angle's series
+    size = np.sqrt((want ** 2).mean(-1, keepdims=True)) * 8
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 64 * 2.0 ** -24 * size).all()
