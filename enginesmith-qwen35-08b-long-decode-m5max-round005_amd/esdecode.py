@@ -246,7 +246,7 @@ class DeviceQ4:
 
 
 class DeviceKV8:
-    """A key/value cache in 8 bits resident on the device (es_kv8)."""
+    """A key/value cache in 8 bits resident on the device (es_kv8), all its blocks without rows."""
 
     BLOCK = 64
 
@@ -256,6 +256,9 @@ class DeviceKV8:
         n = self.heads * self.blocks
         self.k, self.v = DeviceBuffer(n * self.BLOCK * 256), DeviceBuffer(n * self.BLOCK * 256)
         self.k_scale, self.v_scale = DeviceBuffer(n), DeviceBuffer(n)
+        for b in (self.k_scale, self.v_scale):
+            b.fill(255)
+        synchronize()  # streams of their own do not wait for the fills
         self.struct = KV8(self.k.ptr, self.v.ptr, self.k_scale.ptr, self.v_scale.ptr, self.heads, self.capacity)
 
 

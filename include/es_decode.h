@@ -311,8 +311,10 @@ int es_attn_decode(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_
  * smallest power (2^-127 at least) that brings the block's largest finite
  * magnitude to at most 448. With blocks = (capacity + 63) / 64: k and v hold
  * [heads, blocks, 16384] codes (16-byte aligned), k_scale and v_scale [heads,
- * blocks] bytes, device memory of the caller, which needs no initialisation. In
- * a block the codes lie in the order of the matrix instructions:
+ * blocks] bytes, device memory of the caller. The codes need no initialisation;
+ * the scale bytes are 255 before a block's first write (a block without rows),
+ * unless that write starts at the block's first position. In a block the codes
+ * lie in the order of the matrix instructions:
  *   k [position/32 %2][d/64][d/16 %2][d/32 %2][position %32][d %16]
  *   v [d/32][position/8 %2][position/4 %2][d %32][position/16 %4][position %4]
  * heads 1 .. 256, capacity 1 .. 2^22.
@@ -322,8 +324,8 @@ int es_attn_decode(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_
  * `position` keeps its power of two if rows of it stay, raised where the new rows
  * need it: its earlier codes are then rounded again, exact except where they
  * become subnormal (below 2^-6 of the power). So rows written one by one get the
- * same powers as rows written at once. Where no row of that block before
- * `position` was ever written, its scale bytes must be 255 (a block without rows).
+ * same powers as rows written at once. Scale bytes of anything but 255 are taken
+ * for the power of rows before `position`, whether there are any or not.
  *
  * A position whose K or V row of a head holds a NaN or an infinity is stored as
  * NaN: it reads back as NaN throughout, and every query that attends to it
