@@ -208,7 +208,7 @@ __device__ __forceinline__ void prepare_query(const Kv8Prep& p, size_t at, const
 // Memory bounds it: 131072 rows of 2 heads, 403 MB, take 77 us (5.2 TB/s, what a
 // large copy reaches). Prepare of 4096 rows, 8 query and 2 KV heads: 46 MB in
 // 15 us (alone the queries 10.4, the keys with their 64-bit arithmetic on half of the
-// CUs 12).
+// CUs 12, when their product with the gain was in 32 bits).
 constexpr int kVPad = kBlockBytes + (kBlockBytes / 256) * 16;
 __device__ __forceinline__ int v_lds(int byte) { return byte + (byte >> 8) * 16; }
 
@@ -588,7 +588,7 @@ constexpr int kOne = 127, kLo = 127 - 4, kProb = 127 - 4;  // scale operands, 2^
 // For the rest of those 32 themselves: where their largest outweighs the other three of its four
 // eights by 2^kAlone, what is at most the largest of these takes a product of its
 // own, at a power of two by that one. (For every block with a key 2^18 below its largest a
-// prompt chunk took 4 % longer at scores of unit deviation and 24 % at a deviation of two, so 2 and 3 %.)
+// prompt chunk took 4 % longer at scores of unit deviation and 24 % at a deviation of two, so 2 and 3.)
 constexpr float kRest = 0.03125f, kMostShift = kProb - 5, kNoShift = -2.0f, kMostRef = 0x1p18f, kAlone = 13.0f;
 constexpr int kRestScale = -5, kNever = 500;
 // Exponent of a power of two by the logarithm, less m, of what comes to 2^7 .. 2^8: the most where there
@@ -646,9 +646,9 @@ __device__ __forceinline__ void lds_barrier() {
 // powers of two of 32 keys and the reference, and the block before's probabilities. What bounds a
 // short context is how many bytes each CU must fetch (measured 20 a cycle), a long one memory
 // (131072 tokens, 2 heads: 134 MB in 25 us, 5.3 TB/s), many queries the products and
-// exponentials of four waves on a SIMD. (Probabilities before the barrier, at one power
-// of two, with 8 query and 2 KV heads: 1000 rows alone 14.3 us and 15.8 so, 128 behind 28672 45.6 and 50.2, one
-// behind 131071 28.4 and 28.9.)
+// exponentials of four waves on a SIMD. (Probabilities before the barrier, at one power of
+// two for all keys, with 8 query and 2 KV heads: 1000 rows alone 14.2 us and 15.8 so, 128 behind 28672
+// 44.2 and 48.8, one behind 131071 28.4 and 28.9.)
 // The next block's K is fetched as soon as this one's products have read it, its V
 // likewise: 32 KB of a group on their way.
 // The bound of 1024 threads holds for every G: it keeps the compiler to the 128
@@ -1136,8 +1136,8 @@ __device__ __forceinline__ void wait_vmcnt() {
 // matrix core while the other works on its softmax. K and V reach LDS by DMA, in the
 // order of the operands, two to three phases ahead; the queries' lower part stays in
 // LDS, as registers are full: 128 of sums, 24 of queries, 32 of scores, operands.
-// Measured: 4096 rows behind 28672, 8 query and 2 KV heads, 832 to 870 us by the card (1.0e12
-// operations, 1.2e15 a second; 2 % less before the powers of two of 32 keys). A phase takes 3100
+// Measured: 4096 rows behind 28672, 8 query and 2 KV heads, 803 to 870 us by the card (1.0e12
+// operations, 1.2e15 a second; 2 % less with one power of two for all keys). A phase takes 3100
 // cycles, 2048 of them of the matrix core, and with all 256 CUs at it the clock falls from 2.4 to
 // 1.9 GHz. Four waves with 32 queries and
 // all keys each, the same steps interleaved within a wave, took 3530 cycles; eight
@@ -1486,8 +1486,8 @@ constexpr int kRowLeast = 96;  // pairs of a head from which on 128-pair blocks 
 //   rows: 1.28 for 64 keys of 128 pairs with a CU of its own, up to 1.6 when all CUs are
 //     at it (the clock falls), 10 a round; with ranges 6, and writing and joining them
 // Measured, 8 query and 2 KV heads where not said otherwise: 500 rows alone 8 us with 16 pairs
-// a block and 14 with 32; 1000 alone 21 and 16; 32 rows behind 70000 43 and 34, rows 47
-// with 128 ranges; 128 behind 28672 57, 49 and rows 57 with 32; 512 behind 28672 few 146,
+// a block and 14 with 32; 1000 alone 19 and 16; 32 rows behind 70000 40 and 34, rows 47
+// with 128 ranges; 128 behind 28672 49, 48 and rows 57 with 32; 512 behind 28672 few 146,
 // rows 119 with eight; 2048 behind 30000 few 568, rows 663 with one, 435 with two; 4200
 // behind 28672 few 1273, rows 1304 with one and 1010 with three; 700 behind 20000, 32 and
 // 8 heads, 557, 444 with one; 4096 alone 111 and 107.
