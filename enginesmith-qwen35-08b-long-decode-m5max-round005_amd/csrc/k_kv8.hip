@@ -769,8 +769,8 @@ __global__ __launch_bounds__(1024) void k_kv8_attn_few(Kv8 c, Kv8Attn a) {
 #pragma unroll
     for (int i = from; i < 4; ++i) w[i] = __builtin_shufflevector(at[i * 128], at[i * 128 + 64], 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  // One tile's upper parts stay in registers, all of them before the lower parts were read again here:
-  // 40 rows behind 20000 18.2 us, 18.4 with half of them, 19.1 with none.
+  // One tile's upper parts stay in registers, which have no room for the lower ones too (40 rows behind
+  // 20000 18.4 us, 19.1 with none).
   i32x8 w[4];
   if constexpr (NT == 1) queries(0, w, 0);
   // largest scores of a query in a block: [first or second 8 of every 16 tokens][wave]

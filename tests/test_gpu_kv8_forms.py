@@ -56,3 +56,29 @@ def test_every_form_gives_every_row_and_head_its_own(hq, hk, rows, position):
     # probabilities of eight bits, all alike and so all off the same way, sums of n in 32 bits, the output's rounding
     assert (np.abs(got[..., :1] - 1) <= 2.0 ** -8 * 2 + n * 2.0 ** -24).all()
     assert (np.abs(got[..., 1:] - share) <= (2.0 ** -8 * 2 + n * 2.0 ** -24) * share).all()
+
+
+@pytest.mark.parametrize("hq,hk,rows,position", [(8, 2, 1, 500), (8, 2, 1, 3000), (8, 2, 40, 5000), (32, 8, 131, 64), (8, 2, 9, 30000),
+                                                 (32, 8, 700, 300), (8, 2, 2048, 6000)])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("size", [8, 11, 14, 16])
+def test_large_scores_pick_the_largest(hq, hk, rows, position, sign, size):
+    """Scores of 2^size to 2^(size + 10), all of one sign and 32 nats apart at least: every query gets the values of its
+    largest key (or keys: those of one score have the same)."""
+    n = position + rows
+    r = rng(70 + n + size)
+    heights = (np.arange(8, 16) / 8 * 2.0 ** np.arange(10)[:, None]).ravel()[:79]  # e4m3 numbers, 1 to 896
+    which = r.integers(0, 79, n)
+    of_height = kv8.round_e4m3(r.normal(0, 1, (79, DIM)))  # at powers of two of 2^-7 and less what the cache holds
+    k = bf16(np.broadcast_to(heights[which][:, None, None], (n, 1, DIM)))
+    v = bf16(of_height[which][:, None])
+    cache = kv8.new_cache(hk, n, 0xff)
+    dk, dv = E.DeviceBuffer.from_numpy(k), E.DeviceBuffer.from_numpy(v)
+    E.check(E.lib().es_kv8_write(cache.struct, dk.ptr, dv.ptr, DIM, 0, 0, n, None))
+    E.synchronize()
+    q = bf16(np.full((rows, hq, DIM), sign * 2.0 ** (size - 4)))  # score: q height 256 / 16
+    got = f32(kv8.attend(cache, q, position)).astype(np.float64)
+    best = (np.maximum if sign > 0 else np.minimum).accumulate(which)[position:]
+    want = of_height[best][:, None]
+    # a probability's eight bits and the output's rounding
+    assert (np.abs(got - want) <= 2.0 ** -7 * np.abs(want) + 1e-12).all()
