@@ -64,6 +64,27 @@ bool kv8_heads_fit(int q_heads, int kv_heads, int rows) {
   return q_heads >= 1 && kv_heads >= 1 && q_heads % kv_heads == 0 && rows >= 1 && (int64_t)rows * q_heads <= (1 << 22);
 }
 
+// The nodes of a tree, and the context before them; "" when they hold.
+const char* tree_fault(const uint64_t* paths, int rows) {
+  if (!paths || (uintptr_t)paths & 7) return "paths must be an 8-byte aligned pointer";
+  if (rows < 1 || rows > es::kTree) return "rows 1 .. 64 required";
+  return "";
+}
+const char* tree_cache_fault(const uint16_t* kcache, const uint16_t* vcache, int kv_heads, int capacity, int position) {
+  if (!kcache || !vcache) return "null argument";
+  if (kv_heads < 1 || kv_heads > 256) return "kv_heads 1 .. 256 required";
+  if (capacity < 1 || capacity > (1 << 22) || position < 0 || position > capacity)
+    return "capacity 1 .. 2^22 and position 0 .. capacity required";
+  return "";
+}
+bool tree_heads_fit(int q_heads, int kv_heads) {
+  return kv_heads >= 1 && kv_heads <= 256 && q_heads >= 1 && q_heads <= 1024 && q_heads % kv_heads == 0;
+}
+bool logprob_fits(int rows, int vocab, int top) {
+  return rows >= 1 && rows <= (1 << 20) && vocab >= 1 && vocab <= (1 << 22) && top >= 0 && top <= es::kLogprobTop &&
+         top <= vocab;
+}
+
 hipStream_t S(void* s) { return static_cast<hipStream_t>(s); }
 
 int engine_rc(int rc, const std::string& err) {
@@ -519,6 +540,150 @@ int es_attn_kv8(const uint16_t* query, int q_heads, const es_kv8* cache, int pos
   a.position = position;
   a.rows = rows;
   return hip_status(es::launch_kv8_attn(to_kv8(cache), a, S(stream)), "es_attn_kv8");
+}
+
+// ---- trees of drafted tokens ----
+static_assert(ES_TREE_MAX == es::kTree, "the header's limit is the kernels'");
+
+int es_tree_paths(const int32_t* parents, int rows, uint64_t* paths) {
+  if (!parents || !paths) return fail(ES_ERR_INVALID, "es_tree_paths: null argument");
+  if (rows < 1 || rows > ES_TREE_MAX) return fail(ES_ERR_INVALID, "es_tree_paths: rows 1 .. 64 required");
+  for (int i = 0; i < rows; ++i)
+    if (parents[i] < -2 || parents[i] >= i)
+      return fail(ES_ERR_INVALID, "es_tree_paths: parents[" + std::to_string(i) + "] must be a node before it, -1 or -2");
+  for (int i = 0; i < rows; ++i) {
+    const int up = parents[i];
+    paths[i] = up == -2 || (up >= 0 && !paths[up]) ? 0 : uint64_t(1) << i | (up >= 0 ? paths[up] : 0);
+  }
+  return ES_OK;
+}
+
+size_t es_attn_tree_scratch_bytes(int q_heads, int kv_heads, int rows) {
+  if (!tree_heads_fit(q_heads, kv_heads) || rows < 1 || rows > es::kTree) return 0;
+  return es::tree_attn_scratch_bytes(q_heads, kv_heads, rows);
+}
+
+int es_attn_tree(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t* v_proj, const uint16_t* q_gain,
+                 const uint16_t* k_gain, const float* inv_freq, const uint64_t* paths, int rows, int q_heads,
+                 int kv_heads, const uint16_t* kcache, const uint16_t* vcache, int capacity, int position,
+                 void* scratch, size_t scratch_bytes, uint16_t* k_tree, uint16_t* gated, void* stream) {
+  const char* fault = tree_fault(paths, rows);
+  if (!*fault) fault = tree_cache_fault(kcache, vcache, kv_heads, capacity, position);
+  if (*fault) return fail(ES_ERR_INVALID, std::string("es_attn_tree: ") + fault);
+  if (!q_proj || !k_proj || !v_proj || !q_gain || !k_gain || !inv_freq || !k_tree || !gated)
+    return fail(ES_ERR_INVALID, "es_attn_tree: null argument");
+  if (!tree_heads_fit(q_heads, kv_heads))
+    return fail(ES_ERR_INVALID, "es_attn_tree: q_heads a multiple of kv_heads and at most 1024 required");
+  if (!aligned16({q_proj, k_proj, v_proj, q_gain, k_gain, inv_freq, kcache, vcache, scratch, k_tree, gated}))
+    return fail(ES_ERR_INVALID, "es_attn_tree: pointers must be 16-byte aligned");
+  if (gated == q_proj || gated == k_proj || gated == v_proj || gated == k_tree || k_tree == q_proj || k_tree == k_proj ||
+      k_tree == v_proj)
+    return fail(ES_ERR_INVALID, "es_attn_tree: k_tree and gated must not alias the projections or each other");
+  if (!scratch || scratch_bytes < es::tree_attn_scratch_bytes(q_heads, kv_heads, rows))
+    return fail(ES_ERR_INVALID, "es_attn_tree: scratch smaller than es_attn_tree_scratch_bytes(q_heads, kv_heads, rows)");
+  es::TreeAttn a{};
+  a.q_proj = q_proj;
+  a.k_proj = k_proj;
+  a.v_proj = v_proj;
+  a.q_gain = q_gain;
+  a.k_gain = k_gain;
+  a.inv_freq = inv_freq;
+  a.paths = paths;
+  a.rows = rows;
+  a.q_heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.kcache = kcache;
+  a.vcache = vcache;
+  a.capacity = capacity;
+  a.position = position;
+  a.scratch = scratch;
+  a.k_tree = k_tree;
+  a.gated = gated;
+  return hip_status(es::launch_tree_attn(a, S(stream)), "es_attn_tree");
+}
+
+int es_kv_tree_keep(const uint16_t* k_tree, const uint16_t* v_proj, const uint64_t* paths, int node, int rows,
+                    int kv_heads, uint16_t* kcache, uint16_t* vcache, int capacity, int position, void* stream) {
+  const char* fault = tree_fault(paths, rows);
+  if (!*fault) fault = tree_cache_fault(kcache, vcache, kv_heads, capacity, position);
+  if (*fault) return fail(ES_ERR_INVALID, std::string("es_kv_tree_keep: ") + fault);
+  if (!k_tree || !v_proj) return fail(ES_ERR_INVALID, "es_kv_tree_keep: null argument");
+  if (node < 0 || node >= rows || position >= capacity)
+    return fail(ES_ERR_INVALID, "es_kv_tree_keep: node 0 .. rows-1 and a position below the capacity required");
+  if (!aligned16({k_tree, v_proj, kcache, vcache}))
+    return fail(ES_ERR_INVALID, "es_kv_tree_keep: pointers must be 16-byte aligned");
+  const es::TreeKeepKv a{k_tree, v_proj, paths, node, kv_heads, kcache, vcache, capacity, position};
+  return hip_status(es::launch_tree_keep_kv(a, S(stream)), "es_kv_tree_keep");
+}
+
+int es_gdn_tree(const uint16_t* raw, const uint16_t* ring, const uint16_t* conv_w, const uint16_t* a_proj,
+                const uint16_t* b_proj, const float* a_log, const uint16_t* dt_bias, const uint64_t* paths,
+                int position, int rows, const float* state, uint16_t* y, float* keys, float* updates,
+                float* log_decay, void* stream) {
+  const char* fault = tree_fault(paths, rows);
+  if (*fault) return fail(ES_ERR_INVALID, std::string("es_gdn_tree: ") + fault);
+  if (!raw || !ring || !conv_w || !a_proj || !b_proj || !a_log || !dt_bias || !state || !y || !keys || !updates || !log_decay)
+    return fail(ES_ERR_INVALID, "es_gdn_tree: null argument");
+  if (position < 0) return fail(ES_ERR_INVALID, "es_gdn_tree: position >= 0 required");
+  if (!aligned16({raw, ring, conv_w, a_proj, b_proj, a_log, dt_bias, state, y, keys, updates, log_decay}))
+    return fail(ES_ERR_INVALID, "es_gdn_tree: pointers must be 16-byte aligned");
+  if (keys == updates || keys == state || updates == state || y == raw)
+    return fail(ES_ERR_INVALID, "es_gdn_tree: outputs must not alias the inputs or each other");
+  const es::TreeGdn a{raw, ring, conv_w, a_proj, b_proj, a_log, dt_bias, paths, position, rows, state, y, keys, updates, log_decay};
+  return hip_status(es::launch_tree_gdn(a, S(stream)), "es_gdn_tree");
+}
+
+int es_gdn_tree_keep(const uint16_t* raw, const float* keys, const float* updates, const float* log_decay,
+                     const uint64_t* paths, int node, int rows, int position, uint16_t* ring, const float* state,
+                     float* state_out, void* stream) {
+  const char* fault = tree_fault(paths, rows);
+  if (*fault) return fail(ES_ERR_INVALID, std::string("es_gdn_tree_keep: ") + fault);
+  if (!raw || !keys || !updates || !log_decay || !ring || !state || !state_out)
+    return fail(ES_ERR_INVALID, "es_gdn_tree_keep: null argument");
+  if (node < 0 || node >= rows || position < 0)
+    return fail(ES_ERR_INVALID, "es_gdn_tree_keep: node 0 .. rows-1 and position >= 0 required");
+  if (!aligned16({raw, keys, updates, log_decay, ring, state, state_out}))
+    return fail(ES_ERR_INVALID, "es_gdn_tree_keep: pointers must be 16-byte aligned");
+  if (state_out == keys || state_out == updates || raw == ring)
+    return fail(ES_ERR_INVALID, "es_gdn_tree_keep: outputs must not alias the draft's tensors");
+  const es::TreeKeepGdn a{raw, keys, updates, log_decay, paths, node, position, ring, state, state_out};
+  return hip_status(es::launch_tree_keep_gdn(a, S(stream)), "es_gdn_tree_keep");
+}
+
+// ---- scores of logits ----
+size_t es_logprob_scratch_bytes(int rows, int vocab, int top) {
+  return logprob_fits(rows, vocab, top) ? es::logprob_scratch_bytes(rows, vocab, top) : 0;
+}
+
+int es_logprob_rows(const uint16_t* logits, int64_t row_stride, int rows, int vocab, const uint32_t* tokens, int top,
+                    void* scratch, size_t scratch_bytes, float* logprob, float* entropy, float* lse,
+                    uint32_t* top_ids, float* top_logprobs, void* stream) {
+  if (!logits || (uintptr_t)logits & 1) return fail(ES_ERR_INVALID, "es_logprob_rows: logits null or not 2-byte aligned");
+  if (!logprob_fits(rows, vocab, top))
+    return fail(ES_ERR_INVALID, "es_logprob_rows: rows 1 .. 2^20, vocab 1 .. 2^22, top 0 .. min(32, vocab) required");
+  if (row_stride < vocab || row_stride > (int64_t(1) << 40))
+    return fail(ES_ERR_INVALID, "es_logprob_rows: row_stride vocab .. 2^40 required");
+  if (!logprob != !tokens) return fail(ES_ERR_INVALID, "es_logprob_rows: tokens and logprob go together");
+  if ((top > 0) != (top_ids != nullptr) || (top > 0) != (top_logprobs != nullptr))
+    return fail(ES_ERR_INVALID, "es_logprob_rows: top_ids and top_logprobs go with top > 0");
+  if (!logprob && !entropy && !lse && !top) return fail(ES_ERR_INVALID, "es_logprob_rows: no output");
+  const size_t need = es::logprob_scratch_bytes(rows, vocab, top);
+  if (!aligned16({scratch}) || (need && (!scratch || scratch_bytes < need)))
+    return fail(ES_ERR_INVALID, "es_logprob_rows: scratch smaller than es_logprob_scratch_bytes(rows, vocab, top) or not 16-byte aligned");
+  es::LogprobArgs a{};
+  a.logits = logits;
+  a.stride = row_stride;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.top = top;
+  a.tokens = tokens;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.lse = lse;
+  a.top_ids = top_ids;
+  a.top_logprobs = top_logprobs;
+  a.scratch = scratch;
+  return hip_status(es::launch_logprob(a, S(stream)), "es_logprob_rows");
 }
 
 // ---- head ----

@@ -371,4 +371,74 @@ hipError_t launch_kv8_read(const Kv8& c, int position, int rows, uint16_t* k, ui
                            int64_t head_stride, hipStream_t s);
 hipError_t launch_kv8_attn(const Kv8& c, Kv8Attn a, hipStream_t s);
 
+// ---- scores of logits, k_logprob.hip ----
+// Callers check shapes, alignment and bounds; the launchers do not.
+constexpr int kLogprobTop = 32;  // most alternatives
+struct LogprobArgs {
+  const uint16_t* logits;
+  int64_t stride;
+  int rows, vocab, top;
+  const uint32_t* tokens;
+  float *logprob, *entropy, *lse;  // each optional
+  uint32_t* top_ids;
+  float* top_logprobs;
+  void* scratch;
+  int ranges, per;  // ranges of a row and 8-element vectors of each (by the launcher)
+};
+size_t logprob_scratch_bytes(int rows, int vocab, int top);
+hipError_t launch_logprob(LogprobArgs a, hipStream_t s);
+
+// ---- a tree of drafted tokens, k_tree.hip and k_gdn_tree.hip ----
+// Callers check shapes, alignment and bounds; the launchers do not.
+constexpr int kTree = 64;             // most nodes
+constexpr int kTreePartFloats = 260;  // a range's 256 sums, reference and sum of exponentials, to a multiple of 16 bytes
+// The nodes on node i's path, itself the last; none for a node left out.
+__host__ __device__ inline uint64_t tree_path(uint64_t word, int i) {
+  return word >> i & 1 ? word & ((2ull << i) - 1) : 0;
+}
+struct TreeAttn {
+  const uint16_t *q_proj, *k_proj, *v_proj, *q_gain, *k_gain;
+  const float* inv_freq;
+  const uint64_t* paths;
+  int rows, q_heads, kv_heads;
+  const uint16_t *kcache, *vcache;
+  int capacity, position;
+  void* scratch;
+  uint16_t *k_tree, *gated;
+  uint16_t* query;  // in the scratch, as part (by the launcher, as the rest)
+  float* part;
+  int group, queries, tiles, ranges;
+};
+size_t tree_attn_scratch_bytes(int q_heads, int kv_heads, int rows);
+hipError_t launch_tree_attn(TreeAttn a, hipStream_t s);
+struct TreeKeepKv {
+  const uint16_t *k_tree, *v_proj;
+  const uint64_t* paths;
+  int node, kv_heads;
+  uint16_t *kcache, *vcache;
+  int capacity, position;
+};
+hipError_t launch_tree_keep_kv(const TreeKeepKv& a, hipStream_t s);
+struct TreeGdn {
+  const uint16_t *raw, *ring, *conv_w, *a_proj, *b_proj;
+  const float* a_log;
+  const uint16_t* dt_bias;
+  const uint64_t* paths;
+  int position, rows;
+  const float* state;
+  uint16_t* y;
+  float *keys, *updates, *log_decay;
+};
+hipError_t launch_tree_gdn(const TreeGdn& a, hipStream_t s);
+struct TreeKeepGdn {
+  const uint16_t* raw;
+  const float *keys, *updates, *log_decay;
+  const uint64_t* paths;
+  int node, position;
+  uint16_t* ring;
+  const float* state;
+  float* state_out;
+};
+hipError_t launch_tree_keep_gdn(const TreeKeepGdn& a, hipStream_t s);
+
 }  // namespace es

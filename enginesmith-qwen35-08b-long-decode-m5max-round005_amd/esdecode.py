@@ -107,6 +107,15 @@ _SIGNATURES = {
     "es_attn_kv8_scratch_bytes": (c_size_t, [c_int, c_int, c_int]),
     "es_attn_kv8": (c_int, [c_void_p, c_int, POINTER(KV8), c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p,
                             c_void_p]),
+    "es_tree_paths": (c_int, [c_void_p, c_int, c_void_p]),
+    "es_attn_tree_scratch_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "es_attn_tree": (c_int, [c_void_p] * 7 + [c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_size_t,
+                             c_void_p, c_void_p, c_void_p]),
+    "es_kv_tree_keep": (c_int, [c_void_p] * 3 + [c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "es_gdn_tree": (c_int, [c_void_p] * 8 + [c_int, c_int] + [c_void_p] * 6),
+    "es_gdn_tree_keep": (c_int, [c_void_p] * 5 + [c_int, c_int, c_int] + [c_void_p] * 4),
+    "es_logprob_scratch_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "es_logprob_rows": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_size_t] + [c_void_p] * 6),
     "es_weights_tensor_shape": (c_int, [c_int, c_int, c_int, POINTER(ctypes.c_int64), c_int]),
     "es_checkpoint_config": (c_int, [c_char_p, POINTER(c_int), POINTER(c_int)]),
     "es_checkpoint_load": (c_int, [c_char_p, c_int, c_int, c_void_p, c_size_t]),
@@ -472,6 +481,14 @@ def time_copy(nbytes: int, reps: int = 10) -> float:
         src.close()
         dst.close()
     return ms.value
+
+
+def tree_paths(parents) -> np.ndarray:
+    """Path words of a tree of drafted tokens (es_tree_paths): uint64, for the operators' `paths`."""
+    parents = np.ascontiguousarray(parents, dtype=np.int32)
+    out = np.zeros(parents.size, dtype=np.uint64)
+    check(lib().es_tree_paths(_ptr(parents), parents.size, _ptr(out)))
+    return out
 
 
 def rope_inv_freq() -> np.ndarray:

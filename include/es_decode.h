@@ -390,6 +390,86 @@ int es_attn_kv8(const uint16_t* query, int q_heads, const es_kv8* cache, int pos
                 const uint16_t* gate, void* scratch, size_t scratch_bytes, uint16_t* out, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* Trees of drafted tokens                                             */
+/* ------------------------------------------------------------------ */
+/* Checking up to ES_TREE_MAX drafted tokens in one pass, instead of a decode
+ * step for each: the layers' operators over a tree of tokens behind `position`
+ * consumed ones, and those that bring cache and state behind an accepted path.
+ * No reference counterpart. Rows are nodes; projections, MLP and head of the rows
+ * are the row operators' (es_q4_matvec_rows, es_q4_gemm, ...).
+ *
+ * paths [rows] (device, 8-byte aligned): bit j of word i says that node j is node i
+ * or one of its ancestors, which come before it (es_tree_paths makes the words
+ * from parents). A node's position is `position` + the number of its ancestors.
+ * Bits above i count for nothing, and a word without bit i leaves the node out: its
+ * outputs are zeros, whatever its inputs hold, and no other node may have it on
+ * its path. Infinities and NaN of a node reach only the nodes whose path holds it.
+ *
+ * A draft's pass: for each layer es_attn_tree or es_gdn_tree, which change neither
+ * cache nor state; for the accepted node's path es_kv_tree_keep or
+ * es_gdn_tree_keep with what they left; the next position is `position` + the
+ * path's length. */
+#define ES_TREE_MAX 64
+
+/* Path words of a tree, on the host: parents[i] is a node before i, -1 (behind the
+ * last consumed token) or -2 (left out, as are nodes behind it). rows 1 ..
+ * ES_TREE_MAX. */
+int es_tree_paths(const int32_t* parents, int rows, uint64_t* paths);
+
+/* Scratch bytes of es_attn_tree for these heads and this number of rows, at any
+ * position and capacity (0 for bad arguments). More rows can need less: a buffer
+ * for several numbers takes the largest. */
+size_t es_attn_tree_scratch_bytes(int q_heads, int kv_heads, int rows);
+
+/* es_attn_prepare_rows, attention and es_attn_gate_rows for a tree: node i's query
+ * = RoPE(RMSNorm(q head) * q_gain) and its key k_tree [rows, kv_heads, 256] =
+ * RoPE(RMSNorm(k head) * k_gain), both rounded to bf16; it attends to rows 0 ..
+ * position-1 of kcache/vcache [kv_heads, capacity, 256] and to the nodes of its
+ * path (keys k_tree, values v_proj); gated [rows, q_heads, 256] = bf16(o *
+ * sigmoid(gate)), o = softmax(q.K^T / 16) V. q_proj [rows, q_heads, 512]
+ * (query|gate), k_proj, v_proj [rows, kv_heads, 256], inv_freq 32 device floats;
+ * query head h reads KV head h / (q_heads / kv_heads). Norms and angles in 64 bits
+ * up to 32, softmax in 32, the probabilities rounded to bf16 for the products, eps
+ * 1e-6. rows 1 .. ES_TREE_MAX, kv_heads 1 .. 256, q_heads a multiple of it up to
+ * 1024, capacity 1 .. 2^22, position 0 .. capacity. Pointers 16-byte aligned,
+ * outputs apart from the inputs. Scratch must not be used by two calls at once. */
+int es_attn_tree(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t* v_proj, const uint16_t* q_gain,
+                 const uint16_t* k_gain, const float* inv_freq, const uint64_t* paths, int rows, int q_heads,
+                 int kv_heads, const uint16_t* kcache, const uint16_t* vcache, int capacity, int position,
+                 void* scratch, size_t scratch_bytes, uint16_t* k_tree, uint16_t* gated, void* stream);
+
+/* K and V rows of an accepted path into the cache: rows position, position + 1, ...
+ * take the rows of `node`'s path in k_tree and v_proj [rows, kv_heads, 256], in order.
+ * Rows from the capacity on are dropped; nothing else changes. node 0 .. rows-1, as
+ * for es_attn_tree otherwise (position below the capacity). */
+int es_kv_tree_keep(const uint16_t* k_tree, const uint16_t* v_proj, const uint64_t* paths, int node, int rows,
+                    int kv_heads, uint16_t* kcache, uint16_t* vcache, int capacity, int position, void* stream);
+
+/* es_gdn_prepare_rows and es_gdn_recur_rows for a tree, state [16, 128v, 128k] fp32
+ * and ring [4, 6144] left as they are: raw [rows, 6144] projected q|k|v, a_proj,
+ * b_proj [rows, 16]; the convolution runs along a node's path (its ancestors'
+ * raw rows, then the ring's), SiLU, q = L2 norm * 128^-1/2, k = L2 norm (eps 1e-6),
+ * log g = -exp(A_log) softplus(a + dt_bias), beta = sigmoid(b), and with S the state
+ * behind the node's parent u = beta (v - g S k), S' = g S + u k^T, y [rows, 2048] =
+ * bf16(S' q). keys and updates [rows, 16, 128] fp32 take k and u, log_decay [rows, 16]
+ * fp32 log g, as es_gdn_tree_keep wants them. In fp32 (squares of the norms and sums
+ * of log g in 64 bits), without the reference's roundings to bf16 on the way.
+ * position >= 0, rows 1 .. ES_TREE_MAX; pointers 16-byte aligned, outputs apart
+ * from each other and the inputs. */
+int es_gdn_tree(const uint16_t* raw, const uint16_t* ring, const uint16_t* conv_w, const uint16_t* a_proj,
+                const uint16_t* b_proj, const float* a_log, const uint16_t* dt_bias, const uint64_t* paths,
+                int position, int rows, const float* state, uint16_t* y, float* keys, float* updates,
+                float* log_decay, void* stream);
+
+/* State and ring behind an accepted path: state_out (may be state) = S' of `node`
+ * above, from what es_gdn_tree left, and the ring's slots of the path's last four
+ * positions take their raw rows. A node left out changes nothing. node 0 ..
+ * rows-1; position and rows as for es_gdn_tree. */
+int es_gdn_tree_keep(const uint16_t* raw, const float* keys, const float* updates, const float* log_decay,
+                     const uint64_t* paths, int node, int rows, int position, uint16_t* ring, const float* state,
+                     float* state_out, void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Vocab head (head_lse.metal:11-98 with rms_norm_bf16, model.rs:290-300) */
 /* ------------------------------------------------------------------ */
 /* Scratch for es_head_greedy: per-block (max, sum exp) partials. */
@@ -414,6 +494,26 @@ int es_head_greedy(const es_q4* embed, const uint16_t* h, const uint16_t* gain,
 #define ES_HEAD_NOALLOC_MAX_VOCAB 1048576
 int es_head_greedy_noalloc(const es_q4* embed, const uint16_t* h, const uint16_t* gain, uint16_t* norm_out,
                            uint16_t* logits, uint32_t* token, float* lse, void* stream);
+
+/* Scratch bytes of es_logprob_rows (0 where it needs none, or for bad arguments).
+ * More rows can need less: a buffer for several numbers takes the largest. */
+size_t es_logprob_scratch_bytes(int rows, int vocab, int top);
+
+/* Scores of rows of bf16 logits, row r at logits + r * row_stride (elements, at
+ * least vocab; no alignment needed): logprob[r] = log softmax(row)[tokens[r]],
+ * entropy[r] = -sum of p log p in nats, lse[r] = log sum exp, and the `top` largest
+ * logits' ids (by value, equal ones by lower id) and log probabilities,
+ * top_ids and top_logprobs [rows, top]. A token excluded by -inf has p = 0. Sums in
+ * fp32 without the largest element's 1, joined in 64 bits. A row that holds a NaN or
+ * +infinity, or nothing but -inf, gets NaN and keeps its ids (NaN ranks below -inf)
+ * and, without a NaN, its lse of +-infinity; so does the log probability of a token
+ * that is not below vocab. logprob (with tokens), entropy and lse are optional;
+ * top 0 .. 32 and at most vocab, 0 without top_ids and top_logprobs. rows 1 .. 2^20,
+ * vocab 1 .. 2^22. scratch 16-byte aligned, not used by two calls at once. No
+ * reference counterpart. */
+int es_logprob_rows(const uint16_t* logits, int64_t row_stride, int rows, int vocab, const uint32_t* tokens, int top,
+                    void* scratch, size_t scratch_bytes, float* logprob, float* entropy, float* lse,
+                    uint32_t* top_ids, float* top_logprobs, void* stream);
 
 /* ------------------------------------------------------------------ */
 /* Model weights (weights.rs:11-44 checks; model.rs:41-78 names)        */
