@@ -23,10 +23,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kTileQ = 128;   // queries of a block: four tiles of 32, each on two waves
 constexpr int kKeys = 32;     // keys of a stage
 constexpr int kStages = 4;
-constexpr int kKRow = 264;    // bf16 elements between K rows in LDS (16 rows x 4 chunks of a read spread over the banks)
-constexpr int kVRow = 288;    // and between V rows (4 rows x 64 bytes of a transposing read)
-constexpr int kStage = kKeys * (kKRow + kVRow);
-constexpr int kHalf = 64 * 130;  // floats that a wave leaves for the other of its tile: 128 sums, reference and sum a lane
+constexpr int kRow = 256;     // bf16 elements between rows in LDS
+constexpr int kStage = 2 * kKeys * kRow;  // K rows, then V rows
+constexpr int kHalf = 64 * 128;  // output sums that a wave leaves for the other of its tile
 
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
@@ -71,29 +70,53 @@ __global__ __launch_bounds__(256) void k_tree_prepare(TreeAttn a) {
 }
 
 // ---- attention ----
-// V^T fragments by transposing reads: eight from one base, keys 0..3 and 4..7 of the
-// lane's eight for four 32-dim tiles at OFF + 64 t. All complete before the statement ends.
-constexpr int kHi = 2 * 4 * kVRow;  // bytes from a key row to the fourth after it
+// Chunk c (16 bytes) of a row lies at slot c ^ (row & 15) of K and c ^ 4 (row & 3) of
+// V, so that the 16 rows of a fragment's read, and the four rows x 64 bytes of a
+// transposing read, cover all banks once.
+//
+// V^T fragments by transposing reads: keys 0..3 and 4..7 of the lane's eight for the
+// four 32-dim tiles whose addresses are a[0..3], OFF bytes on. All complete before
+// the statement ends.
 template <int OFF>
-__device__ __forceinline__ void read_v(uint32_t a, u32x4 (&v)[4]) {
+__device__ __forceinline__ void read_v(const uint32_t (&a)[4], u32x4 (&v)[4]) {
   uint64_t x0, x1, x2, x3, y0, y1, y2, y3;
   asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%9\n\t"
-      "ds_read_b64_tr_b16 %4, %8 offset:%10\n\t"
-      "ds_read_b64_tr_b16 %1, %8 offset:%9+64\n\t"
-      "ds_read_b64_tr_b16 %5, %8 offset:%10+64\n\t"
-      "ds_read_b64_tr_b16 %2, %8 offset:%9+128\n\t"
-      "ds_read_b64_tr_b16 %6, %8 offset:%10+128\n\t"
-      "ds_read_b64_tr_b16 %3, %8 offset:%9+192\n\t"
-      "ds_read_b64_tr_b16 %7, %8 offset:%10+192\n\t"
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(x0), "=&v"(x1), "=&v"(x2), "=&v"(x3), "=&v"(y0), "=&v"(y1), "=&v"(y2), "=&v"(y3)
-      : "v"(a), "n"(OFF), "n"(kHi + OFF)
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF), "n"(OFF + 2 * 4 * kRow)
       : "memory");
   const uint64_t x[4] = {x0, x1, x2, x3}, y[4] = {y0, y1, y2, y3};
 #pragma unroll
   for (int t = 0; t < 4; ++t)
     v[t] = u32x4{(uint32_t)x[t], (uint32_t)(x[t] >> 32), (uint32_t)y[t], (uint32_t)(y[t] >> 32)};
+}
+
+// K fragments: the four 16-byte chunks at a[0..3], OFF bytes on. As the V reads in
+// assembly with their own wait: the compiler takes a read of LDS as dependent on
+// every DMA in flight and would wait for the next stages' too.
+template <int OFF>
+__device__ __forceinline__ void read_k(const uint32_t (&a)[4], u32x4 (&k)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %4 offset:%8\n\t"
+      "ds_read_b128 %1, %5 offset:%8\n\t"
+      "ds_read_b128 %2, %6 offset:%8\n\t"
+      "ds_read_b128 %3, %7 offset:%8\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF)
+      : "memory");
+}
+// Barrier for what the waves have waited for themselves (their DMA, counted) and LDS.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // Block = (range, KV head, tile of 128 queries), eight waves: wave w has the 32
@@ -105,6 +128,7 @@ __device__ __forceinline__ void read_v(uint32_t a, u32x4 (&v)[4]) {
 // all others leaves its value as it is.
 __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   __shared__ __attribute__((aligned(16))) uint16_t kv[kStages][kStage];
+  __shared__ float half_ref[4][64], half_sum[4][64];
   __shared__ uint64_t path[kTree];
   __shared__ uint32_t odd_rows[2];  // nodes whose V holds an infinity or a NaN
   static_assert(sizeof(kv) >= 4 * kHalf * sizeof(float), "the halves fit the staging memory");
@@ -123,40 +147,50 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   const int q0 = tile * kTileQ + 32 * (wave & 3);  // the wave's queries
   const bool busy = q0 < a.queries;
   const int mine = min(q0 + (lane & 31), a.queries - 1);  // the lane's query once the scores are swapped
-  if (t < kTree) path[t] = t < a.rows ? tree_path(a.paths[t], t) : 0;
-  if (t < 2) odd_rows[t] = 0;
   bf16x8 qf[2][8];
-  if (busy) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int q = min(q0 + 16 * u + qi, a.queries - 1), row = q / a.group;
-      const uint16_t* const from = a.query + ((size_t)row * a.q_heads + kvh * a.group + q - row * a.group) * 256 + 8 * g;
+  for (int u = 0; u < 2; ++u) {
+    const int q = min(q0 + 16 * u + qi, a.queries - 1), row = q / a.group;
+    const uint16_t* const from = a.query + ((size_t)row * a.q_heads + kvh * a.group + q - row * a.group) * 256 + 8 * g;
 #pragma unroll
-      for (int s = 0; s < 8; ++s) qf[u][s] = *reinterpret_cast<const bf16x8*>(from + 32 * s);
-    }
+    for (int s = 0; s < 8; ++s) qf[u][s] = *reinterpret_cast<const bf16x8*>(from + 32 * s);
   }
-  // DMA of 32 keys: wave w rows 4 w .. 4 w + 3 of K and V, a row of 512 bytes an
-  // instruction. Rows past the last one repeat it: their products are masked.
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int s = 0; s < 8; ++s) asm volatile("" : "+v"(qf[u][s]));
+  // DMA of 32 keys: wave w rows 4 w .. 4 w + 3 of K and of V, two rows (1 KB) an
+  // instruction, lane l slot l % 32 of row l / 32 of the two. Rows past the last one
+  // repeat it: their products are masked.
   const uint16_t* const kbase = tree ? a.k_tree + kvh * 256 : a.kcache + (size_t)kvh * a.capacity * 256;
   const uint16_t* const vbase = tree ? a.v_proj + kvh * 256 : a.vcache + (size_t)kvh * a.capacity * 256;
   const uint32_t stride = tree ? (uint32_t)a.kv_heads * 512u : 512u;
   const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc((void*)kbase, 0, -1, 0x00020000);
   const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc((void*)vbase, 0, -1, 0x00020000);
-  const uint32_t lane_off = (uint32_t)lane * 16u;
-  auto issue = [&](int kb) {
-    uint16_t* const stage = kv[(kb - kb0) % kStages];
-    if (lane < 32) {
+  uint32_t kchunk[2], vchunk[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 4 * wave + i;
-        const uint32_t at = (uint32_t)min(kb * kKeys + r, n - 1) * stride;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (__attribute__((address_space(3))) void*)(stage + r * kKRow), 16,
-                                                 lane_off, at, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            vrs, (__attribute__((address_space(3))) void*)(stage + kKeys * kKRow + r * kVRow), 16, lane_off, at, 0, 0);
+  for (int i = 0; i < 2; ++i) {
+    const int r = 4 * wave + 2 * i + (lane >> 5);
+    kchunk[i] = (uint32_t)(((lane & 31) ^ (r & 15)) * 16);
+    vchunk[i] = (uint32_t)(((lane & 31) ^ 4 * (r & 3)) * 16);
+  }
+  auto issue = [&](int kb, int st) {
+    uint16_t* const stage = kv[st];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 4 * wave + 2 * i;
+      uint32_t at = (uint32_t)(kb * kKeys + r) * stride, more = (uint32_t)(lane >> 5) * stride;
+      if (kb * kKeys + kKeys > n) {
+        at = 0;
+        more = (uint32_t)min(kb * kKeys + r + (lane >> 5), n - 1) * stride;
       }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (__attribute__((address_space(3))) void*)(stage + r * kRow), 16,
+                                               kchunk[i] + more, at, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (__attribute__((address_space(3))) void*)(stage + (kKeys + r) * kRow), 16,
+                                               vchunk[i] + more, at, 0, 0);
     }
   };
+  for (int kb = kb0; kb < min(kb0 + kStages - 1, kb1); ++kb) issue(kb, kb - kb0);
   f32x16 ot[8];  // O^T: dims 32 i + 8 (r / 4) + 4 (l / 32) + r % 4 of query l % 32
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -166,25 +200,35 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   float ref = -3.0e38f, sum = 0.0f;
   const float c = 0.0625f * 1.4426950408889634f;  // log2(e) / 16
   const uint32_t kv_base = (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) uint16_t*)(&kv[0][0]));
-  const uint32_t v_lane =
-      (uint32_t)(2 * (kKeys * kKRow + (16 * kh + 8 * (g >> 1) + (qi >> 2)) * kVRow + 16 * (g & 1) + 4 * (qi & 3)));
-  for (int kb = kb0; kb < min(kb0 + kStages - 1, kb1); ++kb) issue(kb);
-  __syncthreads();
-  const uint64_t seen = tree ? path[mine / a.group] : 0;
+  uint32_t k_at[4], v_at[4];  // LDS bytes: dims 32 s + 8 g of key qi, s % 4 = i; dims 32 t + 16 (g & 1), t % 4 = i
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    k_at[i] = kv_base + (uint32_t)(2 * ((16 * kh + qi) * kRow + ((4 * i + g) ^ qi) * 8));
+    const int r = 16 * kh + 8 * (g >> 1) + (qi >> 2);
+    v_at[i] = kv_base + (uint32_t)(2 * ((kKeys + r) * kRow + 32 * (i ^ (r & 3)) + 16 * (g & 1) + 4 * (qi & 3)));
+  }
+  uint64_t seen = 0;
+  if (tree) {
+    if (t < kTree) path[t] = t < a.rows ? tree_path(a.paths[t], t) : 0;
+    if (t < 2) odd_rows[t] = 0;
+    __syncthreads();
+    seen = path[mine / a.group];
+  }
+  int st = kStages - 1;
   for (int kb = kb0; kb < kb1; ++kb) {
+    st = (st + 1) % kStages;
     const int ahead = min(kStages - 2, kb1 - 1 - kb);
     if (ahead >= 2)
-      wait_vmcnt<16>();
-    else if (ahead == 1)
       wait_vmcnt<8>();
+    else if (ahead == 1)
+      wait_vmcnt<4>();
     else
       wait_vmcnt<0>();
-    __syncthreads();  // block kb is there, and every wave is past block kb - 1
-    uint16_t* const stage = kv[(kb - kb0) % kStages];
-    if (kb + kStages - 1 < kb1) issue(kb + kStages - 1);
+    stage_barrier();  // block kb is there, and every wave is past block kb - 1
+    if (kb + kStages - 1 < kb1) issue(kb + kStages - 1, (st + kStages - 1) % kStages);
     if (tree) {
       // A masked key's value counts 0 times: infinities and NaN leave the products and join at the end.
-      uint32_t* const v = reinterpret_cast<uint32_t*>(stage + kKeys * kKRow + (t >> 4) * kVRow + (t & 15) * 16);
+      uint32_t* const v = reinterpret_cast<uint32_t*>(kv[st] + (kKeys + (t >> 4)) * kRow + (t & 15) * 16);
       bool odd = false;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -200,20 +244,31 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
       __syncthreads();
     }
     if (!busy) continue;
-    const uint16_t* const ks = stage + 16 * kh * kKRow;
-    const uint32_t vs = kv_base + (uint32_t)(2 * kStage * ((kb - kb0) % kStages)) + v_lane;
-    f32x4 st[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    uint32_t ka[4], va[4];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const bf16x8 kf = *reinterpret_cast<const bf16x8*>(ks + qi * kKRow + 32 * s + 8 * g);
+    for (int i = 0; i < 4; ++i) {
+      ka[i] = k_at[i] + (uint32_t)(2 * kStage) * st;
+      va[i] = v_at[i] + (uint32_t)(2 * kStage) * st;
+    }
+    f32x4 sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-      for (int u = 0; u < 2; ++u) st[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[u][s], st[u], 0, 0, 0);
+    for (int s4 = 0; s4 < 2; ++s4) {
+      u32x4 kf[4];
+      if (s4 == 0)
+        read_k<0>(ka, kf);
+      else
+        read_k<256>(ka, kf);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf[i]), qf[u][4 * s4 + i], sc[u], 0, 0, 0);
     }
     // keys 4 g + r of query l % 16 of both groups -> keys 8 (l / 32) + e of query l % 32
     float x[8];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(st[0][r]), __float_as_uint(st[1][r]), false, false);
+      const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(sc[0][r]), __float_as_uint(sc[1][r]), false, false);
       x[r] = __uint_as_float(p[0]);
       x[4 + r] = __uint_as_float(p[1]);
     }
@@ -253,15 +308,15 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
     for (int d4 = 0; d4 < 2; ++d4) {
       u32x4 vf[4];
       if (d4 == 0)
-        read_v<0>(vs, vf);
+        read_v<0>(va, vf);
       else
-        read_v<256>(vs, vf);
+        read_v<256>(va, vf);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         ot[4 * d4 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[i]), pf, ot[4 * d4 + i], 0, 0, 0);
     }
   }
-  __syncthreads();  // the staging memory is free
+  stage_barrier();  // the staging memory is free
   float* const half = reinterpret_cast<float*>(&kv[0][0]) + (wave & 3) * kHalf;
   if (kh && busy) {
 #pragma unroll
@@ -270,12 +325,12 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
       for (int r = 0; r < 4; ++r)
         *reinterpret_cast<float4*>(half + ((4 * i + r) * 64 + lane) * 4) =
             make_float4(ot[i][4 * r], ot[i][4 * r + 1], ot[i][4 * r + 2], ot[i][4 * r + 3]);
-    half[64 * 128 + lane] = ref;
-    half[64 * 129 + lane] = sum;
+    half_ref[wave & 3][lane] = ref;
+    half_sum[wave & 3][lane] = sum;
   }
   __syncthreads();
   if (kh || !busy) return;
-  const float ref1 = half[64 * 128 + lane], sum1 = half[64 * 129 + lane], top = fmaxf(ref, ref1);
+  const float ref1 = half_ref[wave][lane], sum1 = half_sum[wave][lane], top = fmaxf(ref, ref1);
   const float f0 = __builtin_amdgcn_exp2f(ref - top), f1 = __builtin_amdgcn_exp2f(ref1 - top);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -289,6 +344,7 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
     }
   if (tree) {
     const uint64_t odd = (uint64_t)odd_rows[1] << 32 | odd_rows[0];
+#pragma unroll 1
     for (uint64_t left = odd; left; left &= left - 1) {
       const int j = __builtin_ctzll(left);
       const uint16_t* const v = vbase + (size_t)j * a.kv_heads * 256 + 4 * (lane >> 5);
@@ -296,9 +352,11 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const uint32_t w = v[32 * i + 8 * (r >> 2) + (r & 3)];
-          if (on && (w & 0x7f80u) == 0x7f80u) ot[i][r] += bf2f(w);
+        for (int r = 0; r < 4; ++r) {
+          const uint2 w = *reinterpret_cast<const uint2*>(v + 32 * i + 8 * r);
+          const float y[4] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ot[i][4 * r + e] += on && !(fabsf(y[e]) < INFINITY) ? y[e] : 0.0f;
         }
     }
   }
