@@ -141,8 +141,12 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   const bool tree = range == a.ranges;
   const int n = tree ? a.rows : a.position;  // keys
   const int blocks = (n + kKeys - 1) / kKeys;
-  const int kb0 = tree ? 0 : (int)((int64_t)blocks * range / a.ranges);
-  const int kb1 = tree ? blocks : (int)((int64_t)blocks * (range + 1) / a.ranges);
+  // A range is every `ranges`-th block of 32 keys, so that at any time all blocks read
+  // one window of the cache: contiguous ranges read 256 streams at equal distances, at
+  // 3.9 TB/s against 4.4, and 5.0 with loads that pass the caches by (1 node at 131008,
+  // whole calls of 69, 60 and 54 us).
+  const int first = tree ? 0 : range, every = tree ? 1 : a.ranges;
+  const int steps = (blocks - first + every - 1) / every;
   const int qi = lane & 15, g = lane >> 4, kh = wave >> 2;
   const int q0 = tile * kTileQ + 32 * (wave & 3);  // the wave's queries
   const bool busy = q0 < a.queries;
@@ -185,12 +189,12 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
         more = (uint32_t)min(kb * kKeys + r + (lane >> 5), n - 1) * stride;
       }
       __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (__attribute__((address_space(3))) void*)(stage + r * kRow), 16,
-                                               kchunk[i] + more, at, 0, 0);
+                                               kchunk[i] + more, at, 0, kLoadNonTemporal);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (__attribute__((address_space(3))) void*)(stage + (kKeys + r) * kRow), 16,
-                                               vchunk[i] + more, at, 0, 0);
+                                               vchunk[i] + more, at, 0, kLoadNonTemporal);
     }
   };
-  for (int kb = kb0; kb < min(kb0 + kStages - 1, kb1); ++kb) issue(kb, kb - kb0);
+  for (int i = 0; i < min(kStages - 1, steps); ++i) issue(first + i * every, i);
   f32x16 ot[8];  // O^T: dims 32 i + 8 (r / 4) + 4 (l / 32) + r % 4 of query l % 32
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -215,9 +219,9 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
     seen = path[mine / a.group];
   }
   int st = kStages - 1;
-  for (int kb = kb0; kb < kb1; ++kb) {
+  for (int i = 0, kb = first; i < steps; ++i, kb += every) {
     st = (st + 1) % kStages;
-    const int ahead = min(kStages - 2, kb1 - 1 - kb);
+    const int ahead = min(kStages - 2, steps - 1 - i);
     if (ahead >= 2)
       wait_vmcnt<8>();
     else if (ahead == 1)
@@ -225,7 +229,7 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
     else
       wait_vmcnt<0>();
     stage_barrier();  // block kb is there, and every wave is past block kb - 1
-    if (kb + kStages - 1 < kb1) issue(kb + kStages - 1, (st + kStages - 1) % kStages);
+    if (i + kStages - 1 < steps) issue(kb + (kStages - 1) * every, (st + kStages - 1) % kStages);
     if (tree) {
       // A masked key's value counts 0 times: infinities and NaN leave the products and join at the end.
       uint32_t* const v = reinterpret_cast<uint32_t*>(kv[st] + (kKeys + (t >> 4)) * kRow + (t & 15) * 16);
