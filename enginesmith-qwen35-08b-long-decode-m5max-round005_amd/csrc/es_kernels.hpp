@@ -391,7 +391,7 @@ hipError_t launch_logprob(LogprobArgs a, hipStream_t s);
 // ---- a tree of drafted tokens, k_tree.hip and k_gdn_tree.hip ----
 // Callers check shapes, alignment and bounds; the launchers do not.
 constexpr int kTree = 64;             // most nodes
-constexpr int kTreePartFloats = 260;  // a range's 256 sums, reference and sum of exponentials, to a multiple of 16 bytes
+constexpr int kTreePartFloats = 32 * 258;  // 256 sums, reference and sum of exponentials of 32 queries in a range
 // The nodes on node i's path, itself the last; none for a node left out.
 __host__ __device__ inline uint64_t tree_path(uint64_t word, int i) {
   return word >> i & 1 ? word & ((2ull << i) - 1) : 0;
@@ -405,9 +405,9 @@ struct TreeAttn {
   int capacity, position;
   void* scratch;
   uint16_t *k_tree, *gated;
-  uint16_t* query;  // in the scratch, as part (by the launcher, as the rest)
-  float* part;
-  int group, queries, tiles, ranges;
+  float* part;  // the scratch (by the launcher, as the rest)
+  int group, queries, tiles, parts, ranges;
+  uint32_t group_inv;
 };
 size_t tree_attn_scratch_bytes(int q_heads, int kv_heads, int rows);
 hipError_t launch_tree_attn(TreeAttn a, hipStream_t s);

@@ -10,7 +10,6 @@
 // bits, and leaves them to the kernel that joins the ranges. The nodes' own keys
 // are one more range, the only one with a mask.
 #include <algorithm>
-#include <type_traits>
 
 #include "es_kernels.hpp"
 
@@ -18,6 +17,7 @@ namespace es {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTileQ = 128;   // queries of a block: four tiles of 32, each on two waves
@@ -25,100 +25,46 @@ constexpr int kKeys = 32;     // keys of a stage
 constexpr int kStages = 4;
 constexpr int kRow = 256;     // bf16 elements between rows in LDS
 constexpr int kStage = 2 * kKeys * kRow;  // K rows, then V rows
-constexpr int kHalf = 64 * 128;  // output sums that a wave leaves for the other of its tile
+constexpr int kPart = kTreePartFloats;    // floats of a tile of 32 queries in a range
 
+__device__ __forceinline__ uint32_t lds_bytes(const void* p) {
+  return (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) void*)p);
+}
+// 16 (or 4) bytes a lane from memory to LDS, lane after lane from `to` on. In
+// assembly, and waited for by count: the compiler takes every read of LDS as dependent on
+// every such load in flight and would wait for the next stages' too.
+struct Source {
+  u32x4 words;
+  __device__ explicit Source(const void* p)
+      : words{(uint32_t)(uintptr_t)p, (uint32_t)((uintptr_t)p >> 32), 0xffffffffu, 0x00020000u} {}
+};
+__device__ __forceinline__ void dma16(const Source& s, uint32_t to, uint32_t lane_off, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(lane_off),
+               "s"(s.words), "s"(off)
+               : "memory");
+}
+__device__ __forceinline__ void dma16_past_caches(const Source& s, uint32_t to, uint32_t lane_off, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds" ::"s"(to), "v"(lane_off),
+               "s"(s.words), "s"(off)
+               : "memory");
+}
+__device__ __forceinline__ void dma4(const Source& s, uint32_t to, uint32_t lane_off, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(to), "v"(lane_off),
+               "s"(s.words), "s"(off)
+               : "memory");
+}
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
-
-// ---- queries and keys of the nodes ----
-// One wave a (node, head): the q heads, then the k heads. RMS norm with the
-// squares in 64 bits (they pass 32 bits' range before the head does), rotation with
-// angles in 64 bits, one rounding. A node left out gets zeros.
-__global__ __launch_bounds__(256) void k_tree_prepare(TreeAttn a) {
-  const int lane = threadIdx.x & 63, heads = a.q_heads + a.kv_heads;
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= a.rows * heads) return;
-  const int row = i / heads, head = i - row * heads;
-  const bool of_q = head < a.q_heads;
-  const size_t at = of_q ? (size_t)row * a.q_heads + head : (size_t)row * a.kv_heads + head - a.q_heads;
-  const uint16_t* const from = of_q ? a.q_proj + at * 512 : a.k_proj + at * 256;
-  const uint2 xv = *reinterpret_cast<const uint2*>(from + 4 * lane);
-  const uint2 gv = *reinterpret_cast<const uint2*>((of_q ? a.q_gain : a.k_gain) + 4 * lane);
-  const uint64_t path = tree_path(a.paths[row], row);
-  float sn, cs;
-  es_sincos_angle((double)(a.position + __popcll(path) - 1) * (double)a.inv_freq[lane & 31], &sn, &cs);
-  const float x[4] = {bf_lo(xv.x), bf_hi(xv.x), bf_lo(xv.y), bf_hi(xv.y)};
-  const float gain[4] = {bf_lo(gv.x), bf_hi(gv.x), bf_lo(gv.y), bf_hi(gv.y)};
-  double ss = 0.0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) ss = fma((double)x[e], (double)x[e], ss);
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) ss += __shfl_xor(ss, k);
-  const double inv = 1.0 / sqrt(ss * (1.0 / 256.0) + 1e-6);
-  float r[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float y = (float)((double)x[e] * inv * (double)gain[e]);
-    const int f = ((lane * 4) & 31) + e;
-    const float s1 = __shfl(sn, f), c1 = __shfl(cs, f), p1 = dpp_row_ror8(y);  // dim d ^ 32 is in lane ^ 8
-    r[e] = lane < 8 ? fmaf(y, c1, -(p1 * s1)) : lane < 16 ? fmaf(p1, s1, y * c1) : y;
-  }
-  const uint2 packed = path ? make_uint2(pack_bf2(r[0], r[1]), pack_bf2(r[2], r[3])) : make_uint2(0, 0);
-  *reinterpret_cast<uint2*>((of_q ? a.query : a.k_tree) + at * 256 + 4 * lane) = packed;
-}
-
-// ---- attention ----
-// Chunk c (16 bytes) of a row lies at slot c ^ (row & 15) of K and c ^ 4 (row & 3) of
-// V, so that the 16 rows of a fragment's read, and the four rows x 64 bytes of a
-// transposing read, cover all banks once.
-//
-// V^T fragments by transposing reads: keys 0..3 and 4..7 of the lane's eight for the
-// four 32-dim tiles whose addresses are a[0..3], OFF bytes on. All complete before
-// the statement ends.
-template <int OFF>
-__device__ __forceinline__ void read_v(const uint32_t (&a)[4], u32x4 (&v)[4]) {
-  uint64_t x0, x1, x2, x3, y0, y1, y2, y3;
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %2, %10 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(x0), "=&v"(x1), "=&v"(x2), "=&v"(x3), "=&v"(y0), "=&v"(y1), "=&v"(y2), "=&v"(y3)
-      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF), "n"(OFF + 2 * 4 * kRow)
-      : "memory");
-  const uint64_t x[4] = {x0, x1, x2, x3}, y[4] = {y0, y1, y2, y3};
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-    v[t] = u32x4{(uint32_t)x[t], (uint32_t)(x[t] >> 32), (uint32_t)y[t], (uint32_t)(y[t] >> 32)};
-}
-
-// K fragments: the four 16-byte chunks at a[0..3], OFF bytes on. As the V reads in
-// assembly with their own wait: the compiler takes a read of LDS as dependent on
-// every DMA in flight and would wait for the next stages' too.
-template <int OFF>
-__device__ __forceinline__ void read_k(const uint32_t (&a)[4], u32x4 (&k)[4]) {
-  asm volatile(
-      "ds_read_b128 %0, %4 offset:%8\n\t"
-      "ds_read_b128 %1, %5 offset:%8\n\t"
-      "ds_read_b128 %2, %6 offset:%8\n\t"
-      "ds_read_b128 %3, %7 offset:%8\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3])
-      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF)
-      : "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 // Barrier for what the waves have waited for themselves (their DMA, counted) and LDS.
-__device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// ---- attention ----
+// Chunk c (16 bytes) of a row lies at slot c ^ (row & 15) of K and of the queries, and
+// c ^ 4 (row & 3) of V, so that the 16 rows of a fragment's read, and the four rows x 64
+// bytes of a transposing read, cover all banks once.
+//
 // Block = (range, KV head, tile of 128 queries), eight waves: wave w has the 32
 // queries of tile w & 3 and the keys 16 (w >> 2) .. + 15 of every 32, with a
 // softmax state of its own; the two halves meet at the end. Scores S^T = K Q^T on
@@ -126,12 +72,17 @@ __device__ __forceinline__ void stage_barrier() {
 // whose exponentials, rounded to bf16, are the operand of O^T += V^T P^T on
 // 32x32x16 products. The sum is taken over the rounded ones, so a key that outweighs
 // all others leaves its value as it is.
+//
+// The block makes its queries itself (norm, rotation, one rounding to bf16) while its
+// first keys are on their way; a block of the nodes' own keys makes those too.
 __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   __shared__ __attribute__((aligned(16))) uint16_t kv[kStages][kStage];
-  __shared__ float half_ref[4][64], half_sum[4][64];
-  __shared__ uint64_t path[kTree];
+  __shared__ __attribute__((aligned(16))) float2 turn[kTree][32];  // cosine and sine by number of ancestors
+  __shared__ __attribute__((aligned(16))) uint16_t gain[2][256];
+  __shared__ __attribute__((aligned(16))) float freq[32];
+  __shared__ __attribute__((aligned(16))) uint64_t word[kTree];
+  __shared__ float left_ref[8][64], left_sum[8][64];
   __shared__ uint32_t odd_rows[2];  // nodes whose V holds an infinity or a NaN
-  static_assert(sizeof(kv) >= 4 * kHalf * sizeof(float), "the halves fit the staging memory");
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   // the tiles that read the same keys on one XCD (block b on XCD b % 8)
@@ -150,27 +101,14 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   const int qi = lane & 15, g = lane >> 4, kh = wave >> 2;
   const int q0 = tile * kTileQ + 32 * (wave & 3);  // the wave's queries
   const bool busy = q0 < a.queries;
-  const int mine = min(q0 + (lane & 31), a.queries - 1);  // the lane's query once the scores are swapped
-  bf16x8 qf[2][8];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int q = min(q0 + 16 * u + qi, a.queries - 1), row = q / a.group;
-    const uint16_t* const from = a.query + ((size_t)row * a.q_heads + kvh * a.group + q - row * a.group) * 256 + 8 * g;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) qf[u][s] = *reinterpret_cast<const bf16x8*>(from + 32 * s);
-  }
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int s = 0; s < 8; ++s) asm volatile("" : "+v"(qf[u][s]));
+  auto node_of = [&](int q) { return a.group == 1 ? q : (int)__umulhi((uint32_t)q, a.group_inv); };
   // DMA of 32 keys: wave w rows 4 w .. 4 w + 3 of K and of V, two rows (1 KB) an
   // instruction, lane l slot l % 32 of row l / 32 of the two. Rows past the last one
   // repeat it: their products are masked.
-  const uint16_t* const kbase = tree ? a.k_tree + kvh * 256 : a.kcache + (size_t)kvh * a.capacity * 256;
-  const uint16_t* const vbase = tree ? a.v_proj + kvh * 256 : a.vcache + (size_t)kvh * a.capacity * 256;
+  const Source ksrc(tree ? a.k_proj + kvh * 256 : a.kcache + (size_t)kvh * a.capacity * 256);
+  const Source vsrc(tree ? a.v_proj + kvh * 256 : a.vcache + (size_t)kvh * a.capacity * 256);
   const uint32_t stride = tree ? (uint32_t)a.kv_heads * 512u : 512u;
-  const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc((void*)kbase, 0, -1, 0x00020000);
-  const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc((void*)vbase, 0, -1, 0x00020000);
+  const uint32_t kv_base = lds_bytes(&kv[0][0]);
   uint32_t kchunk[2], vchunk[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -179,7 +117,7 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
     vchunk[i] = (uint32_t)(((lane & 31) ^ 4 * (r & 3)) * 16);
   }
   auto issue = [&](int kb, int st) {
-    uint16_t* const stage = kv[st];
+    const uint32_t stage = kv_base + (uint32_t)(2 * kStage) * st;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = 4 * wave + 2 * i;
@@ -188,14 +126,142 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
         at = 0;
         more = (uint32_t)min(kb * kKeys + r + (lane >> 5), n - 1) * stride;
       }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (__attribute__((address_space(3))) void*)(stage + r * kRow), 16,
-                                               kchunk[i] + more, at, 0, kLoadNonTemporal);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (__attribute__((address_space(3))) void*)(stage + (kKeys + r) * kRow), 16,
-                                               vchunk[i] + more, at, 0, kLoadNonTemporal);
+      dma16_past_caches(ksrc, stage + 2 * r * kRow, kchunk[i] + more, at);
+      dma16_past_caches(vsrc, stage + 2 * (kKeys + r) * kRow, vchunk[i] + more, at);
     }
   };
-  for (int i = 0; i < min(kStages - 1, steps); ++i) issue(first + i * every, i);
-  f32x16 ot[8];  // O^T: dims 32 i + 8 (r / 4) + 4 (l / 32) + r % 4 of query l % 32
+  // Small inputs; the queries, 16 a wave, into the stages after the first two; the first two stages.
+  const int l0 = 16 * wave;  // the queries of the tile that the wave makes
+  const bool makes = tile * kTileQ + l0 < a.queries;
+  if (wave < 2) {
+    if (lane < 32) dma16(Source(wave ? a.k_gain : a.q_gain), lds_bytes(gain[wave]), lane * 16, 0);
+  } else if (wave == 2) {
+    if (lane < 8) dma16(Source(a.inv_freq), lds_bytes(freq), lane * 16, 0);
+  } else if (wave == 3) {
+    if (lane < 2 * a.rows) dma4(Source(a.paths), lds_bytes(word), lane * 4, 0);
+    if (lane + 64 < 2 * a.rows) dma4(Source(a.paths), lds_bytes(word + 32), lane * 4, 256);
+  }
+  if (makes) {
+    const Source qsrc(a.q_proj + (size_t)kvh * a.group * 512);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int l = l0 + 2 * i + (lane >> 5), q = min(tile * kTileQ + l, a.queries - 1), row = node_of(q);
+      dma16(qsrc, kv_base + (uint32_t)(2 * (2 * kStage + (l0 + 2 * i) * kRow)),
+            (uint32_t)(row * a.q_heads + q - row * a.group) * 1024u + (uint32_t)(((lane & 31) ^ (l & 15)) * 16), 0);
+    }
+  }
+  issue(first, 0);
+  if (steps > 1) {
+    issue(first + every, 1);
+    wait_vmcnt<8>();
+  } else {
+    wait_vmcnt<4>();
+  }
+  stage_barrier();
+  for (int d = t >> 5; d < a.rows; d += 16) {
+    float sn, cs;
+    es_sincos_angle((double)(a.position + d) * (double)freq[t & 31], &sn, &cs);
+    turn[d][t & 31] = make_float2(cs, sn);
+  }
+  if (t < 2) odd_rows[t] = 0;
+  if (tree) wait_vmcnt<0>();
+  stage_barrier();
+  // A head is made by four lanes, with dims 32 s + 8 g .. + 7: the queries, then the
+  // nodes' keys where this is their block (four waves, 16 each).
+#pragma unroll 1
+  for (int pass = 0; pass < (tree ? 2 : 1); ++pass) {
+    if (pass ? wave >= 4 || 16 * wave >= a.rows : !makes) continue;
+    const int r = l0 + qi;  // of the tile's queries or of the nodes
+    char* const head = reinterpret_cast<char*>(pass ? &kv[wave >> 1][(r & 31) * kRow] : &kv[2][r * kRow]);
+    const int node = pass ? r : node_of(min(tile * kTileQ + r, a.queries - 1));
+    const uint64_t path = node < a.rows ? tree_path(word[node], node) : 0;
+    u32x4 x[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[s] = *reinterpret_cast<const u32x4*>(head + ((4 * s + g) ^ qi) * 16);
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[e] = fmaf(bf_hi(x[s][e]), bf_hi(x[s][e]), fmaf(bf_lo(x[s][e]), bf_lo(x[s][e]), part[e]));
+    float2 p = rows_xor16((part[0] + part[1]) + (part[2] + part[3]));
+    p = rows_xor32(p.x + p.y);
+    float ss = p.x + p.y, inv = 1.0f / sqrtf(ss * (1.0f / 256.0f) + 1e-6f);
+    if (__any(!(ss < INFINITY))) {
+      // The squares pass 32 bits' range before the head does: such a head by 2^-72, beside
+      // which the eps is nothing. An infinity or a NaN stays one.
+      float big = 0.0f;
+#pragma unroll 1
+      for (int e = 0; e < 64; ++e) {
+        const uint32_t w = *reinterpret_cast<const uint16_t*>(head + ((4 * (e >> 3) + g) ^ qi) * 16 + 2 * (e & 7));
+        big = fmaf(bf2f(w) * 0x1p-72f, bf2f(w) * 0x1p-72f, big);
+      }
+      p = rows_xor16(big);
+      p = rows_xor32(p.x + p.y);
+      if (!(ss < INFINITY)) {
+        inv = 1.0f / sqrtf((p.x + p.y) * (1.0f / 256.0f));
+        const float by = 0x1p-72f;  // exact on bf16 of this size; smaller dims are nothing beside it
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[s][e] = pack_bf2(bf_lo(x[s][e]) * by, bf_hi(x[s][e]) * by);
+      }
+    }
+    const uint16_t* const by = gain[pass] + 8 * g;
+    float lo[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const u32x4 gv = *reinterpret_cast<const u32x4*>(by + 32 * s);
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[2 * e] = bf_lo(x[s][e]) * inv * bf_lo(gv[e]);
+        y[2 * e + 1] = bf_hi(x[s][e]) * inv * bf_hi(gv[e]);
+      }
+      if (s == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo[e] = y[e];
+        continue;
+      }
+      if (s == 1) {  // dims d and d + 32 of the rotated 64
+        const float4* const cs = reinterpret_cast<const float4*>(&turn[path ? __popcll(path) - 1 : 0][8 * g]);
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 c2 = cs[e];
+          w[e] = pack_bf2(fmaf(lo[2 * e], c2.x, -(y[2 * e] * c2.y)), fmaf(lo[2 * e + 1], c2.z, -(y[2 * e + 1] * c2.w)));
+          y[2 * e] = fmaf(lo[2 * e], c2.y, y[2 * e] * c2.x);
+          y[2 * e + 1] = fmaf(lo[2 * e + 1], c2.w, y[2 * e + 1] * c2.z);
+        }
+        x[0] = w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[s][e] = pack_bf2(y[2 * e], y[2 * e + 1]);
+    }
+    const bool out = pass && !path;  // a node left out has no key
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if (out) x[s] = u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(head + ((4 * s + g) ^ qi) * 16) = x[s];
+    }
+    if (pass && tile == 0 && r < a.rows) {
+      uint16_t* const to = a.k_tree + ((size_t)r * a.kv_heads + kvh) * 256 + 8 * g;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) *reinterpret_cast<u32x4*>(to + 32 * s) = x[s];
+    }
+  }
+  stage_barrier();
+  bf16x8 qf[2][8];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      qf[u][s] = *reinterpret_cast<const bf16x8*>(&kv[2][(32 * (wave & 3) + 16 * u + qi) * kRow + ((4 * s + g) ^ qi) * 8]);
+  uint64_t seen = 0;
+  if (tree) {
+    const int node = node_of(min(q0 + (lane & 31), a.queries - 1));
+    seen = tree_path(word[node], node);
+  }
+  f32x16 ot[8];  // O^T: dims 32 (i ^ 4 kh) + 8 (r / 4) + 4 (l / 32) + r % 4 of query l % 32
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -203,36 +269,30 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   // The reference starts below every score but finite: a half may have no key.
   float ref = -3.0e38f, sum = 0.0f;
   const float c = 0.0625f * 1.4426950408889634f;  // log2(e) / 16
-  const uint32_t kv_base = (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) uint16_t*)(&kv[0][0]));
-  uint32_t k_at[4], v_at[4];  // LDS bytes: dims 32 s + 8 g of key qi, s % 4 = i; dims 32 t + 16 (g & 1), t % 4 = i
+  uint32_t k_at[4], v_at[4];  // bytes in a stage: dims 32 s + 8 g of key qi, s % 4 = i; dims 32 t + 16 (g & 1), t % 4 = i
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    k_at[i] = kv_base + (uint32_t)(2 * ((16 * kh + qi) * kRow + ((4 * i + g) ^ qi) * 8));
+    k_at[i] = (uint32_t)(2 * ((16 * kh + qi) * kRow + ((4 * i + g) ^ qi) * 8));
     const int r = 16 * kh + 8 * (g >> 1) + (qi >> 2);
-    v_at[i] = kv_base + (uint32_t)(2 * ((kKeys + r) * kRow + 32 * (i ^ (r & 3)) + 16 * (g & 1) + 4 * (qi & 3)));
-  }
-  uint64_t seen = 0;
-  if (tree) {
-    if (t < kTree) path[t] = t < a.rows ? tree_path(a.paths[t], t) : 0;
-    if (t < 2) odd_rows[t] = 0;
-    __syncthreads();
-    seen = path[mine / a.group];
+    v_at[i] = (uint32_t)(2 * ((kKeys + r) * kRow + 32 * (i ^ (r & 3)) + 16 * (g & 1) + 4 * (qi & 3))) ^ (uint32_t)(256 * kh);
   }
   int st = kStages - 1;
   for (int i = 0, kb = first; i < steps; ++i, kb += every) {
     st = (st + 1) % kStages;
-    const int ahead = min(kStages - 2, steps - 1 - i);
+    const int ahead = min(i ? kStages - 2 : 1, steps - 1 - i);
     if (ahead >= 2)
       wait_vmcnt<8>();
     else if (ahead == 1)
       wait_vmcnt<4>();
     else
       wait_vmcnt<0>();
-    stage_barrier();  // block kb is there, and every wave is past block kb - 1
+    stage_barrier();  // block kb is there, and every wave is past block kb - 1 (or has its queries)
+    if (i == 0 && steps > 2) issue(kb + 2 * every, 2);
     if (i + kStages - 1 < steps) issue(kb + (kStages - 1) * every, (st + kStages - 1) % kStages);
+    char* const stage = reinterpret_cast<char*>(kv[st]);
     if (tree) {
       // A masked key's value counts 0 times: infinities and NaN leave the products and join at the end.
-      uint32_t* const v = reinterpret_cast<uint32_t*>(kv[st] + (kKeys + (t >> 4)) * kRow + (t & 15) * 16);
+      uint32_t* const v = reinterpret_cast<uint32_t*>(stage + 2 * (kKeys + (t >> 4)) * kRow + (t & 15) * 32);
       bool odd = false;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -245,28 +305,15 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
       }
       const int key = kb * kKeys + (t >> 4);
       if (odd && key < n) atomicOr(&odd_rows[key >> 5], 1u << (key & 31));
-      __syncthreads();
+      stage_barrier();
     }
     if (!busy) continue;
-    uint32_t ka[4], va[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ka[i] = k_at[i] + (uint32_t)(2 * kStage) * st;
-      va[i] = v_at[i] + (uint32_t)(2 * kStage) * st;
-    }
     f32x4 sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-    for (int s4 = 0; s4 < 2; ++s4) {
-      u32x4 kf[4];
-      if (s4 == 0)
-        read_k<0>(ka, kf);
-      else
-        read_k<256>(ka, kf);
+    for (int s = 0; s < 8; ++s) {
+      const bf16x8 kf = *reinterpret_cast<const bf16x8*>(stage + k_at[s & 3] + 256 * (s >> 2));
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf[i]), qf[u][4 * s4 + i], sc[u], 0, 0, 0);
+      for (int u = 0; u < 2; ++u) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[u][s], sc[u], 0, 0, 0);
     }
     // keys 4 g + r of query l % 16 of both groups -> keys 8 (l / 32) + e of query l % 32
     float x[8];
@@ -302,45 +349,45 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
     sum = sum * factor + (s2.x + s2.y);
     if (__any(mnew > ref)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int d = 0; d < 8; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) ot[i][r] *= factor;
+        for (int r = 0; r < 16; ++r) ot[d][r] *= factor;
     }
     ref = mnew;
     const bf16x8 pf = __builtin_bit_cast(bf16x8, pb);
+    // V^T by transposing reads: keys 0 .. 3 and 4 .. 7 of the lane's eight
 #pragma unroll
-    for (int d4 = 0; d4 < 2; ++d4) {
-      u32x4 vf[4];
-      if (d4 == 0)
-        read_v<0>(va, vf);
-      else
-        read_v<256>(va, vf);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        ot[4 * d4 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[i]), pf, ot[4 * d4 + i], 0, 0, 0);
+    for (int d = 0; d < 8; ++d) {
+      typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
+      const lds_i16x4 at = (lds_i16x4)(stage + (v_at[d & 3] ^ (uint32_t)(64 * (d & 4))));
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + kRow);
+      const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, ot[d], 0, 0, 0);
     }
   }
-  stage_barrier();  // the staging memory is free
-  float* const half = reinterpret_cast<float*>(&kv[0][0]) + (wave & 3) * kHalf;
-  if (kh && busy) {
+  // The two waves of a tile each finish half of the dims, their first four sums; the
+  // other four and the softmax state go through LDS.
+  stage_barrier();
+  float* const room = reinterpret_cast<float*>(&kv[0][0]);
+  if (busy) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<float4*>(half + ((4 * i + r) * 64 + lane) * 4) =
-            make_float4(ot[i][4 * r], ot[i][4 * r + 1], ot[i][4 * r + 2], ot[i][4 * r + 3]);
-    half_ref[wave & 3][lane] = ref;
-    half_sum[wave & 3][lane] = sum;
+        *reinterpret_cast<float4*>(room + ((16 * wave + 4 * i + r) * 64 + lane) * 4) =
+            make_float4(ot[4 + i][4 * r], ot[4 + i][4 * r + 1], ot[4 + i][4 * r + 2], ot[4 + i][4 * r + 3]);
+    left_ref[wave][lane] = ref;
+    left_sum[wave][lane] = sum;
   }
-  __syncthreads();
-  if (kh || !busy) return;
-  const float ref1 = half_ref[wave][lane], sum1 = half_sum[wave][lane], top = fmaxf(ref, ref1);
+  stage_barrier();
+  if (!busy || q0 + (lane & 31) >= a.queries) return;
+  const float ref1 = left_ref[wave ^ 4][lane], sum1 = left_sum[wave ^ 4][lane], top = fmaxf(ref, ref1);
   const float f0 = __builtin_amdgcn_exp2f(ref - top), f1 = __builtin_amdgcn_exp2f(ref1 - top);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float4 o = *reinterpret_cast<const float4*>(half + ((4 * i + r) * 64 + lane) * 4);
+      const float4 o = *reinterpret_cast<const float4*>(room + ((16 * (wave ^ 4) + 4 * i + r) * 64 + lane) * 4);
       ot[i][4 * r] = fmaf(o.x, f1, ot[i][4 * r] * f0);
       ot[i][4 * r + 1] = fmaf(o.y, f1, ot[i][4 * r + 1] * f0);
       ot[i][4 * r + 2] = fmaf(o.z, f1, ot[i][4 * r + 2] * f0);
@@ -349,12 +396,12 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   if (tree) {
     const uint64_t odd = (uint64_t)odd_rows[1] << 32 | odd_rows[0];
 #pragma unroll 1
-    for (uint64_t left = odd; left; left &= left - 1) {
-      const int j = __builtin_ctzll(left);
-      const uint16_t* const v = vbase + (size_t)j * a.kv_heads * 256 + 4 * (lane >> 5);
+    for (uint64_t more = odd; more; more &= more - 1) {
+      const int j = __builtin_ctzll(more);
+      const uint16_t* const v = a.v_proj + ((size_t)j * a.kv_heads + kvh) * 256 + 128 * kh + 4 * (lane >> 5);
       const bool on = seen >> j & 1;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const uint2 w = *reinterpret_cast<const uint2*>(v + 32 * i + 8 * r);
@@ -364,56 +411,62 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
         }
     }
   }
-  const int q = q0 + (lane & 31);
-  if (q >= a.queries) return;
-  float* const part = a.part + ((size_t)unit * a.queries + q) * kTreePartFloats;
+  // A tile of a range as it lies in the lanes: dims 8 j + 4 (l / 32) .. + 3 of query l % 32 at (64 j + l) 4.
+  float* const part = a.part + ((size_t)unit * a.parts + (q0 >> 5)) * kPart;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      *reinterpret_cast<float4*>(part + 32 * i + 8 * r + 4 * (lane >> 5)) =
+      *reinterpret_cast<float4*>(part + ((16 * kh + 4 * i + r) * 64 + lane) * 4) =
           make_float4(ot[i][4 * r], ot[i][4 * r + 1], ot[i][4 * r + 2], ot[i][4 * r + 3]);
-  if (lane < 32) *reinterpret_cast<float2*>(part + 256) = make_float2(top, fmaf(sum1, f1, sum * f0));
+  if (kh == 0 && lane < 32) *reinterpret_cast<float2*>(part + 8192 + 2 * lane) = make_float2(top, fmaf(sum1, f1, sum * f0));
 }
 
-// Joins the ranges of a node's head: block = (node, head), wave w takes ranges w,
-// w + 4, ..., a lane four dims; then the output gate.
-__global__ __launch_bounds__(256) void k_tree_join(TreeAttn a) {
-  __shared__ float4 part_o[4][64];
-  __shared__ float2 part_s[4];
+// Joins the ranges: block = (8 dims, tile of 32 queries, KV head), wave w takes ranges
+// w, w + 16, ..., a lane four dims of a query; then the output gate.
+__global__ __launch_bounds__(1024) void k_tree_join(TreeAttn a) {
+  __shared__ float4 part_o[16][64];
+  __shared__ float2 part_s[16][32];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int row = blockIdx.x / a.q_heads, head = blockIdx.x % a.q_heads;
-  const int kvh = head / a.group, q = row * a.group + head % a.group;
+  const int j = blockIdx.x & 31, tile = (blockIdx.x >> 5) % a.parts, kvh = (blockIdx.x >> 5) / a.parts;
+  const int q = min(32 * tile + (lane & 31), a.queries - 1), row = a.group == 1 ? q : (int)__umulhi((uint32_t)q, a.group_inv);
+  const size_t at = (size_t)row * a.q_heads + kvh * a.group + q - row * a.group;
+  const int dim = 8 * j + 4 * (lane >> 5);
+  uint2 gate = make_uint2(0, 0);
+  uint64_t path = 0;
+  if (wave == 0) {
+    gate = *reinterpret_cast<const uint2*>(a.q_proj + at * 512 + 256 + dim);
+    path = tree_path(a.paths[row], row);
+  }
   float ref = -3.0e38f, sum = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto join = [&](float r1, float s1, float4 o1) {
-    const float top = fmaxf(ref, r1), f0 = __builtin_amdgcn_exp2f(ref - top), f1 = __builtin_amdgcn_exp2f(r1 - top);
+  auto join = [&](float2 s1, float4 o1) {
+    const float top = fmaxf(ref, s1.x), f0 = __builtin_amdgcn_exp2f(ref - top), f1 = __builtin_amdgcn_exp2f(s1.x - top);
     o.x = fmaf(o1.x, f1, o.x * f0);
     o.y = fmaf(o1.y, f1, o.y * f0);
     o.z = fmaf(o1.z, f1, o.z * f0);
     o.w = fmaf(o1.w, f1, o.w * f0);
-    sum = fmaf(s1, f1, sum * f0);
+    sum = fmaf(s1.y, f1, sum * f0);
     ref = top;
   };
-#pragma unroll 4
-  for (int i = wave; i <= a.ranges; i += 4) {
-    const float* const part = a.part + ((size_t)(i * a.kv_heads + kvh) * a.queries + q) * kTreePartFloats;
-    const float4 o1 = *reinterpret_cast<const float4*>(part + 4 * lane);
-    const float2 s1 = *reinterpret_cast<const float2*>(part + 256);
-    join(s1.x, s1.y, o1);
+  if (32 * tile + (lane & 31) < a.queries) {
+#pragma unroll 8
+    for (int i = wave; i <= a.ranges; i += 16) {
+      const float* const part = a.part + ((size_t)(i * a.kv_heads + kvh) * a.parts + tile) * kPart;
+      join(*reinterpret_cast<const float2*>(part + 8192 + 2 * (lane & 31)),
+           *reinterpret_cast<const float4*>(part + (64 * j + lane) * 4));
+    }
   }
   part_o[wave][lane] = o;
-  if (lane == 0) part_s[wave] = make_float2(ref, sum);
+  if (lane < 32) part_s[wave][lane] = make_float2(ref, sum);
   __syncthreads();
-  if (wave) return;
-  for (int w = 1; w < 4; ++w) join(part_s[w].x, part_s[w].y, part_o[w][lane]);
-  const size_t at = (size_t)row * a.q_heads + head;
-  const uint2 gate = *reinterpret_cast<const uint2*>(a.q_proj + at * 512 + 256 + 4 * lane);
+  if (wave || 32 * tile + (lane & 31) >= a.queries) return;
+  for (int w = 1; w < 16 && w <= a.ranges; ++w) join(part_s[w][lane & 31], part_o[w][lane]);
   auto gated = [&](float x, float z) { return x / sum / (1.0f + __builtin_amdgcn_exp2f(-z * 1.44269504088896341f)); };
   uint2 out = make_uint2(pack_bf2(gated(o.x, bf_lo(gate.x)), gated(o.y, bf_hi(gate.x))),
                          pack_bf2(gated(o.z, bf_lo(gate.y)), gated(o.w, bf_hi(gate.y))));
-  if (!tree_path(a.paths[row], row)) out = make_uint2(0, 0);
-  *reinterpret_cast<uint2*>(a.gated + at * 256 + 4 * lane) = out;
+  if (!path) out = make_uint2(0, 0);
+  *reinterpret_cast<uint2*>(a.gated + at * 256 + dim) = out;
 }
 
 // ---- an accepted path into the cache ----
@@ -439,22 +492,21 @@ int most_ranges(int kv_heads, int tiles) { return std::max(1, 256 / (kv_heads * 
 
 size_t tree_attn_scratch_bytes(int q_heads, int kv_heads, int rows) {
   const int queries = rows * (q_heads / kv_heads), tiles = (queries + kTileQ - 1) / kTileQ;
-  return (size_t)rows * q_heads * 512 +
-         (size_t)(most_ranges(kv_heads, tiles) + 1) * kv_heads * queries * kTreePartFloats * sizeof(float);
+  return (size_t)(most_ranges(kv_heads, tiles) + 1) * kv_heads * ((queries + 31) / 32) * kPart * sizeof(float);
 }
 
 hipError_t launch_tree_attn(TreeAttn a, hipStream_t s) {
   a.group = a.q_heads / a.kv_heads;
+  a.group_inv = 0xffffffffu / (uint32_t)a.group + 1;  // its product's high word is q / group for q below 2^16
   a.queries = a.rows * a.group;
   a.tiles = (a.queries + kTileQ - 1) / kTileQ;
+  a.parts = (a.queries + 31) / 32;
   const int blocks = (a.position + kKeys - 1) / kKeys;
   a.ranges = std::min(most_ranges(a.kv_heads, a.tiles), (blocks + 1) / 2);
-  a.query = static_cast<uint16_t*>(a.scratch);
-  a.part = reinterpret_cast<float*>(a.query + (size_t)a.rows * a.q_heads * 256);
-  const int heads = a.rows * (a.q_heads + a.kv_heads), units = (a.ranges + 1) * a.kv_heads;
-  k_tree_prepare<<<(heads + 3) / 4, 256, 0, s>>>(a);
+  a.part = static_cast<float*>(a.scratch);
+  const int units = (a.ranges + 1) * a.kv_heads;
   k_tree_attn<<<(units + 7) / 8 * 8 * a.tiles, 512, 0, s>>>(a);
-  k_tree_join<<<a.rows * a.q_heads, 256, 0, s>>>(a);
+  k_tree_join<<<32 * a.parts * a.kv_heads, 1024, 0, s>>>(a);
   return hipGetLastError();
 }
 
