@@ -406,8 +406,8 @@ struct TreeAttn {
   void* scratch;
   uint16_t *k_tree, *gated;
   float* part;  // the scratch (by the launcher, as the rest)
-  int group, queries, tiles, parts, ranges;
-  uint32_t group_inv;
+  int group, queries, tiles, parts, ranges, per, more;
+  uint32_t group_inv, kv_heads_inv;
 };
 size_t tree_attn_scratch_bytes(int q_heads, int kv_heads, int rows);
 hipError_t launch_tree_attn(TreeAttn a, hipStream_t s);

@@ -85,19 +85,18 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   __shared__ uint32_t odd_rows[2];  // nodes whose V holds an infinity or a NaN
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  // the tiles that read the same keys on one XCD (block b on XCD b % 8)
-  const int unit = (blockIdx.x >> 3) / a.tiles * 8 + (blockIdx.x & 7), tile = (blockIdx.x >> 3) % a.tiles;
+  // the tiles that read the same keys on one XCD (a launch's blocks go to the 8 XCDs in turn, x first)
+  const int unit = 8 * blockIdx.z + blockIdx.x, tile = blockIdx.y;
   if (unit >= (a.ranges + 1) * a.kv_heads) return;
-  const int range = unit / a.kv_heads, kvh = unit % a.kv_heads;
+  const int range = a.kv_heads == 1 ? unit : (int)__umulhi((uint32_t)unit, a.kv_heads_inv), kvh = unit - range * a.kv_heads;
   const bool tree = range == a.ranges;
   const int n = tree ? a.rows : a.position;  // keys
-  const int blocks = (n + kKeys - 1) / kKeys;
   // A range is every `ranges`-th block of 32 keys, so that at any time all blocks read
   // one window of the cache: contiguous ranges read 256 streams at equal distances, at
   // 3.9 TB/s against 4.4, and 5.0 with loads that pass the caches by (1 node at 131008,
   // whole calls of 69, 60 and 54 us).
   const int first = tree ? 0 : range, every = tree ? 1 : a.ranges;
-  const int steps = (blocks - first + every - 1) / every;
+  const int steps = tree ? (n + kKeys - 1) / kKeys : a.per + (range < a.more);
   const int qi = lane & 15, g = lane >> 4, kh = wave >> 2;
   const int q0 = tile * kTileQ + 32 * (wave & 3);  // the wave's queries
   const bool busy = q0 < a.queries;
@@ -130,9 +129,8 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
       dma16_past_caches(vsrc, stage + 2 * (kKeys + r) * kRow, vchunk[i] + more, at);
     }
   };
-  // Small inputs; the queries, 16 a wave, into the stages after the first two; the first two stages.
-  const int l0 = 16 * wave;  // the queries of the tile that the wave makes
-  const bool makes = tile * kTileQ + l0 < a.queries;
+  // Small inputs; the queries, two an instruction, into the stages after the first two; the first two stages.
+  const int made = min(kTileQ, a.queries - tile * kTileQ);  // queries of the tile
   if (wave < 2) {
     if (lane < 32) dma16(Source(wave ? a.k_gain : a.q_gain), lds_bytes(gain[wave]), lane * 16, 0);
   } else if (wave == 2) {
@@ -141,14 +139,12 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
     if (lane < 2 * a.rows) dma4(Source(a.paths), lds_bytes(word), lane * 4, 0);
     if (lane + 64 < 2 * a.rows) dma4(Source(a.paths), lds_bytes(word + 32), lane * 4, 256);
   }
-  if (makes) {
-    const Source qsrc(a.q_proj + (size_t)kvh * a.group * 512);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int l = l0 + 2 * i + (lane >> 5), q = min(tile * kTileQ + l, a.queries - 1), row = node_of(q);
-      dma16(qsrc, kv_base + (uint32_t)(2 * (2 * kStage + (l0 + 2 * i) * kRow)),
-            (uint32_t)(row * a.q_heads + q - row * a.group) * 1024u + (uint32_t)(((lane & 31) ^ (l & 15)) * 16), 0);
-    }
+  const Source qsrc(a.q_proj + (size_t)kvh * a.group * 512);
+#pragma unroll 1
+  for (int i = 2 * wave; i < made; i += 16) {
+    const int l = i + (lane >> 5), q = min(tile * kTileQ + l, a.queries - 1), row = node_of(q);
+    dma16(qsrc, kv_base + (uint32_t)(2 * (2 * kStage + i * kRow)),
+          (uint32_t)(row * a.q_heads + q - row * a.group) * 1024u + (uint32_t)(((lane & 31) ^ (l & 15)) * 16), 0);
   }
   issue(first, 0);
   if (steps > 1) {
@@ -166,15 +162,17 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   if (t < 2) odd_rows[t] = 0;
   if (tree) wait_vmcnt<0>();
   stage_barrier();
-  // A head is made by four lanes, with dims 32 s + 8 g .. + 7: the queries, then the
-  // nodes' keys where this is their block (four waves, 16 each).
+  // A head is made by four lanes, with dims 32 s + 8 g .. + 7, 16 heads a wave: the
+  // queries, then the nodes' keys where this is their block. (With 16 lanes a head one
+  // round of four heads takes 2200 cycles, this one of 16 3300.)
+  const int qunits = (made + 15) >> 4, units = qunits + (tree ? (a.rows + 15) >> 4 : 0);
 #pragma unroll 1
-  for (int pass = 0; pass < (tree ? 2 : 1); ++pass) {
-    if (pass ? wave >= 4 || 16 * wave >= a.rows : !makes) continue;
-    const int r = l0 + qi;  // of the tile's queries or of the nodes
-    char* const head = reinterpret_cast<char*>(pass ? &kv[wave >> 1][(r & 31) * kRow] : &kv[2][r * kRow]);
-    const int node = pass ? r : node_of(min(tile * kTileQ + r, a.queries - 1));
-    const uint64_t path = node < a.rows ? tree_path(word[node], node) : 0;
+  for (int i = wave; i < units; i += 8) {
+    const bool key = i >= qunits;
+    const int r = 16 * (key ? i - qunits : i) + qi;  // of the nodes or of the tile's queries
+    char* const head = reinterpret_cast<char*>(key ? &kv[r >> 5][(r & 31) * kRow] : &kv[2][r * kRow]);
+    const int node = key ? min(r, a.rows - 1) : node_of(min(tile * kTileQ + r, a.queries - 1));
+    const uint64_t path = tree_path(word[node], node);
     u32x4 x[8];
 #pragma unroll
     for (int s = 0; s < 8; ++s) x[s] = *reinterpret_cast<const u32x4*>(head + ((4 * s + g) ^ qi) * 16);
@@ -185,28 +183,25 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
       for (int e = 0; e < 4; ++e) part[e] = fmaf(bf_hi(x[s][e]), bf_hi(x[s][e]), fmaf(bf_lo(x[s][e]), bf_lo(x[s][e]), part[e]));
     float2 p = rows_xor16((part[0] + part[1]) + (part[2] + part[3]));
     p = rows_xor32(p.x + p.y);
-    float ss = p.x + p.y, inv = 1.0f / sqrtf(ss * (1.0f / 256.0f) + 1e-6f);
+    const float ss = p.x + p.y;
+    float inv = __builtin_amdgcn_rsqf(ss * (1.0f / 256.0f) + 1e-6f);
     if (__any(!(ss < INFINITY))) {
       // The squares pass 32 bits' range before the head does: such a head by 2^-72, beside
       // which the eps is nothing. An infinity or a NaN stays one.
       float big = 0.0f;
-#pragma unroll 1
-      for (int e = 0; e < 64; ++e) {
-        const uint32_t w = *reinterpret_cast<const uint16_t*>(head + ((4 * (e >> 3) + g) ^ qi) * 16 + 2 * (e & 7));
-        big = fmaf(bf2f(w) * 0x1p-72f, bf2f(w) * 0x1p-72f, big);
-      }
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lo = bf_lo(x[s][e]) * 0x1p-72f, hi = bf_hi(x[s][e]) * 0x1p-72f;
+          big = fmaf(hi, hi, fmaf(lo, lo, big));
+          if (!(ss < INFINITY)) x[s][e] = pack_bf2(lo, hi);
+        }
       p = rows_xor16(big);
       p = rows_xor32(p.x + p.y);
-      if (!(ss < INFINITY)) {
-        inv = 1.0f / sqrtf((p.x + p.y) * (1.0f / 256.0f));
-        const float by = 0x1p-72f;  // exact on bf16 of this size; smaller dims are nothing beside it
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[s][e] = pack_bf2(bf_lo(x[s][e]) * by, bf_hi(x[s][e]) * by);
-      }
+      if (!(ss < INFINITY)) inv = __builtin_amdgcn_rsqf((p.x + p.y) * (1.0f / 256.0f));
     }
-    const uint16_t* const by = gain[pass] + 8 * g;
+    const uint16_t* const by = gain[key] + 8 * g;
     float lo[8];
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
@@ -237,16 +232,30 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[s][e] = pack_bf2(y[2 * e], y[2 * e + 1]);
     }
-    const bool out = pass && !path;  // a node left out has no key
+    uint16_t* const to = a.k_tree + ((size_t)node * a.kv_heads + kvh) * 256 + 8 * g;
+    const bool out = key && !path, store = key && tile == 0 && r < a.rows;
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      if (out) x[s] = u32x4{0, 0, 0, 0};
+      if (out) x[s] = u32x4{0, 0, 0, 0};  // a node left out has no key
       *reinterpret_cast<u32x4*>(head + ((4 * s + g) ^ qi) * 16) = x[s];
+      if (store) *reinterpret_cast<u32x4*>(to + 32 * s) = x[s];
     }
-    if (pass && tile == 0 && r < a.rows) {
-      uint16_t* const to = a.k_tree + ((size_t)r * a.kv_heads + kvh) * 256 + 8 * g;
+  }
+  if (tree) {
+    // A masked key's value counts 0 times: infinities and NaN leave the products and join at the end.
+    for (int key = t >> 4; key < kKeys * steps; key += 32) {
+      uint32_t* const v = reinterpret_cast<uint32_t*>(&kv[key >> 5][(kKeys + (key & 31)) * kRow + (t & 15) * 16]);
+      bool odd = false;
 #pragma unroll
-      for (int s = 0; s < 8; ++s) *reinterpret_cast<u32x4*>(to + 32 * s) = x[s];
+      for (int e = 0; e < 8; ++e) {
+        uint32_t w = v[e];
+        const bool lo = (w & 0x7f80u) == 0x7f80u, hi = (w & 0x7f800000u) == 0x7f800000u;
+        if (lo) w &= 0xffff0000u;
+        if (hi) w &= 0xffffu;
+        if (lo || hi) v[e] = w;
+        odd |= lo || hi;
+      }
+      if (odd && key < n) atomicOr(&odd_rows[key >> 5], 1u << (key & 31));
     }
   }
   stage_barrier();
@@ -276,45 +285,35 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
     const int r = 16 * kh + 8 * (g >> 1) + (qi >> 2);
     v_at[i] = (uint32_t)(2 * ((kKeys + r) * kRow + 32 * (i ^ (r & 3)) + 16 * (g & 1) + 4 * (qi & 3))) ^ (uint32_t)(256 * kh);
   }
-  int st = kStages - 1;
-  for (int i = 0, kb = first; i < steps; ++i, kb += every) {
-    st = (st + 1) % kStages;
-    const int ahead = min(i ? kStages - 2 : 1, steps - 1 - i);
-    if (ahead >= 2)
-      wait_vmcnt<8>();
-    else if (ahead == 1)
-      wait_vmcnt<4>();
-    else
-      wait_vmcnt<0>();
-    stage_barrier();  // block kb is there, and every wave is past block kb - 1 (or has its queries)
-    if (i == 0 && steps > 2) issue(kb + 2 * every, 2);
-    if (i + kStages - 1 < steps) issue(kb + (kStages - 1) * every, (st + kStages - 1) % kStages);
-    char* const stage = reinterpret_cast<char*>(kv[st]);
-    if (tree) {
-      // A masked key's value counts 0 times: infinities and NaN leave the products and join at the end.
-      uint32_t* const v = reinterpret_cast<uint32_t*>(stage + 2 * (kKeys + (t >> 4)) * kRow + (t & 15) * 32);
-      bool odd = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        uint32_t w = v[e];
-        const bool lo = (w & 0x7f80u) == 0x7f80u, hi = (w & 0x7f800000u) == 0x7f800000u;
-        if (lo) w &= 0xffff0000u;
-        if (hi) w &= 0xffffu;
-        if (lo || hi) v[e] = w;
-        odd |= lo || hi;
-      }
-      const int key = kb * kKeys + (t >> 4);
-      if (odd && key < n) atomicOr(&odd_rows[key >> 5], 1u << (key & 31));
-      stage_barrier();
-    }
-    if (!busy) continue;
-    f32x4 sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+  auto scores = [&](int st, f32x4 (&sc)[2]) {
+    const char* const stage = reinterpret_cast<const char*>(kv[st]);
+    sc[0] = sc[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
       const bf16x8 kf = *reinterpret_cast<const bf16x8*>(stage + k_at[s & 3] + 256 * (s >> 2));
 #pragma unroll
       for (int u = 0; u < 2; ++u) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[u][s], sc[u], 0, 0, 0);
     }
+  };
+  stage_barrier();  // every wave has its queries
+  if (steps > 2) issue(first + 2 * every, 2);
+  int st = 0;
+  for (int i = 0, kb = first; i < steps; ++i, kb += every) {
+    const int ahead = min(kStages - 2, steps - 1 - i);
+    if (ahead >= 2)
+      wait_vmcnt<8>();
+    else if (ahead == 1)
+      wait_vmcnt<4>();
+    else
+      wait_vmcnt<0>();
+    stage_barrier();  // block i is there, and every wave is past block i - 1
+    if (i + 3 < steps) issue(kb + 3 * every, (st + 3) % kStages);
+    char* const stage = reinterpret_cast<char*>(kv[st]);
+    const int now = st;
+    st = (st + 1) % kStages;
+    if (!busy) continue;
+    f32x4 sc[2];
+    scores(now, sc);
     // keys 4 g + r of query l % 16 of both groups -> keys 8 (l / 32) + e of query l % 32
     float x[8];
 #pragma unroll
@@ -504,8 +503,11 @@ hipError_t launch_tree_attn(TreeAttn a, hipStream_t s) {
   const int blocks = (a.position + kKeys - 1) / kKeys;
   a.ranges = std::min(most_ranges(a.kv_heads, a.tiles), (blocks + 1) / 2);
   a.part = static_cast<float*>(a.scratch);
+  a.per = a.ranges ? blocks / a.ranges : 0;
+  a.more = a.ranges ? blocks % a.ranges : 0;
   const int units = (a.ranges + 1) * a.kv_heads;
-  k_tree_attn<<<(units + 7) / 8 * 8 * a.tiles, 512, 0, s>>>(a);
+  a.kv_heads_inv = 0xffffffffu / (uint32_t)a.kv_heads + 1;
+  k_tree_attn<<<dim3(8, a.tiles, (units + 7) / 8), 512, 0, s>>>(a);
   k_tree_join<<<32 * a.parts * a.kv_heads, 1024, 0, s>>>(a);
   return hipGetLastError();
 }
