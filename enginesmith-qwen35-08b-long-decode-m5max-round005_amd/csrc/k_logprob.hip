@@ -8,12 +8,14 @@
 // keeps the digits of its log probability and of the entropy.
 //
 // One read of the row. A block walks a range of it in segments, 16 bytes a
-// thread and load, with the maximum so far as the reference of its sums; the
-// segment after the one at hand is on its way. The top list is kept in LDS as
-// 64-bit keys (the value's bits made monotone, then the complement of the index:
-// of equal values the lowest index ranks first), and a segment is looked at for it
-// only if its maximum passes the list's last value. Rows too few to fill the card
-// are cut in ranges, which a second kernel joins.
+// thread and load, the segment after the one at hand on its way; each wave keeps
+// sums of its own against the largest it has met. The top list is kept in LDS as
+// 64-bit keys (the value's bits made monotone, then the complement of the index: of
+// equal values the lowest index ranks first). Elements that pass the list's last
+// value as it was when the list was last brought up to date go to a buffer, and
+// only a buffer of some size is ranked: of 248320 logits some hundreds get there,
+// and one or two rankings a row do. Rows too few to fill the card are cut in ranges,
+// which a second kernel joins.
 #include <algorithm>
 
 #include "es_kernels.hpp"
@@ -22,8 +24,10 @@ namespace es {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr int kCand = 1024;  // candidates a selection ranks at once: kLogprobTop lists or threads of 32
-static_assert(kLogprobTop == 32, "kCand holds 32 elements of 32 threads, or 32 lists of 32");
+constexpr int kCand = 1024 + 2;  // keys of the buffer, and room behind them
+constexpr int kMost = 1024;      // keys it takes
+constexpr int kFlush = 256;      // keys from which it is ranked
+static_assert(kLogprobTop * kLogprobTop <= kMost, "the join ranks as many lists as the list is long");
 
 struct RangeStats {
   float m;       // largest logit (NaN if there is one)
@@ -43,6 +47,11 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   const uint32_t o = (uint32_t)(key >> 32);
   return o == 0 ? __builtin_nanf("") : bf2f(o & 0x8000u ? o ^ 0x8000u : o ^ 0xffffu);
 }
+// The lowest value that passes v; -inf where v is a NaN, which everything else passes.
+__device__ __forceinline__ float above(float v) {
+  const int b = __float_as_int(v);
+  return v != v ? -__builtin_inff() : v == 0.0f ? __int_as_float(1) : __int_as_float(b < 0 ? b - 1 : b + 1);
+}
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return ~(uint32_t)key; }
 
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
@@ -60,25 +69,31 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 struct Shared {
-  uint64_t list[2][kLogprobTop];  // the largest keys so far, in order; one of the two at a time
-  uint64_t cand[kCand];
-  float lane_max[256];
+  uint64_t list[2][kLogprobTop];  // the largest keys when last brought up to date, in order; one of the two at a time
+  __attribute__((aligned(16))) uint64_t cand[kCand];
+  __attribute__((aligned(16))) float group_max[64];
   uint64_t wave_key[2][4];
-  float wave_max[2][4];
+  float wave_m[4];
   double sum[2][4];
-  float t0;
-  int count;
+  int count[4];
 };
 
 // Joins the n candidates to the nl keys of list `at`: the `top` largest of both,
 // in order, into the other one. A key's place is the number of larger ones.
 __device__ __forceinline__ void rank_into(Shared& sh, int at, int nl, int n, int top) {
-  const int all = nl + n;
-  for (int i = threadIdx.x; i < all; i += 256) {
+  typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+  if (threadIdx.x == 0) sh.cand[n] = 0;  // pairs are compared
+  __syncthreads();
+  for (int i = threadIdx.x; i < nl + n; i += 256) {
     const uint64_t mine = i < nl ? sh.list[at][i] : sh.cand[i - nl];
     int place = 0;
+#pragma unroll 1
     for (int j = 0; j < nl; ++j) place += sh.list[at][j] > mine;
-    for (int j = 0; j < n; ++j) place += sh.cand[j] > mine;
+#pragma unroll 2
+    for (int j = 0; j < n; j += 2) {
+      const u64x2 two = *reinterpret_cast<const u64x2*>(&sh.cand[j]);
+      place += (two[0] > mine) + (two[1] > mine);
+    }
     if (place < top) sh.list[at ^ 1][place] = mine;
   }
   __syncthreads();
@@ -88,7 +103,7 @@ __device__ __forceinline__ void rank_into(Shared& sh, int at, int nl, int n, int
 __device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, float m, double r, double d,
                                            const uint64_t* list) {
   const bool finite = fabsf(m) < __builtin_inff();
-  const double log_sum = finite ? log1p(r) : (double)__builtin_nanf("");
+  const double log_sum = finite ? (double)log1pf((float)r) : (double)__builtin_nanf("");
   if (threadIdx.x == 0) {
     if (a.logprob) {
       const uint32_t token = a.tokens[row];
@@ -109,130 +124,154 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, float 
 
 // V: 16-byte vectors of a thread in a segment.
 template <int V>
-__global__ __launch_bounds__(256) void k_logprob(LogprobArgs a) {
+__global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) {
   __shared__ Shared sh;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int row = blockIdx.x / a.ranges, range = blockIdx.x % a.ranges;
-  // Vectors lie on the 16-byte grid of memory: vector j holds elements 8 j - off .. + 7 of the row.
+  const int row = blockIdx.x, range = blockIdx.y, top = a.top;
+  // Vectors lie on the 16-byte grid of memory: vector j holds elements 8 j - off .. + 7
+  // of the row. Those with elements outside the row are segments of their own.
   const uint16_t* const x0 = a.logits + (int64_t)row * a.stride;
   const int off = (int)((uintptr_t)x0 >> 1 & 7);
   const u32x4* const grid = reinterpret_cast<const u32x4*>(x0 - off);
   const int j0 = range * a.per, j1 = min(j0 + a.per, (a.vocab + off + 7) >> 3);
-  const int whole0 = off ? 1 : 0, whole1 = (a.vocab + off) >> 3;  // vectors within the row
-  auto load = [&](int first, u32x4 (&x)[V]) {
+  const int whole0 = max(j0, off ? 1 : 0), whole1 = min(j1, (a.vocab + off) >> 3);  // of vectors within the row
+  const bool head = j0 < whole0 && j0 < j1, tail = whole1 < j1 && whole1 >= j0 + head;
+  const int main = max(0, (whole1 - whole0 + 256 * V - 1) / (256 * V));
+  const int first = head ? -1 : 0, last = main + tail;  // segments -1 (the head), 0 .. main - 1, main (the tail)
+  auto load = [&](int s, u32x4 (&x)[V]) {
+    const int j = whole0 + s * 256 * V + t;
+    if (s >= 0 && whole0 + (s + 1) * 256 * V <= whole1) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int j = first + v * 256 + t;
-      x[v] = u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};  // -inf outside the row
-      if (j >= whole0 && j < min(whole1, j1)) {
-        x[v] = grid[j];
-      } else if (j < j1) {
-        uint64_t lo = 0, hi = 0;
-#pragma unroll 1
-        for (int e = 7; e >= 0; --e) {
-          const int i = 8 * j + e - off;
-          hi = hi << 16 | lo >> 48;
-          lo = lo << 16 | (i >= 0 && i < a.vocab ? x0[i] : 0xff80u);
-        }
-        x[v] = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
-      }
+      for (int v = 0; v < V; ++v) x[v] = __builtin_nontemporal_load(grid + j + 256 * v);
+      return;
     }
-  };
-  // f(element, index) of the thread's elements of the row, in a rolled loop: for what few segments need
-  auto each = [&](const u32x4 (&x)[V], int seg, auto f) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      uint64_t lo = x[v][0] | (uint64_t)x[v][1] << 32, hi = x[v][2] | (uint64_t)x[v][3] << 32;
-      const int j = seg + v * 256 + t;
-      if (j >= j1) continue;
+    for (int v = 0; v < V; ++v) x[v] = u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};  // -inf outside
+    if (s >= 0 && s < main) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (j + 256 * v < whole1) x[v] = grid[j + 256 * v];
+    } else if (t == 0) {  // the elements of one vector that are the row's
+      const int at = 8 * (s < 0 ? 0 : whole1) - off;
+      uint64_t lo = 0, hi = 0;
 #pragma unroll 1
-      for (int e = 0; e < 8; ++e) {
-        const int i = 8 * j + e - off;
-        if (i >= 0 && i < a.vocab) f(bf2f((uint32_t)lo & 0xffffu), (uint32_t)i);
-        lo = lo >> 16 | hi << 48;
-        hi >>= 16;
+      for (int e = 7; e >= 0; --e) {
+        hi = hi << 16 | lo >> 48;
+        lo = lo << 16 | (at + e >= 0 && at + e < a.vocab ? x0[at + e] : 0xff80u);
       }
+      x[0] = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
     }
   };
   auto value = [](const u32x4 (&x)[V], int v, int e) { return e & 1 ? bf_hi(x[v][e >> 1]) : bf_lo(x[v][e >> 1]); };
-  float m = -__builtin_inff(), last = -__builtin_inff();  // largest so far; the list's last value once it is full
-  float r = 0.0f, d = 0.0f;                               // the thread's part of R and D
-  int at = 0, nl = 0, buf = 0;
+  // the row's index of element 0 of the thread's vector v in segment s; far below 0 where there is none
+  auto index_of = [&](int s, int v) {
+    if (s < 0 || s >= main) return t == 0 && v == 0 ? 8 * (s < 0 ? 0 : whole1) - off : -64;
+    const int j = whole0 + s * 256 * V + 256 * v + t;
+    return j < whole1 ? 8 * j - off : -64;
+  };
+  auto half = [](const u32x4& x, int h) {  // element h, h from a rolled loop
+    const uint32_t w = h < 2 ? x[0] : h < 4 ? x[1] : h < 6 ? x[2] : x[3];
+    return h & 1 ? bf_hi(w) : bf_lo(w);
+  };
+  // f(element, index) of the thread's elements, in a rolled loop: few threads need it
+  auto each = [&](const u32x4 (&x)[V], int s, auto f) {
+#pragma unroll 1
+    for (int h = 0; h < 8; ++h)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int i = index_of(s, v) + h;
+        if (i >= 0 && i < a.vocab) f(half(x[v], h), (uint32_t)i);
+      }
+  };
+  float m = -__builtin_inff();   // the wave's largest so far
+  float r = 0.0f, d = 0.0f;      // the thread's part of R and D
+  float bar = -__builtin_inff(); // what passes the last value of the full list reaches it
+  int at = 0, nl = 0, held = 0, turn = 0;  // the list in use, its keys, and the buffer's
+  if (t < 4) sh.count[t] = 0;
+  __syncthreads();
   u32x4 next[V];
-  load(j0, next);
-  for (int seg = j0; seg < j1; seg += 256 * V) {
+  if (first < last) load(first, next);
+  for (int s = first; s < last; ++s) {
     u32x4 x[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) x[v] = next[v];
-    if (seg + 256 * V < j1) load(seg + 256 * V, next);
-    float tm = -__builtin_inff();
+    if (s + 1 < last) load(s + 1, next);
+    float vm[V], tm = -__builtin_inff();  // a NaN is passed over
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int v = 0; v < V; ++v) {
+      vm[v] = fmaxf(value(x, v, 0), value(x, v, 1));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) tm = maximum(tm, value(x, v, e));
-    float wm = tm;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) wm = maximum(wm, __shfl_xor(wm, s));
-    if (lane == 0) sh.wave_max[buf][wave] = wm;
-    __syncthreads();
-    const float* const w = sh.wave_max[buf];
-    const float ms = maximum(maximum(w[0], w[1]), maximum(w[2], w[3]));
-    const int first_wave = w[0] == ms ? 0 : w[1] == ms ? 1 : w[2] == ms ? 2 : 3;
-    buf ^= 1;
-    if (a.top && !(nl == a.top && ms <= last)) {
-      // Candidates pass the list's last value, or, while the list is not full, reach
-      // the top-th largest of the threads' maxima, which as many elements at least do.
-      const int top = a.top;
-      const bool nan = ms != ms || last != last;
-      bool strict = nl == top, done = false;
-      auto threshold = [&] {
-        sh.lane_max[t] = tm;
-        __syncthreads();
-        int gt = 0, ge = 0;
-        for (int i = 0; i < 256; ++i) {
-          const float o = sh.lane_max[i];
-          gt += o > tm;
-          ge += o >= tm;
-        }
-        if (gt < top && ge >= top) sh.t0 = tm;
-        __syncthreads();
-        return sh.t0;
-      };
-      float thr = last;
-      int n = 0;
-      if (!nan) {
-        if (!strict) thr = threshold();
-        for (int attempt = 0; attempt < 2; ++attempt) {
-          if (t == 0) sh.count = 0;
+      for (int e = 2; e < 8; e += 2) vm[v] = fmaxf(vm[v], fmaxf(value(x, v, e), value(x, v, e + 1)));
+      tm = fmaxf(tm, vm[v]);
+    }
+    if (top) {
+      // What passes the full list's last value joins the buffer. Where the list is not
+      // full, or more pass than the buffer takes, it is what reaches the top-th largest
+      // of the 64 groups' maxima of this segment, which as many elements at least do.
+      bool full = nl == top, slow = false;
+      const int before = held;
+#pragma unroll 1
+      for (;;) {
+        float thr = bar;
+        if (!full) {
+          float gm = fmaxf(tm, dpp_xor1(tm));
+          gm = fmaxf(gm, dpp_xor2(gm));
+          if ((t & 3) == 0) sh.group_max[t >> 2] = gm;
           __syncthreads();
-          if (strict ? tm > thr : tm >= thr)
-            each(x, seg, [&](float y, uint32_t i) {
-              if (strict ? y > thr : y >= thr) {
-                const int p = atomicAdd(&sh.count, 1);
-                if (p < kCand) sh.cand[p] = key_of(y, i);
+          const float mine = sh.group_max[lane];
+          int gt = 0, ge = 0;
+#pragma unroll 2
+          for (int i = 0; i < 64; i += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(&sh.group_max[i]);
+            gt += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+            ge += (o.x >= mine) + (o.y >= mine) + (o.z >= mine) + (o.w >= mine);
+          }
+          thr = __shfl(mine, __builtin_ctzll(__ballot(gt < top && ge >= top)));
+        }
+        int* const count = &sh.count[turn & 3];
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (vm[v] >= thr) {
+            uint32_t hits = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) hits |= value(x, v, e) >= thr ? 1u << e : 0u;
+            const int i0 = index_of(s, v);
+            for (; hits; hits &= hits - 1) {
+              const int e = __builtin_ctz(hits), i = i0 + e;
+              if (i >= 0 && i < a.vocab) {
+                const int p = held + atomicAdd(count, 1);
+                if (p < kMost) sh.cand[p] = key_of(half(x[v], e), i);
               }
-            });
-          __syncthreads();
-          n = sh.count;
-          __syncthreads();
-          done = n <= kCand;
-          if (done || !strict) break;
-          // over kCand elements pass `last`, so more threads than the list is long do: their top-th maximum passes it too
-          thr = threshold();
-          strict = false;
+            }
+          }
+        __syncthreads();
+        // a count for each turn, cleared two turns ahead: one barrier a segment
+        int n = held + *count;
+        if (t == 0) sh.count[(turn + 2) & 3] = 0;
+        ++turn;
+        const bool over = n > kMost;
+        if (over) n = full ? before : 0;  // without this segment's
+        const int there = s < 0 ? min(8 - off, a.vocab) : s >= main ? a.vocab + off - 8 * whole1 : min(256 * V, whole1 - whole0 - s * 256 * V) * 8;
+        slow = !full && (over || n < min(top, there));  // too many equals, or fewer than there are: the others are NaN
+        held = n;
+        if (!slow && (!full || over || n >= kFlush || s + 1 == last)) {
+          rank_into(sh, at, nl, n, top);
+          nl = min(top, nl + n);
+          at ^= 1;
+          bar = nl == top ? above(key_value(sh.list[at][top - 1])) : -__builtin_inff();
+          held = 0;
         }
+        if (!(over && full)) break;
+        full = false;
       }
-      if (done) {
-        rank_into(sh, at, nl, n, top);
-        nl = min(top, nl + n);
-      } else {
-        // Too many equals, or a NaN: the largest key below the one before, `top` times.
+      if (slow) {
+        // The largest key below the one before, `top` times (the buffer is empty).
         uint64_t below = ~0ull;
         int got = 0;
         for (; got < top; ++got) {
           uint64_t best = 0;
           if (t < nl && sh.list[at][t] < below) best = sh.list[at][t];
-          each(x, seg, [&](float y, uint32_t i) {
+          each(x, s, [&](float y, uint32_t i) {
             const uint64_t k = key_of(y, i);
             if (k < below && k > best) best = k;
           });
@@ -246,44 +285,40 @@ __global__ __launch_bounds__(256) void k_logprob(LogprobArgs a) {
           below = best;
         }
         nl = got;
+        at ^= 1;
+        held = 0;
         __syncthreads();
+        bar = nl == top ? above(key_value(sh.list[at][top - 1])) : -__builtin_inff();
       }
-      at ^= 1;
-      last = nl == top ? key_value(sh.list[at][top - 1]) : -__builtin_inff();
     }
-    if (!(fabsf(ms) < __builtin_inff())) {  // only -inf, or an infinity or a NaN, which stays
-      m = maximum(m, ms);
+    const float ms = wave_max(tm);
+    if (!(fabsf(ms) < __builtin_inff()) || m == __builtin_inff()) {
+      // nothing but -inf and NaN, or an infinity, which stays: only a NaN is still told apart
+      m = fmaxf(m, ms);
+#pragma unroll 1
+      for (int h = 0; h < 8; ++h)
+#pragma unroll
+        for (int v = 0; v < V; ++v) r = half(x[v], h) != half(x[v], h) ? __builtin_nanf("") : r;
       continue;
     }
-    if (ms > m) {
+    const bool fresh = ms > m;
+    if (fresh) {
       if (m > -__builtin_inff()) {  // the sums to the new reference; what was the largest joins them
         const float delta = (m - ms) * kLog2e, f = __builtin_amdgcn_exp2f(delta);
         d = f > 0.0f ? f * fmaf(delta, r, d) : 0.0f;
         r *= f;
-        if (t == 0 && f > 0.0f) {
+        if (lane == 0 && f > 0.0f) {
           r += f;
           d = fmaf(f, delta, d);
         }
       }
       m = ms;
-      if (wave == first_wave && lane == __ffsll(__ballot(tm == ms)) - 1) {  // one copy of it leaves
-        bool gone = false;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const bool hit = !gone && value(x, v, e) == ms;
-            if (hit) x[v][e >> 1] = e & 1 ? (x[v][e >> 1] & 0xffffu) | 0xff800000u : (x[v][e >> 1] & 0xffff0000u) | 0xff80u;
-            gone |= hit;
-          }
-      }
     }
-    if (!(fabsf(m) < __builtin_inff())) continue;
     // x log2(e) - c in one rounding, c = m log2(e) rounded; delta takes the sums to m itself
     const bool small = fabsf(m) < 1e30f;
     const float c = m * kLog2e, delta = fmaf(m, kLog2e, -c);
     float pr = 0.0f, pd = 0.0f;
-    if (small) {
+    if (small && !fresh) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
@@ -293,38 +328,64 @@ __global__ __launch_bounds__(256) void k_logprob(LogprobArgs a) {
           pd = fmaf(p, z, pd);
         }
     }
-    if (!small || __any(pd != pd)) {  // an excluded element (0 times -inf), or magnitudes that the product would pass
+    if (!small || fresh || __any(pd != pd)) {
+      // The largest, of which one copy stays out; excluded elements, where 0 times -inf is 0
+      // here; magnitudes that the product would pass.
+      bool out = fresh && lane == __builtin_ctzll(__ballot(tm == ms));
       pr = pd = 0.0f;
+#pragma unroll 1
+      for (int h = 0; h < 8; ++h)
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float z = small ? fmaf(value(x, v, e), kLog2e, -c) : (value(x, v, e) - m) * kLog2e;
-          const float p = __builtin_amdgcn_exp2f(z);
+        for (int v = 0; v < V; ++v) {
+          const float y = half(x[v], h), z = small ? fmaf(y, kLog2e, -c) : (y - m) * kLog2e;
+          const bool skip = out && y == ms;
+          out = out && !skip;
+          const float p = skip ? 0.0f : __builtin_amdgcn_exp2f(z);
           pr += p;
-          pd = fmaf(p, fmaxf(z, -3e38f), pd);
+          pd = fmaf(p, z > -3e38f ? z : -3e38f, pd);
         }
     }
     const float f = small ? __builtin_amdgcn_exp2f(-delta) : 1.0f;
     d = fmaf(f, small ? fmaf(-delta, pr, pd) : pd, d);
     r = fmaf(f, pr, r);
   }
-  const double wr = wave_sum((double)r), wd = wave_sum((double)d);
+  // the waves' sums to the block's largest, in 64 bits; the largest of the other waves join
+  if (lane == 0) sh.wave_m[wave] = m;
+  __syncthreads();
+  const float* const w = sh.wave_m;
+  const float all = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+  const int owner = w[0] == all ? 0 : w[1] == all ? 1 : w[2] == all ? 2 : 3;
+  double sr = wave_sum((double)r), sd = wave_sum((double)d);
+  if (m > -__builtin_inff() && fabsf(all) < __builtin_inff()) {
+    if (wave != owner) {
+      const float delta = (m - all) * kLog2e, f = __builtin_amdgcn_exp2f(delta);
+      sr += 1.0;
+      sd = f > 0.0f ? f * (sd + delta * sr) : 0.0;
+      sr *= f;
+    }
+  }
   if (lane == 0) {
-    sh.sum[0][wave] = wr;
-    sh.sum[1][wave] = wd;
+    sh.sum[0][wave] = sr;
+    sh.sum[1][wave] = sd;
   }
   __syncthreads();
-  const double sr = sh.sum[0][0] + sh.sum[0][1] + sh.sum[0][2] + sh.sum[0][3];
-  const double sd = sh.sum[1][0] + sh.sum[1][1] + sh.sum[1][2] + sh.sum[1][3];
-  if (a.ranges == 1) {
-    finish_row(a, row, m, sr, sd, sh.list[at]);
+  sr = sh.sum[0][0] + sh.sum[0][1] + sh.sum[0][2] + sh.sum[0][3];
+  sd = sh.sum[1][0] + sh.sum[1][1] + sh.sum[1][2] + sh.sum[1][3];
+  const float largest = sr != sr ? __builtin_nanf("") : all;
+  // The outputs' addresses are fetched here again: held through the loop they leave too few scalar registers.
+  typedef const __attribute__((address_space(4))) LogprobArgs* kernarg;
+  kernarg late = (kernarg)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(late));
+  const LogprobArgs b = *(const LogprobArgs*)late;
+  if (b.ranges == 1) {
+    finish_row(b, row, largest, sr, sd, sh.list[at]);
     return;
   }
-  RangeStats* const stats = static_cast<RangeStats*>(a.scratch);
-  uint64_t* const keys = reinterpret_cast<uint64_t*>(stats + (size_t)a.rows * a.ranges);
-  if (t == 0) stats[blockIdx.x] = RangeStats{m, 0.0f, sr, sd};
-  if (t < a.top) keys[(size_t)blockIdx.x * a.top + t] = t < nl ? sh.list[at][t] : 0;
+  RangeStats* const stats = static_cast<RangeStats*>(b.scratch);
+  uint64_t* const keys = reinterpret_cast<uint64_t*>(stats + (size_t)b.rows * b.ranges);
+  const size_t block = (size_t)row * b.ranges + range;
+  if (t == 0) stats[block] = RangeStats{largest, 0.0f, sr, sd};
+  if (t < top) keys[block * top + t] = t < nl ? sh.list[at][t] : 0;
 }
 
 // Joins a row's ranges (at most 256): a thread each for the sums, then the top
@@ -332,33 +393,34 @@ __global__ __launch_bounds__(256) void k_logprob(LogprobArgs a) {
 // first keys hold all of it.
 __global__ __launch_bounds__(256) void k_logprob_join(LogprobArgs a) {
   __shared__ Shared sh;
-  __shared__ uint64_t heads[256];
-  __shared__ uint64_t t0;
+  __shared__ __attribute__((aligned(16))) uint64_t heads[256];
+  __shared__ int lists[kLogprobTop];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.x, top = a.top, n = a.ranges;
   const RangeStats* const stats = static_cast<const RangeStats*>(a.scratch) + (size_t)row * n;
   const uint64_t* const keys =
       reinterpret_cast<const uint64_t*>(static_cast<const RangeStats*>(a.scratch) + (size_t)a.rows * n) + (size_t)row * n * top;
   RangeStats s = {-__builtin_inff(), 0.0f, 0.0, 0.0};
-  if (t < n) s = stats[t];
+  uint64_t mine = 0;
+  if (t < n) {
+    s = stats[t];
+    if (top) mine = keys[(size_t)t * top];
+  }
   float m = s.m;
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) m = maximum(m, __shfl_xor(m, k));
-  if (lane == 0) sh.wave_max[0][wave] = m;
-  if (top) heads[t] = t < n ? keys[(size_t)t * top] : 0;
-  if (t == 0) {
-    sh.count = 0;
-    t0 = 0;
-  }
+  if (lane == 0) sh.wave_m[wave] = m;
+  heads[t] = mine;
+  if (t == 0) sh.count[0] = 0;
   __syncthreads();
-  const float* const w = sh.wave_max[0];
+  const float* const w = sh.wave_m;
   m = maximum(maximum(w[0], w[1]), maximum(w[2], w[3]));
   const int first_wave = w[0] == m ? 0 : w[1] == m ? 1 : w[2] == m ? 2 : 3;
   double r = 0.0, d = 0.0;
   if (fabsf(m) < __builtin_inff() && s.m > -__builtin_inff()) {
-    const double delta = ((double)s.m - (double)m) * 1.4426950408889634074, f = exp2(delta);
+    const float delta = (s.m - m) * kLog2e, f = __builtin_amdgcn_exp2f(delta);
     const bool owner = wave == first_wave && lane == __ffsll(__ballot(s.m == m)) - 1;
     r = s.r + (owner ? 0.0 : 1.0);
-    d = f > 0.0 ? f * (s.d + delta * r) : 0.0;
+    d = f > 0.0f ? f * (s.d + delta * r) : 0.0;
     r *= f;
   }
   r = wave_sum(r);
@@ -368,21 +430,25 @@ __global__ __launch_bounds__(256) void k_logprob_join(LogprobArgs a) {
     sh.sum[1][wave] = d;
   }
   if (top) {
-    if (n >= top && t < n) {
-      int place = 0;
-      for (int i = 0; i < n; ++i) place += heads[i] > heads[t];
-      if (place == top - 1) t0 = heads[t];
+    // a list's place among the first keys; only one range can be empty, so that no two are equal
+    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+    int place = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; i += 2) {
+      const u64x2 two = *reinterpret_cast<const u64x2*>(&heads[i]);
+      place += (two[0] > mine) + (two[1] > mine);
+    }
+    if (t < n && place < top) lists[place] = t;
+    __syncthreads();
+    const int many = min(n, top);
+    const uint64_t last = n >= top ? heads[lists[top - 1]] : 0;
+    for (int i = t; i < many * top; i += 256) {
+      const int list = i / top;
+      const uint64_t key = keys[(size_t)lists[list] * top + (i - list * top)];
+      if (key && key >= last) sh.cand[atomicAdd(&sh.count[0], 1)] = key;
     }
     __syncthreads();
-    if (t < n && heads[t] >= t0) {
-      for (int i = 0; i < top; ++i) {
-        const uint64_t key = keys[(size_t)t * top + i];
-        if (key < t0 || key == 0) break;
-        sh.cand[atomicAdd(&sh.count, 1)] = key;  // at most top lists of top keys: kCand
-      }
-    }
-    __syncthreads();
-    rank_into(sh, 0, 0, sh.count, top);
+    rank_into(sh, 0, 0, sh.count[0], top);
   } else {
     __syncthreads();
   }
@@ -409,7 +475,7 @@ size_t logprob_scratch_bytes(int rows, int vocab, int top) {
 
 hipError_t launch_logprob(LogprobArgs a, hipStream_t s) {
   a.ranges = ranges_of(a.rows, a.vocab, &a.per);
-  const dim3 grid((unsigned)a.rows * a.ranges);
+  const dim3 grid(a.rows, a.ranges);
   if (a.per >= 1024)
     k_logprob<4><<<grid, 256, 0, s>>>(a);
   else

@@ -146,6 +146,19 @@ def test_rows_with_a_nan_or_an_infinity(bad):
         check(x, vocab, tokens, 13, run(x, vocab, tokens, 13))
 
 
+def test_values_behind_a_beginning_of_nan():
+    """A list full of NaN takes every value after them, -inf too."""
+    for vocab, end in ((30000, 9000), (100000, 99990), (300, 290)):
+        x, tokens = logits(3, vocab, 5)
+        x[0, :end] = float("nan")
+        x[1, :end] = float("nan")
+        x[1, end:] = -INF
+        x[2, :end] = -INF
+        x[2, end + 3:] = float("nan")
+        tokens %= vocab
+        check(x, vocab, tokens, 20, run(x, vocab, tokens, 20))
+
+
 def test_rows_without_a_finite_logit():
     x, tokens = logits(2, 300, 5)
     x[1] = -INF
