@@ -24,10 +24,9 @@ namespace es {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr int kCand = 1024 + 2;  // keys of the buffer, and room behind them
-constexpr int kMost = 1024;      // keys it takes
-constexpr int kFlush = 12;       // keys beyond the list's length from which it is ranked: late, more pass; often, more rankings
-                                 // (2048 rows of 248320, 5 and 20 alternatives: 292 and 291 us at 256 keys, 263 and 259 here)
+constexpr int kMost = 1024;  // keys the buffer takes
+constexpr int kFlush = 12;   // keys beyond the list's length from which it is ranked: late, more pass; often, more rankings
+                             // (2048 rows of 248320, 5 and 20 alternatives: 292 and 291 us at 256 keys, 263 and 259 here)
 static_assert(kLogprobTop * kLogprobTop <= kMost, "the join ranks as many lists as the list is long");
 
 struct RangeStats {
@@ -70,8 +69,9 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 struct Shared {
-  uint64_t list[2][kLogprobTop];  // the largest keys when last brought up to date, in order; one of the two at a time
-  __attribute__((aligned(16))) uint64_t cand[kCand];
+  // the top list in order, zeros behind it; from kLogprobTop on the buffer of keys not yet ranked
+  __attribute__((aligned(16))) uint64_t keys[kLogprobTop + kMost + 8];
+  uint64_t out[kLogprobTop];
   __attribute__((aligned(16))) float group_max[64];
   uint64_t wave_key[2][4];
   float wave_m[4];
@@ -79,25 +79,32 @@ struct Shared {
   int count[4];
 };
 
-// Joins the n candidates to the nl keys of list `at`: the `top` largest of both,
-// in order, into the other one. A key's place is the number of larger ones.
-__device__ __forceinline__ void rank_into(Shared& sh, int at, int nl, int n, int top) {
-  typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
-  if (threadIdx.x == 0) sh.cand[n] = 0;  // pairs are compared
+// The new list from `out`, whose first n are its keys.
+__device__ __forceinline__ void new_list(Shared& sh, int n) {
   __syncthreads();
-  for (int i = threadIdx.x; i < nl + n; i += 256) {
-    const uint64_t mine = i < nl ? sh.list[at][i] : sh.cand[i - nl];
+  if (threadIdx.x < kLogprobTop) sh.keys[threadIdx.x] = (int)threadIdx.x < n ? sh.out[threadIdx.x] : 0;
+  __syncthreads();
+}
+// Joins the n keys of the buffer to the nl of the list. A key's place is the
+// number of larger ones, and no two are equal.
+__device__ __forceinline__ void rank_all(Shared& sh, int nl, int n, int top) {
+  typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+  if (threadIdx.x < 8) sh.keys[kLogprobTop + n + threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kLogprobTop + n; i += 256) {
+    const uint64_t mine = sh.keys[i];
+    if (mine == 0) continue;
     int place = 0;
 #pragma unroll 1
-    for (int j = 0; j < nl; ++j) place += sh.list[at][j] > mine;
-#pragma unroll 2
-    for (int j = 0; j < n; j += 2) {
-      const u64x2 two = *reinterpret_cast<const u64x2*>(&sh.cand[j]);
-      place += (two[0] > mine) + (two[1] > mine);
+    for (int j = 0; j < kLogprobTop + n; j += 8) {
+      const u64x2* const at = reinterpret_cast<const u64x2*>(&sh.keys[j]);
+      const u64x2 k0 = at[0], k1 = at[1], k2 = at[2], k3 = at[3];
+      place += (k0[0] > mine) + (k0[1] > mine) + (k1[0] > mine) + (k1[1] > mine);
+      place += (k2[0] > mine) + (k2[1] > mine) + (k3[0] > mine) + (k3[1] > mine);
     }
-    if (place < top) sh.list[at ^ 1][place] = mine;
+    if (place < top) sh.out[place] = mine;
   }
-  __syncthreads();
+  new_list(sh, min(top, nl + n));
 }
 
 // A row's outputs from its largest logit, R, D and the list (called by the whole block).
@@ -187,8 +194,9 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
   float m = -__builtin_inff();   // the wave's largest so far
   float r = 0.0f, d = 0.0f;      // the thread's part of R and D
   float bar = -__builtin_inff(); // what passes the last value of the full list reaches it
-  int at = 0, nl = 0, held = 0, turn = 0;  // the list in use, its keys, and the buffer's
+  int nl = 0, held = 0, turn = 0;  // keys of the list, and of the buffer
   if (t < 4) sh.count[t] = 0;
+  if (t < kLogprobTop) sh.keys[t] = 0;
   __syncthreads();
   u32x4 next[V];
   if (first < last) load(first, next);
@@ -221,7 +229,7 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
           __syncthreads();
           const float mine = sh.group_max[lane];
           int gt = 0, ge = 0;
-#pragma unroll 2
+#pragma unroll 4
           for (int i = 0; i < 64; i += 4) {
             const float4 o = *reinterpret_cast<const float4*>(&sh.group_max[i]);
             gt += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
@@ -241,7 +249,7 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
               const int e = __builtin_ctz(hits), i = i0 + e;
               if (i >= 0 && i < a.vocab) {
                 const int p = held + atomicAdd(count, 1);
-                if (p < kMost) sh.cand[p] = key_of(half(x[v], e), i);
+                if (p < kMost) sh.keys[kLogprobTop + p] = key_of(half(x[v], e), i);
               }
             }
           }
@@ -256,10 +264,9 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
         slow = !full && (over || n < min(top, there));  // too many equals, or fewer than there are: the others are NaN
         held = n;
         if (!slow && (!full || over || n >= kFlush + top || s + 1 == last)) {
-          rank_into(sh, at, nl, n, top);
+          rank_all(sh, nl, n, top);
           nl = min(top, nl + n);
-          at ^= 1;
-          bar = nl == top ? above(key_value(sh.list[at][top - 1])) : -__builtin_inff();
+          bar = nl == top ? above(key_value(sh.keys[top - 1])) : -__builtin_inff();
           held = 0;
         }
         if (!(over && full)) break;
@@ -271,7 +278,7 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
         int got = 0;
         for (; got < top; ++got) {
           uint64_t best = 0;
-          if (t < nl && sh.list[at][t] < below) best = sh.list[at][t];
+          if (t < nl && sh.keys[t] < below) best = sh.keys[t];
           each(x, s, [&](float y, uint32_t i) {
             const uint64_t k = key_of(y, i);
             if (k < below && k > best) best = k;
@@ -282,14 +289,13 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
           const uint64_t* const k4 = sh.wave_key[got & 1];
           for (int i = 0; i < 4; ++i) best = k4[i] > best ? k4[i] : best;
           if (best == 0) break;
-          if (t == 0) sh.list[at ^ 1][got] = best;
+          if (t == 0) sh.out[got] = best;
           below = best;
         }
+        new_list(sh, got);
         nl = got;
-        at ^= 1;
         held = 0;
-        __syncthreads();
-        bar = nl == top ? above(key_value(sh.list[at][top - 1])) : -__builtin_inff();
+        bar = nl == top ? above(key_value(sh.keys[top - 1])) : -__builtin_inff();
       }
     }
     const float ms = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(tm))));
@@ -319,7 +325,23 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
     const bool small = fabsf(m) < 1e30f;
     const float c = m * kLog2e, delta = fmaf(m, kLog2e, -c);
     float pr = 0.0f, pd = 0.0f;
-    if (small && !fresh) {
+    bool out = fresh && lane == __builtin_ctzll(__ballot(tm == ms));  // the lane whose first copy of the largest stays out
+    if (small) {
+      if (fresh) {
+        int place = 8 * V;
+#pragma unroll
+        for (int v = V - 1; v >= 0; --v)
+#pragma unroll
+          for (int e = 7; e >= 0; --e) place = value(x, v, e) == ms ? 8 * v + e : place;
+        const int word = out ? place >> 1 : -1;
+        // so far below it that it adds nothing, and finite
+        const uint32_t low = f2bf(ms - 200.0f - 2.0f * fabsf(ms));
+        const uint32_t keep = place & 1 ? 0xffffu : 0xffff0000u, set = place & 1 ? low << 16 : low;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) x[v][w] = word == 4 * v + w ? (x[v][w] & keep) | set : x[v][w];
+      }
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
@@ -328,17 +350,22 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
           pr += p;
           pd = fmaf(p, z, pd);
         }
-    }
-    if (!small || fresh || __any(pd != pd)) {
-      // The largest, of which one copy stays out; excluded elements, where 0 times -inf is 0
-      // here; magnitudes that the product would pass.
-      bool out = fresh && lane == __builtin_ctzll(__ballot(tm == ms));
-      pr = pd = 0.0f;
+      if (__any(pd != pd)) {  // an excluded element: 0 times -inf is 0 here
+        pd = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float z = fmaxf(fmaf(value(x, v, e), kLog2e, -c), -1e30f);
+            pd = fmaf(__builtin_amdgcn_exp2f(z), z, pd);
+          }
+      }
+    } else {  // magnitudes that the product would pass
 #pragma unroll 1
       for (int h = 0; h < 8; ++h)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float y = half(x[v], h), z = small ? fmaf(y, kLog2e, -c) : (y - m) * kLog2e;
+          const float y = half(x[v], h), z = (y - m) * kLog2e;
           const bool skip = out && y == ms;
           out = out && !skip;
           const float p = skip ? 0.0f : __builtin_amdgcn_exp2f(z);
@@ -379,14 +406,14 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
   asm volatile("" : "+s"(late));
   const LogprobArgs b = *(const LogprobArgs*)late;
   if (b.ranges == 1) {
-    finish_row(b, row, largest, sr, sd, sh.list[at]);
+    finish_row(b, row, largest, sr, sd, sh.keys);
     return;
   }
   RangeStats* const stats = static_cast<RangeStats*>(b.scratch);
   uint64_t* const keys = reinterpret_cast<uint64_t*>(stats + (size_t)b.rows * b.ranges);
   const size_t block = (size_t)row * b.ranges + range;
   if (t == 0) stats[block] = RangeStats{largest, 0.0f, sr, sd};
-  if (t < top) keys[block * top + t] = t < nl ? sh.list[at][t] : 0;
+  if (t < top) keys[block * top + t] = sh.keys[t];
 }
 
 // Joins a row's ranges (at most 256): a thread each for the sums, then the top
@@ -412,6 +439,7 @@ __global__ __launch_bounds__(256) void k_logprob_join(LogprobArgs a) {
   if (lane == 0) sh.wave_m[wave] = m;
   heads[t] = mine;
   if (t == 0) sh.count[0] = 0;
+  if (t < kLogprobTop) sh.keys[t] = 0;
   __syncthreads();
   const float* const w = sh.wave_m;
   m = maximum(maximum(w[0], w[1]), maximum(w[2], w[3]));
@@ -446,15 +474,15 @@ __global__ __launch_bounds__(256) void k_logprob_join(LogprobArgs a) {
     for (int i = t; i < many * top; i += 256) {
       const int list = i / top;
       const uint64_t key = keys[(size_t)lists[list] * top + (i - list * top)];
-      if (key && key >= last) sh.cand[atomicAdd(&sh.count[0], 1)] = key;
+      if (key && key >= last) sh.keys[kLogprobTop + atomicAdd(&sh.count[0], 1)] = key;
     }
     __syncthreads();
-    rank_into(sh, 0, 0, sh.count[0], top);
+    rank_all(sh, 0, sh.count[0], top);
   } else {
     __syncthreads();
   }
   finish_row(a, row, m, sh.sum[0][0] + sh.sum[0][1] + sh.sum[0][2] + sh.sum[0][3],
-             sh.sum[1][0] + sh.sum[1][1] + sh.sum[1][2] + sh.sum[1][3], sh.list[1]);
+             sh.sum[1][0] + sh.sum[1][1] + sh.sum[1][2] + sh.sum[1][3], sh.keys);
 }
 
 // Ranges of a row and vectors of each.
