@@ -107,18 +107,19 @@ __device__ __forceinline__ void rank_all(Shared& sh, int nl, int n, int top) {
   new_list(sh, min(top, nl + n));
 }
 
-// A row's outputs from its largest logit, R, D and the list (called by the whole block).
-__device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, float m, double r, double d,
+// The row's logit of its token, a NaN where there is none; fetched early by thread 0.
+__device__ __forceinline__ float logit_of(const LogprobArgs& a, int row) {
+  if (threadIdx.x || !a.logprob) return __builtin_nanf("");
+  const uint32_t token = a.tokens[row];
+  return token < (uint32_t)a.vocab ? bf2f(a.logits[(int64_t)row * a.stride + token]) : __builtin_nanf("");
+}
+// A row's outputs from its token's and its largest logit, R, D and the list (called by the whole block).
+__device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, float x, float m, double r, double d,
                                            const uint64_t* list) {
   const bool finite = fabsf(m) < __builtin_inff();
   const double log_sum = finite ? (double)log1pf((float)r) : (double)__builtin_nanf("");
   if (threadIdx.x == 0) {
-    if (a.logprob) {
-      const uint32_t token = a.tokens[row];
-      float x = __builtin_nanf("");
-      if (token < (uint32_t)a.vocab) x = bf2f(a.logits[(int64_t)row * a.stride + token]);
-      a.logprob[row] = (float)(((double)x - (double)m) - log_sum);
-    }
+    if (a.logprob) a.logprob[row] = (float)(((double)x - (double)m) - log_sum);
     if (a.entropy) a.entropy[row] = (float)(log_sum - d * 0.69314718055994530942 / (1.0 + r));
     if (a.lse) a.lse[row] = finite ? (float)((double)m + log_sum) : m;
   }
@@ -378,6 +379,7 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
     r = fmaf(f, pr, r);
   }
   // the waves' sums to the block's largest, in 64 bits; the largest of the other waves join
+  const float token_logit = a.ranges == 1 ? logit_of(a, row) : 0.0f;
   if (lane == 0) sh.wave_m[wave] = m;
   __syncthreads();
   const float* const w = sh.wave_m;
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
   asm volatile("" : "+s"(late));
   const LogprobArgs b = *(const LogprobArgs*)late;
   if (b.ranges == 1) {
-    finish_row(b, row, largest, sr, sd, sh.keys);
+    finish_row(b, row, token_logit, largest, sr, sd, sh.keys);
     return;
   }
   RangeStats* const stats = static_cast<RangeStats*>(b.scratch);
@@ -427,6 +429,7 @@ __global__ __launch_bounds__(256) void k_logprob_join(LogprobArgs a) {
   const RangeStats* const stats = static_cast<const RangeStats*>(a.scratch) + (size_t)row * n;
   const uint64_t* const keys =
       reinterpret_cast<const uint64_t*>(static_cast<const RangeStats*>(a.scratch) + (size_t)a.rows * n) + (size_t)row * n * top;
+  const float token_logit = logit_of(a, row);
   RangeStats s = {-__builtin_inff(), 0.0f, 0.0, 0.0};
   uint64_t mine = 0;
   if (t < n) {
@@ -462,10 +465,12 @@ __global__ __launch_bounds__(256) void k_logprob_join(LogprobArgs a) {
     // a list's place among the first keys; only one range can be empty, so that no two are equal
     typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
     int place = 0;
-#pragma unroll 4
-    for (int i = 0; i < n; i += 2) {
-      const u64x2 two = *reinterpret_cast<const u64x2*>(&heads[i]);
-      place += (two[0] > mine) + (two[1] > mine);
+#pragma unroll 2
+    for (int i = 0; i < n; i += 8) {
+      const u64x2* const at = reinterpret_cast<const u64x2*>(&heads[i]);
+      const u64x2 k0 = at[0], k1 = at[1], k2 = at[2], k3 = at[3];
+      place += (k0[0] > mine) + (k0[1] > mine) + (k1[0] > mine) + (k1[1] > mine);
+      place += (k2[0] > mine) + (k2[1] > mine) + (k3[0] > mine) + (k3[1] > mine);
     }
     if (t < n && place < top) lists[place] = t;
     __syncthreads();
@@ -481,7 +486,7 @@ __global__ __launch_bounds__(256) void k_logprob_join(LogprobArgs a) {
   } else {
     __syncthreads();
   }
-  finish_row(a, row, m, sh.sum[0][0] + sh.sum[0][1] + sh.sum[0][2] + sh.sum[0][3],
+  finish_row(a, row, token_logit, m, sh.sum[0][0] + sh.sum[0][1] + sh.sum[0][2] + sh.sum[0][3],
              sh.sum[1][0] + sh.sum[1][1] + sh.sum[1][2] + sh.sum[1][3], sh.keys);
 }
 
