@@ -22,135 +22,219 @@ constexpr int kQk = 132;                 // floats between rows of q and of k
 constexpr int kPair = 65;                // floats between rows of the pair matrices
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(-x * kLog2e)); }
+__device__ __forceinline__ float finite_or_0(float x) { return fabsf(x) < INFINITY ? x : 0.0f; }
+__device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e)); }
+// x of the lane's node less low[i] times that of each node i before it, in order; the
+// 16 nodes lie in the 16 lanes of a row, from which DPP hands out one. 0 times
+// anything is 0 here.
+template <int I>
+__device__ __forceinline__ void substitute(const float (&low)[16], float& x) {
+  if constexpr (I < 16) {
+    const float xi = __builtin_amdgcn_update_dpp(0.0f, x, 0x150 + I, 0xf, 0xf, false);
+    float part;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(part) : "v"(low[I]), "v"(xi));
+    x = x - part;
+    substitute<I + 1>(low, x);
+  }
+}
 // Log gates count from here down as gates of 0.
 __device__ __forceinline__ double bounded(float log_g) { return log_g < -1e30f ? -1e30 : (double)log_g; }
 
-// Block = (16 value rows, head), four waves; 128 blocks.
-__global__ __launch_bounds__(256) void k_gdn_tree(TreeGdn a) {
-  __shared__ float qs[kTree][kQk], ks[kTree][kQk];
+// Block = (16 value rows, head), 16 waves; 128 blocks, each with the head's whole q
+// and k. Five parts, barriers between them:
+//   - the raw rows to LDS, all loads at once; paths and gates
+//   - convolution, SiLU and norms, a row a wave, four channels of q or k a lane
+//   - k S0^T, q S0^T, k k^T and q k^T in 16 x 16 tiles on 32-bit products
+//   - u by substitution: a 16-node block of the triangle in registers, four value
+//     columns a wave, what it gives to later blocks by products again
+//   - y = q S0^T + (pairs) u by products
+// A 0 for what is not on a node's path would carry a NaN or an infinity of u to it:
+// the substitution multiplies by the rule that 0 times anything is 0, the products
+// take 0 for such a u, and where there is one it is added to those behind it alone.
+__global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
+  __shared__ __attribute__((aligned(16))) float qs[kTree][kQk], ks[kTree][kQk];
   __shared__ __attribute__((aligned(16))) union {
     uint16_t staged[4 + kTree][kStagedRow];  // the ring's rows, then the nodes'
     struct {
       float low[kTree][kPair], pair[kTree][kPair];
     } m;
   } un;
-  __shared__ float b[kTree][kSlice + 1], y0[kTree][kSlice + 1];
+  __shared__ float y[kTree][kSlice + 1], u[kTree][kSlice + 1];  // u: v, then what is left of it
   __shared__ uint64_t path[kTree];
   __shared__ double total[kTree];
-  __shared__ float log_gate[kTree], beta[kTree];
-  __shared__ uint8_t tap[kTree][4];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n16 = lane & 15, g = lane >> 4;
+  __shared__ float decay[kTree], beta[kTree];
+  __shared__ uint32_t tap[kTree];
+  __shared__ int odd;
+  const int t = threadIdx.x, lane = t & 63, n16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int h = blockIdx.x >> 3, v0 = (blockIdx.x & 7) * kSlice;
+  const int own = t >> 4, column = t & 15;  // a thread's node and value column, where it has one
   const int rows = a.rows, tiles = (rows + 15) >> 4;
-  // the slice of the state: lane holds S[v0 + n16][16 s + 4 g .. + 3]
-  f32x4 st[8];
+  constexpr int kLoads = ((4 + kTree) * (kStaged / 8) + 1023) / 1024;
+  u32x4 raw[kLoads];
 #pragma unroll
-  for (int s = 0; s < 8; ++s)
-    st[s] = *reinterpret_cast<const f32x4*>(a.state + ((size_t)h * 128 + v0 + n16) * 128 + 16 * s + 4 * g);
-  for (int i = t; i < (4 + rows) * (kStaged / 8); i += 256) {
-    const int r = i / (kStaged / 8), c = i % (kStaged / 8);
+  for (int k = 0; k < kLoads; ++k) {
+    const int i = t + 1024 * k, r = i / (kStaged / 8), c = i % (kStaged / 8);
     const int channel = c < 16 ? h * 128 + 8 * c : c < 32 ? 2048 + h * 128 + 8 * (c - 16) : 4096 + h * 128 + v0 + 8 * (c - 32);
-    const uint16_t* const from = r < 4 ? a.ring + r * kConv : a.raw + (size_t)(r - 4) * kConv;
-    *reinterpret_cast<u32x4*>(&un.staged[r][8 * c]) = *reinterpret_cast<const u32x4*>(from + channel);
+    if (r < 4 + rows) raw[k] = *reinterpret_cast<const u32x4*>((r < 4 ? a.ring + r * kConv : a.raw + (size_t)(r - 4) * kConv) + channel);
   }
-  if (t < kTree) {
-    const uint64_t p = t < rows ? tree_path(a.paths[t], t) : 0;
-    path[t] = p;
-    // rows of the convolution's taps, oldest first: the ring's slot or the ancestor's row
+  // weights of the lane's channels 4 lane .. + 3 of q | k, and of the thread's channel of v
+  const int qk_channel = (lane >> 5) * 2048 + h * 128 + 4 * (lane & 31);
+  const u32x4* const wp = reinterpret_cast<const u32x4*>(a.conv_w + qk_channel * 4);
+  const u32x4 w01 = wp[0], w23 = wp[1];
+  const uint2 wv = *reinterpret_cast<const uint2*>(a.conv_w + (4096 + h * 128 + v0 + (t & 15)) * 4);
+  // the slice of the state, where the wave has a tile with it: lane holds S[v0 + n16][16 s + 4 g .. + 3]
+  f32x4 st[8];
+  if (wave < 2 * tiles) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      st[s] = *reinterpret_cast<const f32x4*>(a.state + ((size_t)h * 128 + v0 + n16) * 128 + 16 * s + 4 * g);
+  }
+  if (wave == 0) {
+    const uint64_t p = lane < rows ? tree_path(a.paths[lane], lane) : 0;
+    path[lane] = p;
+    // rows of the convolution's taps, oldest in the low byte: the ring's slot or the ancestor's row
     const int depth = __popcll(p) - 1;
     uint64_t up = p;
-    for (int k = 3; k >= 0; --k) {
-      const int back = 3 - k;
-      if (back <= depth) {
-        const int j = 63 - __clzll(up);
-        tap[t][k] = (uint8_t)(4 + j);
-        up &= ~(1ull << j);
-      } else {
-        tap[t][k] = (uint8_t)((a.position + depth - back) & 3);
-      }
+    uint32_t taps = 0;
+#pragma unroll
+    for (int back = 0; back < 4; ++back) {
+      const int j = up ? 63 - __clzll(up) : 0;
+      taps |= (uint32_t)(back <= depth ? 4 + j : (a.position + depth - back) & 3) << (24 - 8 * back);
+      up &= ~(1ull << j);
     }
+    tap[lane] = taps;
+    if (lane == 0) odd = 0;
+  }
+#pragma unroll
+  for (int k = 0; k < kLoads; ++k) {
+    const int i = t + 1024 * k, r = i / (kStaged / 8), c = i % (kStaged / 8);
+    if (r < 4 + rows) *reinterpret_cast<u32x4*>(&un.staged[r][8 * c]) = raw[k];
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const uint64_t p = path[lane];
     float log_g = 0.0f, be = 0.0f;
     if (p) {
-      const float x = bf2f(a.a_proj[t * 16 + h]) + bf2f(a.dt_bias[h]);
+      const float x = bf2f(a.a_proj[lane * 16 + h]) + bf2f(a.dt_bias[h]);
       log_g = -expf(a.a_log[h]) * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
-      be = sigmoid(bf2f(a.b_proj[t * 16 + h]));
+      be = sigmoid(bf2f(a.b_proj[lane * 16 + h]));
     }
-    log_gate[t] = log_g;
-    beta[t] = be;
-    if (v0 == 0 && t < rows) a.log_decay[t * 16 + h] = log_g;
+    beta[lane] = be;
+    if (v0 == 0 && lane < rows) a.log_decay[lane * 16 + h] = log_g;
+    // sums along the path: each round adds what twice as many ancestors sum to
+    double sum = p ? bounded(log_g) : 0.0;
+    const uint64_t above = p & ~(1ull << lane);
+    int up = above ? 63 - __clzll(above) : -1;
+#pragma unroll 1
+    for (int k = 1; k < kTree; k <<= 1) {
+      const double more = __shfl(sum, up & 63);
+      const int next = __shfl(up, up & 63);
+      if (up >= 0) {
+        sum += more;
+        up = next;
+      }
+    }
+    total[lane] = sum;
+    decay[lane] = expf((float)sum);
   }
-  __syncthreads();
-  if (t < kTree) {
-    double sum = 0.0;
-    for (uint64_t p = path[t]; p; p &= p - 1) sum += bounded(log_gate[__builtin_ctzll(p)]);
-    total[t] = sum;
-  }
-  // convolution and SiLU: a thread one channel of q or k, then 16 channels of v
-  auto conv = [&](int r, int c, uint2 w) {
-    float x = bf2f(un.staged[tap[r][0]][c]) * bf_lo(w.x);
-    x = fmaf(bf2f(un.staged[tap[r][1]][c]), bf_hi(w.x), x);
-    x = fmaf(bf2f(un.staged[tap[r][2]][c]), bf_lo(w.y), x);
-    x = fmaf(bf2f(un.staged[tap[r][3]][c]), bf_hi(w.y), x);
-    return x / (1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
-  };
   {
-    const int channel = (t >> 7) * 2048 + h * 128 + (t & 127);
-    const uint2 w = *reinterpret_cast<const uint2*>(a.conv_w + channel * 4);
-    float* const out = t < 128 ? &qs[0][t] : &ks[0][t - 128];
-    for (int r = 0; r < 16 * tiles; ++r) out[r * kQk] = path[r] ? conv(r, t, w) : 0.0f;
-    const uint2 wv = *reinterpret_cast<const uint2*>(a.conv_w + (4096 + h * 128 + v0 + (t & 15)) * 4);
-    for (int r = t >> 4; r < 16 * tiles; r += 16) b[r][t & 15] = path[r] ? conv(r, 256 + (t & 15), wv) : 0.0f;
+    float w[4][4];  // [channel][tap]
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t two = c < 2 ? w01[2 * c + (k >> 1)] : w23[2 * (c - 2) + (k >> 1)];
+        w[c][k] = k & 1 ? bf_hi(two) : bf_lo(two);
+      }
+    float* const out = lane < 32 ? &qs[0][4 * lane] : &ks[0][4 * (lane - 32)];
+#pragma unroll 1
+    for (int r = wave; r < 16 * tiles; r += 16) {
+      const uint32_t taps = __builtin_amdgcn_readfirstlane(tap[r]);
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint2 v = *reinterpret_cast<const uint2*>(&un.staged[taps >> (8 * k) & 255][4 * lane]);
+        x[0] = fmaf(bf_lo(v.x), w[0][k], x[0]);
+        x[1] = fmaf(bf_hi(v.x), w[1][k], x[1]);
+        x[2] = fmaf(bf_lo(v.y), w[2][k], x[2]);
+        x[3] = fmaf(bf_hi(v.y), w[3][k], x[3]);
+      }
+      float ss = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        x[c] = silu(x[c]);
+        ss = fmaf(x[c], x[c], ss);
+      }
+      ss = tree32(ss);
+      float inv = __builtin_amdgcn_rsqf(ss + 1e-6f);
+      if (__any(!(ss < INFINITY))) {
+        // the squares pass 32 bits' range before the row does: by 2^-72, beside which the eps is nothing
+        float big = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) big = fmaf(x[c] * 0x1p-72f, x[c] * 0x1p-72f, big);
+        big = tree32(big);
+        if (!(ss < INFINITY)) {
+          inv = __builtin_amdgcn_rsqf(big);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[c] *= 0x1p-72f;
+        }
+      }
+      if (lane < 32) inv *= 0.08838834764831845f;  // q by 128^-1/2 too
+      const bool used = path[r] != 0;
+      const float4 o = used ? make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      *reinterpret_cast<float4*>(out + r * kQk) = o;
+      if (v0 == 0 && lane >= 32 && r < rows)
+        *reinterpret_cast<float4*>(a.keys + ((size_t)r * 16 + h) * 128 + 4 * (lane - 32)) = o;
+    }
+    const int r = own, c = 256 + column;
+    if (r < 16 * tiles) {
+      const uint32_t taps = tap[r];
+      float x = bf2f(un.staged[taps & 255][c]) * bf_lo(wv.x);
+      x = fmaf(bf2f(un.staged[taps >> 8 & 255][c]), bf_hi(wv.x), x);
+      x = fmaf(bf2f(un.staged[taps >> 16 & 255][c]), bf_lo(wv.y), x);
+      x = fmaf(bf2f(un.staged[taps >> 24][c]), bf_hi(wv.y), x);
+      u[r][column] = path[r] ? silu(x) : 0.0f;
+    }
   }
   __syncthreads();
-  // norms: 16 lanes a row, its squares in 64 bits (they pass 32 bits' range before the row does)
-  for (int i = t >> 4; i < 32 * tiles; i += 16) {
-    float* const x = (i & 1 ? ks[i >> 1] : qs[i >> 1]) + 8 * n16;
-    double ss = 0.0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) ss = fma((double)x[k], (double)x[k], ss);
-#pragma unroll
-    for (int k = 1; k < 16; k <<= 1) ss += __shfl_xor(ss, k);
-    const double inv = (i & 1 ? 1.0 : 0.08838834764831844055) / sqrt(ss + 1e-6);  // q by 128^-1/2 too
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = (float)((double)x[k] * inv);
-  }
-  __syncthreads();
-  if (v0 == 0)
-    for (int i = t; i < rows * 32; i += 256)
-      *reinterpret_cast<float4*>(a.keys + ((size_t)(i >> 5) * 16 + h) * 128 + 4 * (i & 31)) =
-          *reinterpret_cast<const float4*>(&ks[i >> 5][4 * (i & 31)]);
   // 16 x 16 tiles of k S0^T and q S0^T, then of k k^T and q k^T on and below the diagonal
   const int lower = tiles * (tiles + 1) / 2, all = 2 * tiles + 2 * lower;
-  for (int i = wave; i < all; i += 4) {
+#pragma unroll 1
+  for (int i = wave; i < all; i += 16) {
     const bool with_state = i < 2 * tiles;
     const int k = with_state ? i : i - 2 * tiles;
     const bool of_q = with_state ? k >= tiles : k >= lower;
-    int ti = with_state ? k % tiles : k % lower, tj = 0;
+    int ti = k - (of_q ? (with_state ? tiles : lower) : 0), tj = 0;
     if (!with_state)
       for (tj = ti, ti = 0; tj > ti; ++ti) tj -= ti + 1;
     const float* const left = (of_q ? qs[0] : ks[0]) + (16 * ti + n16) * kQk + 4 * g;
     const float* const right = ks[16 * tj + n16] + 4 * g;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f}, acc2 = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
       const f32x4 x = *reinterpret_cast<const f32x4*>(left + 16 * s);
-      const f32x4 y = with_state ? st[s] : *reinterpret_cast<const f32x4*>(right + 16 * s);
+      const f32x4 z = with_state ? st[s] : *reinterpret_cast<const f32x4*>(right + 16 * s);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], acc, 0, 0, 0);
+      for (int e = 0; e < 4; e += 2) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], z[e], acc, 0, 0, 0);
+        acc2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e + 1], z[e + 1], acc2, 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = 16 * ti + 4 * g + e;
+      const float sum = acc[e] + acc2[e];
       if (with_state) {
-        const float decay = expf((float)total[r]);
-        if (of_q)
-          y0[r][n16] = path[r] ? decay * acc[e] : 0.0f;
-        else
-          b[r][n16] = path[r] ? beta[r] * (b[r][n16] - decay * acc[e]) : 0.0f;
+        const bool used = path[r] != 0;
+        if (of_q) {
+          y[r][n16] = used ? decay[r] * sum : 0.0f;
+        } else {
+          u[r][n16] = used ? beta[r] * (u[r][n16] - decay[r] * sum) : 0.0f;
+        }
       } else {
         const int c = 16 * tj + n16;
-        const bool on = path[r] >> c & 1;
-        const float x = on ? acc[e] * expf((float)(total[r] - total[c])) : 0.0f;
+        const float x = path[r] >> c & 1 ? sum * __builtin_amdgcn_exp2f((float)(total[r] - total[c]) * kLog2e) : 0.0f;
         if (of_q)
           un.m.pair[r][c] = x;
         else
@@ -159,40 +243,58 @@ __global__ __launch_bounds__(256) void k_gdn_tree(TreeGdn a) {
     }
   }
   __syncthreads();
-  // Substitution, a node a lane and four value rows a wave: node i's u is final
-  // once its ancestors' have left the sum; its descendants take it from theirs.
-  // What is not on a path is selected away, so a NaN stays on its own.
-  const uint64_t mine = path[lane];
-  float u[4], y[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    u[k] = lane < 16 * tiles ? b[lane][4 * wave + k] : 0.0f;
-    y[k] = lane < 16 * tiles ? y0[lane][4 * wave + k] : 0.0f;
-  }
   for (int c = 0; c < tiles; ++c) {
-    float low[16], pair[16];
+    if (wave < 4) {  // lane: node 16 c + n16, value column 4 wave + g
+      float x = u[16 * c + n16][4 * wave + g], low[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const bool in = lane >= 16 * c && lane < 16 * tiles;
-      low[e] = in ? un.m.low[lane][16 * c + e] : 0.0f;
-      pair[e] = in ? un.m.pair[lane][16 * c + e] : 0.0f;
+      for (int i = 0; i < 16; ++i) low[i] = un.m.low[16 * c + n16][16 * c + i];
+      substitute<0>(low, x);
+      u[16 * c + n16][4 * wave + g] = x;
+      if (__any(!(fabsf(x) < INFINITY)) && lane == 0) odd = 1;
     }
+    __syncthreads();
+    if (c + 1 < tiles) {
+      const int ti = c + 1 + wave;
+      if (ti < tiles) {
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int i = 16 * c + e;
-      const bool on = mine >> i & 1;
+        for (int s = 0; s < 4; ++s)
+          acc = __builtin_amdgcn_mfma_f32_16x16x4f32(un.m.low[16 * ti + n16][16 * c + 4 * s + g], finite_or_0(u[16 * c + 4 * s + g][n16]), acc, 0, 0, 0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float ui = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(u[k]), i));
-        u[k] = on && lane != i ? fmaf(-low[e], ui, u[k]) : u[k];
-        y[k] = on ? fmaf(pair[e], ui, y[k]) : y[k];
+        for (int e = 0; e < 4; ++e) u[16 * ti + 4 * g + e][n16] -= acc[e];
+      }
+      __syncthreads();
+      if (odd) {
+        if (own >= 16 * (c + 1) && own < 16 * tiles) {
+          float x = u[own][column];
+          for (int j = 16 * c; j < 16 * (c + 1); ++j)
+            if (path[own] >> j & 1 && !(fabsf(u[j][column]) < INFINITY)) x -= un.m.low[own][j] * u[j][column];
+          u[own][column] = x;
+        }
+        __syncthreads();
       }
     }
   }
-  if (lane < rows) {
-    const size_t at = ((size_t)lane * 16 + h) * 128 + v0 + 4 * wave;
-    *reinterpret_cast<float4*>(a.updates + at) = make_float4(u[0], u[1], u[2], u[3]);
-    *reinterpret_cast<uint2*>(a.y + at) = make_uint2(pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]));
+  if (wave < tiles) {
+    f32x4 acc;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = y[16 * wave + 4 * g + e][n16];
+    for (int c = 0; c <= wave; ++c)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(un.m.pair[16 * wave + n16][16 * c + 4 * s + g], finite_or_0(u[16 * c + 4 * s + g][n16]), acc, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[16 * wave + 4 * g + e][n16] = acc[e];
+  }
+  __syncthreads();
+  if (own < rows) {
+    const size_t at = ((size_t)own * 16 + h) * 128 + v0 + column;
+    float z = y[own][column];
+    if (odd)
+      for (int j = 0; j <= own; ++j)
+        if (path[own] >> j & 1 && !(fabsf(u[j][column]) < INFINITY)) z += un.m.pair[own][j] * u[j][column];
+    a.updates[at] = u[own][column];
+    a.y[at] = (uint16_t)f2bf(z);
   }
 }
 
@@ -237,7 +339,7 @@ __global__ __launch_bounds__(256) void k_gdn_tree_keep(TreeKeepGdn a) {
 }  // namespace
 
 hipError_t launch_tree_gdn(const TreeGdn& a, hipStream_t s) {
-  k_gdn_tree<<<128, 256, 0, s>>>(a);
+  k_gdn_tree<<<128, 1024, 0, s>>>(a);
   return hipGetLastError();
 }
 
