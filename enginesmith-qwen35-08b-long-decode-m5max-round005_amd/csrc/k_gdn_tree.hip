@@ -37,8 +37,9 @@ __device__ __forceinline__ void substitute(const float (&low)[16], float& x) {
     substitute<I + 1>(low, x);
   }
 }
-// Log gates count from here down as gates of 0.
-__device__ __forceinline__ double bounded(float log_g) { return log_g < -1e30f ? -1e30 : (double)log_g; }
+// A gate's log as it enters the sums: from -300 down it is a gate of 0 (32 bits end
+// at -104), and a bound keeps the differences of sums behind it exact.
+__device__ __forceinline__ double bounded(float log_g) { return log_g < -300.0f ? -300.0 : (double)log_g; }
 
 // Block = (16 value rows, head), 16 waves; 128 blocks, each with the head's whole q
 // and k. Five parts, barriers between them:
@@ -315,24 +316,41 @@ __global__ __launch_bounds__(256) void k_gdn_tree_keep(TreeKeepGdn a) {
     }
     return;
   }
+  __shared__ float weight[kTree], decay;
+  __shared__ int node[kTree];
   const int h = blockIdx.x >> 4, v = (blockIdx.x & 15) * 8 + (t >> 5), k = 4 * (t & 31);
   const size_t at = ((size_t)h * 128 + v) * 128 + k;
   f32x4 s = *reinterpret_cast<const f32x4*>(a.state + at);
-  double behind = 0.0;  // log of the gates behind the node at hand
+  const int many = __popcll(path);
+  if (t < kTree) {  // a node a lane: the gates behind it, and its place
+    double sum = path >> t & 1 ? bounded(a.log_decay[t * 16 + h]) : 0.0;
+#pragma unroll
+    for (int d = 1; d < kTree; d <<= 1) {
+      const double more = __shfl_down(sum, d);
+      sum += t + d < kTree ? more : 0.0;
+    }
+    const double behind = __shfl_down(sum, 1);
+    if (path >> t & 1) {
+      const int place = __popcll(path & ((1ull << t) - 1));
+      weight[place] = t + 1 < kTree ? expf((float)behind) : 1.0f;
+      node[place] = t;
+      if (place == 0) decay = expf((float)sum);
+    }
+  }
+  __syncthreads();
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint64_t p = path; p;) {
-    const int j = 63 - __clzll(p);
-    p &= ~(1ull << j);
-    const size_t row = (size_t)j * 16 + h;
-    const float w = expf((float)behind) * a.updates[row * 128 + v];
+#pragma unroll 8
+  for (int i = 0; i < many; ++i) {
+    const size_t row = (size_t)node[i] * 16 + h;
+    const float w = weight[i] * a.updates[row * 128 + v];
     const f32x4 key = *reinterpret_cast<const f32x4*>(a.keys + row * 128 + k);
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] = fmaf(w, key[e], sum[e]);
-    behind += bounded(a.log_decay[row]);
   }
-  const float decay = expf((float)behind);
+  if (many) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) s[e] = path ? fmaf(decay, s[e], sum[e]) : s[e];
+    for (int e = 0; e < 4; ++e) s[e] = fmaf(decay, s[e], sum[e]);
+  }
   *reinterpret_cast<f32x4*>(a.state_out + at) = s;
 }
 

@@ -161,9 +161,9 @@ def test_gdn(rows, kind, position):
     T.check_gdn(s, T.run_gdn(s))
 
 
-@pytest.mark.parametrize("a", [-30.0, 30.0, 1e4])
+@pytest.mark.parametrize("a", [-30.0, 30.0, 1e4, 1e38])
 def test_gdn_gates_at_their_ends(a):
-    """Gates of almost 1, of almost 0 and of 0."""
+    """Gates of almost 1, of almost 0 and of 0, with ordinary ones behind them."""
     s = T.gdn_case(30, 5, T.parents_of("random", 30, 1), seed=3)
     s["a_proj"][::2] = a
     s["b_proj"][1::3] = a
