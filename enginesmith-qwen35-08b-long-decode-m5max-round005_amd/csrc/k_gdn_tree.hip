@@ -63,7 +63,7 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
   __shared__ float y[kTree][kSlice + 1], u[kTree][kSlice + 1];  // u: v, then what is left of it
   __shared__ uint64_t path[kTree];
   __shared__ double total[kTree];
-  __shared__ float decay[kTree], beta[kTree];
+  __shared__ float beta[kTree];
   __shared__ uint32_t tap[kTree];
   __shared__ int odd;
   const int t = threadIdx.x, lane = t & 63, n16 = lane & 15, g = lane >> 4;
@@ -71,6 +71,15 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
   const int h = blockIdx.x >> 3, v0 = (blockIdx.x & 7) * kSlice;
   const int own = t >> 4, column = t & 15;  // a thread's node and value column, where it has one
   const int rows = a.rows, tiles = (rows + 15) >> 4;
+  // wave 0: paths and gates, a node a lane; their chain is the longest of this part
+  uint64_t my_word = 0;
+  float my_a = 0.0f, my_b = 0.0f, rate = 0.0f;
+  if (wave == 0 && lane < rows) {
+    my_word = a.paths[lane];
+    my_a = bf2f(a.a_proj[lane * 16 + h]) + bf2f(a.dt_bias[h]);
+    my_b = bf2f(a.b_proj[lane * 16 + h]);
+    rate = a.a_log[h];
+  }
   constexpr int kLoads = ((4 + kTree) * (kStaged / 8) + 1023) / 1024;
   u32x4 raw[kLoads];
 #pragma unroll
@@ -92,20 +101,38 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
       st[s] = *reinterpret_cast<const f32x4*>(a.state + ((size_t)h * 128 + v0 + n16) * 128 + 16 * s + 4 * g);
   }
   if (wave == 0) {
-    const uint64_t p = lane < rows ? tree_path(a.paths[lane], lane) : 0;
+    const uint64_t p = tree_path(my_word, lane);
     path[lane] = p;
     // rows of the convolution's taps, oldest in the low byte: the ring's slot or the ancestor's row
     const int depth = __popcll(p) - 1;
     uint64_t up = p;
     uint32_t taps = 0;
+    int parent = -1;
 #pragma unroll
     for (int back = 0; back < 4; ++back) {
       const int j = up ? 63 - __clzll(up) : 0;
+      if (back == 1 && up) parent = j;
       taps |= (uint32_t)(back <= depth ? 4 + j : (a.position + depth - back) & 3) << (24 - 8 * back);
       up &= ~(1ull << j);
     }
     tap[lane] = taps;
     if (lane == 0) odd = 0;
+    float log_g = 0.0f;
+    if (p) log_g = -expf(rate) * (fmaxf(my_a, 0.0f) + log1pf(expf(-fabsf(my_a))));
+    beta[lane] = p ? sigmoid(my_b) : 0.0f;
+    if (v0 == 0 && lane < rows) a.log_decay[lane * 16 + h] = log_g;
+    // sums along the path: each round adds what twice as many ancestors sum to
+    double sum = p ? bounded(log_g) : 0.0;
+#pragma unroll 1
+    while (__any(parent >= 0)) {
+      const double more = __shfl(sum, parent & 63);
+      const int next = __shfl(parent, parent & 63);
+      if (parent >= 0) {
+        sum += more;
+        parent = next;
+      }
+    }
+    total[lane] = sum;
   }
 #pragma unroll
   for (int k = 0; k < kLoads; ++k) {
@@ -113,32 +140,6 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
     if (r < 4 + rows) *reinterpret_cast<u32x4*>(&un.staged[r][8 * c]) = raw[k];
   }
   __syncthreads();
-  if (wave == 0) {
-    const uint64_t p = path[lane];
-    float log_g = 0.0f, be = 0.0f;
-    if (p) {
-      const float x = bf2f(a.a_proj[lane * 16 + h]) + bf2f(a.dt_bias[h]);
-      log_g = -expf(a.a_log[h]) * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
-      be = sigmoid(bf2f(a.b_proj[lane * 16 + h]));
-    }
-    beta[lane] = be;
-    if (v0 == 0 && lane < rows) a.log_decay[lane * 16 + h] = log_g;
-    // sums along the path: each round adds what twice as many ancestors sum to
-    double sum = p ? bounded(log_g) : 0.0;
-    const uint64_t above = p & ~(1ull << lane);
-    int up = above ? 63 - __clzll(above) : -1;
-#pragma unroll 1
-    for (int k = 1; k < kTree; k <<= 1) {
-      const double more = __shfl(sum, up & 63);
-      const int next = __shfl(up, up & 63);
-      if (up >= 0) {
-        sum += more;
-        up = next;
-      }
-    }
-    total[lane] = sum;
-    decay[lane] = expf((float)sum);
-  }
   {
     float w[4][4];  // [channel][tap]
 #pragma unroll
@@ -211,35 +212,53 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
       for (tj = ti, ti = 0; tj > ti; ++ti) tj -= ti + 1;
     const float* const left = (of_q ? qs[0] : ks[0]) + (16 * ti + n16) * kQk + 4 * g;
     const float* const right = ks[16 * tj + n16] + 4 * g;
+    f32x4 x[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[s] = *reinterpret_cast<const f32x4*>(left + 16 * s);
+    if (!with_state) {  // a wave's tile with the state is its first
+#pragma unroll
+      for (int s = 0; s < 8; ++s) st[s] = *reinterpret_cast<const f32x4*>(right + 16 * s);
+    }
+    // what the sums meet, read while the products run
+    uint64_t on[4];
+    float by[4], was[4];
+    double sums[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = 16 * ti + 4 * g + e;
+      on[e] = path[r];
+      by[e] = beta[r];
+      sums[e] = total[r];
+      was[e] = u[r][n16];
+    }
+    const double from = with_state ? 0.0 : total[16 * tj + n16];
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f}, acc2 = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(left + 16 * s);
-      const f32x4 z = with_state ? st[s] : *reinterpret_cast<const f32x4*>(right + 16 * s);
+    for (int s = 0; s < 8; ++s)
 #pragma unroll
       for (int e = 0; e < 4; e += 2) {
-        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], z[e], acc, 0, 0, 0);
-        acc2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e + 1], z[e + 1], acc2, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s][e], st[s][e], acc, 0, 0, 0);
+        acc2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s][e + 1], st[s][e + 1], acc2, 0, 0, 0);
       }
-    }
+    float scale[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) scale[e] = __builtin_amdgcn_exp2f((float)(sums[e] - from) * kLog2e);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = 16 * ti + 4 * g + e;
       const float sum = acc[e] + acc2[e];
       if (with_state) {
-        const bool used = path[r] != 0;
-        if (of_q) {
-          y[r][n16] = used ? decay[r] * sum : 0.0f;
-        } else {
-          u[r][n16] = used ? beta[r] * (u[r][n16] - decay[r] * sum) : 0.0f;
-        }
+        if (of_q)
+          y[r][n16] = on[e] ? scale[e] * sum : 0.0f;
+        else
+          u[r][n16] = on[e] ? by[e] * (was[e] - scale[e] * sum) : 0.0f;
       } else {
         const int c = 16 * tj + n16;
-        const float x = path[r] >> c & 1 ? sum * __builtin_amdgcn_exp2f((float)(total[r] - total[c]) * kLog2e) : 0.0f;
+        const float x = on[e] >> c & 1 ? sum * scale[e] : 0.0f;
         if (of_q)
           un.m.pair[r][c] = x;
         else
-          un.m.low[r][c] = c < r ? beta[r] * x : 0.0f;
+          un.m.low[r][c] = c < r ? by[e] * x : 0.0f;
       }
     }
   }
