@@ -57,6 +57,12 @@ template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+// One instruction; fmaxf puts one before each operand that quiets a NaN.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 // Barrier for what the waves have waited for themselves (their DMA, counted) and LDS.
 __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -115,18 +121,19 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
     kchunk[i] = (uint32_t)(((lane & 31) ^ (r & 15)) * 16);
     vchunk[i] = (uint32_t)(((lane & 31) ^ 4 * (r & 3)) * 16);
   }
+  const uint32_t second = (uint32_t)(lane >> 5) * stride;
   auto issue = [&](int kb, int st) {
-    const uint32_t stage = kv_base + (uint32_t)(2 * kStage) * st;
+    const uint32_t to = kv_base + (uint32_t)(2 * kStage) * st + (uint32_t)(4 * wave) * (2 * kRow);
+    uint32_t at = (uint32_t)(kb * kKeys + 4 * wave) * stride, more[2] = {second, second + 2 * stride};
+    if (kb * kKeys + kKeys > n) {
+      at = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) more[i] = (uint32_t)min(kb * kKeys + 4 * wave + 2 * i + (lane >> 5), n - 1) * stride;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = 4 * wave + 2 * i;
-      uint32_t at = (uint32_t)(kb * kKeys + r) * stride, more = (uint32_t)(lane >> 5) * stride;
-      if (kb * kKeys + kKeys > n) {
-        at = 0;
-        more = (uint32_t)min(kb * kKeys + r + (lane >> 5), n - 1) * stride;
-      }
-      dma16_past_caches(ksrc, stage + 2 * r * kRow, kchunk[i] + more, at);
-      dma16_past_caches(vsrc, stage + 2 * (kKeys + r) * kRow, vchunk[i] + more, at);
+      dma16_past_caches(ksrc, to + 4 * i * kRow, kchunk[i] + more[i], at);
+      dma16_past_caches(vsrc, to + 2 * (kKeys + 2 * i) * kRow, vchunk[i] + more[i], at);
     }
   };
   // Small inputs; the queries, two an instruction, into the stages after the first two; the first two stages.
@@ -288,12 +295,14 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   auto scores = [&](int st, f32x4 (&sc)[2]) {
     const char* const stage = reinterpret_cast<const char*>(kv[st]);
     sc[0] = sc[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    bf16x8 kf[8];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const bf16x8 kf = *reinterpret_cast<const bf16x8*>(stage + k_at[s & 3] + 256 * (s >> 2));
+    for (int s = 0; s < 8; ++s) kf[s] = *reinterpret_cast<const bf16x8*>(stage + k_at[s & 3] + 256 * (s >> 2));
+    __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product
 #pragma unroll
-      for (int u = 0; u < 2; ++u) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[u][s], sc[u], 0, 0, 0);
-    }
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[s], qf[u][s], sc[u], 0, 0, 0);
   };
   stage_barrier();  // every wave has its queries
   if (steps > 2) issue(first + 2 * every, 2);
@@ -330,19 +339,19 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = key0 + e < n ? x[e] : -INFINITY;
     }
-    float mloc = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) mloc = fmaxf(mloc, x[e]);
-    const float2 m2 = rows_xor32(mloc);
+    // a NaN may be passed over: its exponential is one too
+    const float2 m2 = rows_xor32(max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]), x[5]));
     // the reference moves only where the maximum passes it by more than 8
-    const float mblk = fmaxf(m2.x, m2.y) * c, mnew = mblk > ref + 8.0f ? mblk : ref;
+    const float mblk = max3(m2.x, m2.y, m2.y) * c, mnew = mblk > ref + 8.0f ? mblk : ref;
     const float factor = __builtin_amdgcn_exp2f(ref - mnew);
     u32x4 pb;
     float psum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      pb[e] = pack_bf2(__builtin_amdgcn_exp2f(fmaf(x[2 * e], c, -mnew)), __builtin_amdgcn_exp2f(fmaf(x[2 * e + 1], c, -mnew)));
-      psum += bf_lo(pb[e]) + bf_hi(pb[e]);
+      const uint32_t two =
+          pack_bf2(__builtin_amdgcn_exp2f(fmaf(x[2 * e], c, -mnew)), __builtin_amdgcn_exp2f(fmaf(x[2 * e + 1], c, -mnew)));
+      psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), psum, false);
+      pb[e] = two;
     }
     const float2 s2 = rows_xor32(psum);
     sum = sum * factor + (s2.x + s2.y);
