@@ -169,83 +169,70 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
   if (t < 2) odd_rows[t] = 0;
   if (tree) wait_vmcnt<0>();
   stage_barrier();
-  // A head is made by four lanes, with dims 32 s + 8 g .. + 7, 16 heads a wave: the
-  // queries, then the nodes' keys where this is their block. (With 16 lanes a head one
-  // round of four heads takes 2200 cycles, this one of 16 3300.)
-  const int qunits = (made + 15) >> 4, units = qunits + (tree ? (a.rows + 15) >> 4 : 0);
+  // A head is made by eight lanes, each with chunks c, c + 8, c + 16 and c + 24 of eight
+  // dims, eight heads a wave: the queries, then the nodes' keys where this is their
+  // block. (Four lanes a head take 3600 cycles for up to 128 heads, 16 lanes 2200 for 32.)
+  const int heads = made + (tree ? a.rows : 0), ci = lane & 7;
 #pragma unroll 1
-  for (int i = wave; i < units; i += 8) {
-    const bool key = i >= qunits;
-    const int r = 16 * (key ? i - qunits : i) + qi;  // of the nodes or of the tile's queries
+  for (int i = 8 * wave + (lane >> 3); i < heads; i += 64) {
+    const bool key = i >= made;
+    const int r = key ? i - made : i;  // of the nodes or of the tile's queries
     char* const head = reinterpret_cast<char*>(key ? &kv[r >> 5][(r & 31) * kRow] : &kv[2][r * kRow]);
-    const int node = key ? min(r, a.rows - 1) : node_of(min(tile * kTileQ + r, a.queries - 1));
+    const int node = key ? r : node_of(tile * kTileQ + r);
     const uint64_t path = tree_path(word[node], node);
-    u32x4 x[8];
+    const uint16_t* const by = gain[key] + 8 * ci;
+    u32x4 x[4], gv[4];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) x[s] = *reinterpret_cast<const u32x4*>(head + ((4 * s + g) ^ qi) * 16);
-    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < 4; ++s) {
+      x[s] = *reinterpret_cast<const u32x4*>(head + ((ci + 8 * s) ^ (r & 15)) * 16);
+      gv[s] = *reinterpret_cast<const u32x4*>(by + 64 * s);
+    }
+    const float4* const cs = reinterpret_cast<const float4*>(&turn[path ? __popcll(path) - 1 : 0][8 * (ci & 3)]);
+    float y[4][8], part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) part[e] = fmaf(bf_hi(x[s][e]), bf_hi(x[s][e]), fmaf(bf_lo(x[s][e]), bf_lo(x[s][e]), part[e]));
-    float2 p = rows_xor16((part[0] + part[1]) + (part[2] + part[3]));
-    p = rows_xor32(p.x + p.y);
-    const float ss = p.x + p.y;
+      for (int e = 0; e < 8; ++e) {
+        y[s][e] = e & 1 ? bf_hi(x[s][e >> 1]) : bf_lo(x[s][e >> 1]);
+        part[s] = fmaf(y[s][e], y[s][e], part[s]);
+      }
+    const float ss = tree8((part[0] + part[1]) + (part[2] + part[3]));
     float inv = __builtin_amdgcn_rsqf(ss * (1.0f / 256.0f) + 1e-6f);
-    if (__any(!(ss < INFINITY))) {
+    if (!(ss < INFINITY)) {
       // The squares pass 32 bits' range before the head does: such a head by 2^-72, beside
       // which the eps is nothing. An infinity or a NaN stays one.
       float big = 0.0f;
 #pragma unroll
-      for (int s = 0; s < 8; ++s)
+      for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float lo = bf_lo(x[s][e]) * 0x1p-72f, hi = bf_hi(x[s][e]) * 0x1p-72f;
-          big = fmaf(hi, hi, fmaf(lo, lo, big));
-          if (!(ss < INFINITY)) x[s][e] = pack_bf2(lo, hi);
+        for (int e = 0; e < 8; ++e) {
+          y[s][e] *= 0x1p-72f;
+          big = fmaf(y[s][e], y[s][e], big);
         }
-      p = rows_xor16(big);
-      p = rows_xor32(p.x + p.y);
-      if (!(ss < INFINITY)) inv = __builtin_amdgcn_rsqf((p.x + p.y) * (1.0f / 256.0f));
+      inv = __builtin_amdgcn_rsqf(tree8(big) * (1.0f / 256.0f));
     }
-    const uint16_t* const by = gain[key] + 8 * g;
-    float lo[8];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const u32x4 gv = *reinterpret_cast<const u32x4*>(by + 32 * s);
-      float y[8];
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[2 * e] = bf_lo(x[s][e]) * inv * bf_lo(gv[e]);
-        y[2 * e + 1] = bf_hi(x[s][e]) * inv * bf_hi(gv[e]);
-      }
-      if (s == 0) {
+      for (int e = 0; e < 8; ++e) y[s][e] = y[s][e] * inv * (e & 1 ? bf_hi(gv[s][e >> 1]) : bf_lo(gv[s][e >> 1]));
+    // the rotated 64 are chunks 0 .. 7: dims d and d + 32 lie four lanes apart
 #pragma unroll
-        for (int e = 0; e < 8; ++e) lo[e] = y[e];
-        continue;
-      }
-      if (s == 1) {  // dims d and d + 32 of the rotated 64
-        const float4* const cs = reinterpret_cast<const float4*>(&turn[path ? __popcll(path) - 1 : 0][8 * g]);
-        u32x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float4 c2 = cs[e];
-          w[e] = pack_bf2(fmaf(lo[2 * e], c2.x, -(y[2 * e] * c2.y)), fmaf(lo[2 * e + 1], c2.z, -(y[2 * e + 1] * c2.w)));
-          y[2 * e] = fmaf(lo[2 * e], c2.y, y[2 * e] * c2.x);
-          y[2 * e + 1] = fmaf(lo[2 * e + 1], c2.w, y[2 * e + 1] * c2.z);
-        }
-        x[0] = w;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[s][e] = pack_bf2(y[2 * e], y[2 * e + 1]);
+    for (int e = 0; e < 8; ++e) {
+      const float4 c2 = cs[e >> 1];
+      const float co = e & 1 ? c2.z : c2.x, si = e & 1 ? c2.w : c2.y;
+      const float above = __builtin_amdgcn_update_dpp(0.0f, y[0][e], 0x12c, 0xf, 0xf, false);  // of lane + 4 (row_ror:12)
+      const float below = __builtin_amdgcn_update_dpp(0.0f, y[0][e], 0x124, 0xf, 0xf, false);  // of lane - 4 (row_ror:4)
+      y[0][e] = ci < 4 ? fmaf(y[0][e], co, -(above * si)) : fmaf(below, si, y[0][e] * co);
     }
-    uint16_t* const to = a.k_tree + ((size_t)node * a.kv_heads + kvh) * 256 + 8 * g;
-    const bool out = key && !path, store = key && tile == 0 && r < a.rows;
+    uint16_t* const to = a.k_tree + ((size_t)node * a.kv_heads + kvh) * 256 + 8 * ci;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      if (out) x[s] = u32x4{0, 0, 0, 0};  // a node left out has no key
-      *reinterpret_cast<u32x4*>(head + ((4 * s + g) ^ qi) * 16) = x[s];
-      if (store) *reinterpret_cast<u32x4*>(to + 32 * s) = x[s];
+    for (int s = 0; s < 4; ++s) {
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = pack_bf2(y[s][2 * e], y[s][2 * e + 1]);
+      if (key && !path) w = u32x4{0, 0, 0, 0};  // a node left out has no key
+      *reinterpret_cast<u32x4*>(head + ((ci + 8 * s) ^ (r & 15)) * 16) = w;
+      if (key && tile == 0) *reinterpret_cast<u32x4*>(to + 64 * s) = w;
     }
   }
   if (tree) {
@@ -435,7 +422,7 @@ __global__ __launch_bounds__(512, 1) void k_tree_attn(TreeAttn a) {
 __global__ __launch_bounds__(1024) void k_tree_join(TreeAttn a) {
   __shared__ float4 part_o[16][64];
   __shared__ float2 part_s[16][32];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int j = blockIdx.x & 31, tile = (blockIdx.x >> 5) % a.parts, kvh = (blockIdx.x >> 5) / a.parts;
   const int q = min(32 * tile + (lane & 31), a.queries - 1), row = a.group == 1 ? q : (int)__umulhi((uint32_t)q, a.group_inv);
   const size_t at = (size_t)row * a.q_heads + kvh * a.group + q - row * a.group;
@@ -448,28 +435,58 @@ __global__ __launch_bounds__(1024) void k_tree_join(TreeAttn a) {
   }
   float ref = -3.0e38f, sum = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto join = [&](float2 s1, float4 o1) {
-    const float top = fmaxf(ref, s1.x), f0 = __builtin_amdgcn_exp2f(ref - top), f1 = __builtin_amdgcn_exp2f(s1.x - top);
-    o.x = fmaf(o1.x, f1, o.x * f0);
-    o.y = fmaf(o1.y, f1, o.y * f0);
-    o.z = fmaf(o1.z, f1, o.z * f0);
-    o.w = fmaf(o1.w, f1, o.w * f0);
-    sum = fmaf(s1.y, f1, sum * f0);
+  // N states and the one so far, to the largest of their references
+  auto join = [&](auto& s1, auto& o1) {
+    constexpr int N = sizeof(s1) / sizeof(s1[0]);
+    float top = ref;
+#pragma unroll
+    for (int k = 0; k < N; ++k) top = fmaxf(top, s1[k].x);
+    const float f = __builtin_amdgcn_exp2f(ref - top);
+    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    sum *= f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float fk = __builtin_amdgcn_exp2f(s1[k].x - top);
+      o.x = fmaf(o1[k].x, fk, o.x);
+      o.y = fmaf(o1[k].y, fk, o.y);
+      o.z = fmaf(o1[k].z, fk, o.z);
+      o.w = fmaf(o1[k].w, fk, o.w);
+      sum = fmaf(s1[k].y, fk, sum);
+    }
     ref = top;
   };
-  if (32 * tile + (lane & 31) < a.queries) {
-#pragma unroll 8
-    for (int i = wave; i <= a.ranges; i += 16) {
-      const float* const part = a.part + ((size_t)(i * a.kv_heads + kvh) * a.parts + tile) * kPart;
-      join(*reinterpret_cast<const float2*>(part + 8192 + 2 * (lane & 31)),
-           *reinterpret_cast<const float4*>(part + (64 * j + lane) * 4));
+  const bool mine = 32 * tile + (lane & 31) < a.queries;
+#pragma unroll 1
+  for (int i0 = wave; i0 <= a.ranges; i0 += 64) {  // four ranges' loads at once: one after the other took 0.9 us each
+    float4 o1[4];
+    float2 s1[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s1[k] = make_float2(-3.0e38f, 0.0f);
+      o1[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i0 + 16 * k <= a.ranges && mine) {
+        const float* const part = a.part + ((size_t)((i0 + 16 * k) * a.kv_heads + kvh) * a.parts + tile) * kPart;
+        s1[k] = *reinterpret_cast<const float2*>(part + 8192 + 2 * (lane & 31));
+        o1[k] = *reinterpret_cast<const float4*>(part + (64 * j + lane) * 4);
+      }
     }
+    join(s1, o1);
   }
   part_o[wave][lane] = o;
   if (lane < 32) part_s[wave][lane] = make_float2(ref, sum);
   __syncthreads();
-  if (wave || 32 * tile + (lane & 31) >= a.queries) return;
-  for (int w = 1; w < 16 && w <= a.ranges; ++w) join(part_s[w][lane & 31], part_o[w][lane]);
+  if (wave || !mine) return;
+#pragma unroll
+  for (int w = 1; w < 16; w += 5) {
+    float4 o1[5];
+    float2 s1[5];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+      s1[k] = part_s[w + k][lane & 31];
+      o1[k] = part_o[w + k][lane];
+    }
+    join(s1, o1);
+  }
   auto gated = [&](float x, float z) { return x / sum / (1.0f + __builtin_amdgcn_exp2f(-z * 1.44269504088896341f)); };
   uint2 out = make_uint2(pack_bf2(gated(o.x, bf_lo(gate.x)), gated(o.y, bf_hi(gate.x))),
                          pack_bf2(gated(o.z, bf_lo(gate.y)), gated(o.w, bf_hi(gate.y))));
@@ -510,7 +527,12 @@ hipError_t launch_tree_attn(TreeAttn a, hipStream_t s) {
   a.tiles = (a.queries + kTileQ - 1) / kTileQ;
   a.parts = (a.queries + 31) / 32;
   const int blocks = (a.position + kKeys - 1) / kKeys;
-  a.ranges = std::min(most_ranges(a.kv_heads, a.tiles), (blocks + 1) / 2);
+  // At least one block of 32 keys a range, three where a tile is 64 queries or more: a range's
+  // partial results are 33 KB for each 32 of them. With 1, 2 and 3 blocks (8 query heads, 2 KV
+  // heads): 1 node at 1020 10.3, 10.9 and 11.6 us, 8 nodes at 1020 11.2, 11.4 and 12.0, 32
+  // nodes at 4000 23.3, 19.7 and 19.0, 64 at 4000 26.0, 26.0 and 23.8.
+  const int least = a.queries < 64 ? 1 : 3;
+  a.ranges = std::min(most_ranges(a.kv_heads, a.tiles), (blocks + least - 1) / least);
   a.part = static_cast<float*>(a.scratch);
   a.per = a.ranges ? blocks / a.ranges : 0;
   a.more = a.ranges ? blocks % a.ranges : 0;
