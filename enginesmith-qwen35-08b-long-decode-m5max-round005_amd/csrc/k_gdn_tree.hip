@@ -65,7 +65,7 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
   __shared__ double total[kTree];
   __shared__ float beta[kTree];
   __shared__ uint32_t tap[kTree];
-  __shared__ int odd;
+  __shared__ int odd[kTree / 16];  // by block of nodes: whether its u holds an infinity or a NaN
   const int t = threadIdx.x, lane = t & 63, n16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int h = blockIdx.x >> 3, v0 = (blockIdx.x & 7) * kSlice;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
       up &= ~(1ull << j);
     }
     tap[lane] = taps;
-    if (lane == 0) odd = 0;
+    if (lane < kTree / 16) odd[lane] = 0;
     float log_g = 0.0f;
     if (p) log_g = -expf(rate) * (fmaxf(my_a, 0.0f) + log1pf(expf(-fabsf(my_a))));
     beta[lane] = p ? sigmoid(my_b) : 0.0f;
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
       for (int i = 0; i < 16; ++i) low[i] = un.m.low[16 * c + n16][16 * c + i];
       substitute<0>(low, x);
       u[16 * c + n16][4 * wave + g] = x;
-      if (__any(!(fabsf(x) < INFINITY)) && lane == 0) odd = 1;
+      if (__any(!(fabsf(x) < INFINITY)) && lane == 0) odd[c] = 1;
     }
     __syncthreads();
     if (c + 1 < tiles) {
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
         for (int e = 0; e < 4; ++e) u[16 * ti + 4 * g + e][n16] -= acc[e];
       }
       __syncthreads();
-      if (odd) {
+      if (odd[c]) {
         if (own >= 16 * (c + 1) && own < 16 * tiles) {
           float x = u[own][column];
           for (int j = 16 * c; j < 16 * (c + 1); ++j)
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
   if (own < rows) {
     const size_t at = ((size_t)own * 16 + h) * 128 + v0 + column;
     float z = y[own][column];
-    if (odd)
+    if (odd[0] | odd[1] | odd[2] | odd[3])
       for (int j = 0; j <= own; ++j)
         if (path[own] >> j & 1 && !(fabsf(u[j][column]) < INFINITY)) z += un.m.pair[own][j] * u[j][column];
     a.updates[at] = u[own][column];

@@ -197,6 +197,24 @@ def test_gdn_keeps_a_nodes_nan_to_its_descendants(bad):
         assert torch.isnan(got[0].view(rows, 16, 128)[node, 1]).any()
 
 
+def test_gdn_of_nan_in_every_block_of_nodes():
+    """A block of 16 nodes with a NaN among blocks without: what is not below it stays, call after call."""
+    rows, parents = 64, T.parents_of("random", 64, 6)
+    s = T.gdn_case(rows, 9, parents, seed=8)
+    clean = T.run_gdn(s)
+    leaves = [i for i in range(rows) if sum(i in p for p in s["nodes"]) == 1]
+    for blocks in ((1,), (2,), (0, 2), (1, 2), (0, 1, 2, 3)):
+        bad = [next(i for i in leaves if i // 16 == b) for b in blocks]
+        t = dict(s, raw=s["raw"].clone())
+        t["raw"][bad] = torch.nan
+        fine = torch.ones(rows, dtype=torch.bool, device="cuda")
+        fine[bad] = False
+        for _ in range(20):
+            for a, b in zip(T.run_gdn(t), clean):
+                assert torch.equal(a[fine], b[fine]), blocks
+                assert a.dtype == torch.float32 and a.shape[1:] == (16,) or torch.isnan(a[bad]).all(), blocks
+
+
 def test_gdn_nodes_left_out():
     rows, parents = 30, T.parents_of("holes", 30, 8)
     s = T.gdn_case(rows, 6, parents, seed=9)
