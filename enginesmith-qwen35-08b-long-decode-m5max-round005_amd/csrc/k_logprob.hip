@@ -70,7 +70,7 @@ __device__ __forceinline__ double wave_sum(double v) {
 
 struct Shared {
   // the top list in order, zeros behind it; from kLogprobTop on the buffer of keys not yet ranked
-  __attribute__((aligned(16))) uint64_t keys[kLogprobTop + kMost + 8];
+  __attribute__((aligned(16))) uint64_t keys[kLogprobTop + kMost + 32];
   uint64_t out[kLogprobTop];
   __attribute__((aligned(16))) float group_max[64];
   uint64_t wave_key[2][4];
@@ -85,23 +85,32 @@ __device__ __forceinline__ void new_list(Shared& sh, int n) {
   if (threadIdx.x < kLogprobTop) sh.keys[threadIdx.x] = (int)threadIdx.x < n ? sh.out[threadIdx.x] : 0;
   __syncthreads();
 }
+// How many of the keys at `keys` pass `mine`: n of them, zeros behind up to a multiple
+// of 8 U; 8 U are read at once.
+template <int U>
+__device__ __forceinline__ int larger(const uint64_t* keys, int n, uint64_t mine) {
+  typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+  int count = 0;
+#pragma unroll 1
+  for (int j = 0; j < n; j += 8 * U) {
+    u64x2 k[4 * U];
+#pragma unroll
+    for (int i = 0; i < 4 * U; ++i) k[i] = reinterpret_cast<const u64x2*>(&keys[j])[i];
+#pragma unroll
+    for (int i = 0; i < 4 * U; ++i) count += (k[i][0] > mine) + (k[i][1] > mine);
+  }
+  return count;
+}
 // Joins the n keys of the buffer to the nl of the list. A key's place is the
 // number of larger ones, and no two are equal.
+template <int U>
 __device__ __forceinline__ void rank_all(Shared& sh, int nl, int n, int top) {
-  typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
-  if (threadIdx.x < 8) sh.keys[kLogprobTop + n + threadIdx.x] = 0;
+  if (threadIdx.x < 8 * U) sh.keys[kLogprobTop + n + threadIdx.x] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < kLogprobTop + n; i += 256) {
     const uint64_t mine = sh.keys[i];
     if (mine == 0) continue;
-    int place = 0;
-#pragma unroll 1
-    for (int j = 0; j < kLogprobTop + n; j += 8) {
-      const u64x2* const at = reinterpret_cast<const u64x2*>(&sh.keys[j]);
-      const u64x2 k0 = at[0], k1 = at[1], k2 = at[2], k3 = at[3];
-      place += (k0[0] > mine) + (k0[1] > mine) + (k1[0] > mine) + (k1[1] > mine);
-      place += (k2[0] > mine) + (k2[1] > mine) + (k3[0] > mine) + (k3[1] > mine);
-    }
+    const int place = larger<U>(sh.keys, kLogprobTop + n, mine);
     if (place < top) sh.out[place] = mine;
   }
   new_list(sh, min(top, nl + n));
@@ -265,7 +274,7 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
         slow = !full && (over || n < min(top, there));  // too many equals, or fewer than there are: the others are NaN
         held = n;
         if (!slow && (!full || over || n >= kFlush + top || s + 1 == last)) {
-          rank_all(sh, nl, n, top);
+          rank_all<1>(sh, nl, n, top);
           nl = min(top, nl + n);
           bar = nl == top ? above(key_value(sh.keys[top - 1])) : -__builtin_inff();
           held = 0;
@@ -418,30 +427,33 @@ __global__ __launch_bounds__(256, V == 4 ? 4 : 6) void k_logprob(LogprobArgs a) 
   if (t < top) keys[block * top + t] = sh.keys[t];
 }
 
-// Joins a row's ranges (at most 256): a thread each for the sums, then the top
-// list from the ranges' lists: those whose first key is among the `top` largest
-// first keys hold all of it.
+// Joins a row's ranges (at most 256): a thread each for the sums, then the top list
+// from the ranges' lists. Of the q lists whose j-th key is largest, each has j keys
+// that reach the smallest of those, so with q j >= top all of the list reaches it: few others do.
 __global__ __launch_bounds__(256) void k_logprob_join(LogprobArgs a) {
   __shared__ Shared sh;
   __shared__ __attribute__((aligned(16))) uint64_t heads[256];
-  __shared__ int lists[kLogprobTop];
+  __shared__ uint64_t least;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.x, top = a.top, n = a.ranges;
   const RangeStats* const stats = static_cast<const RangeStats*>(a.scratch) + (size_t)row * n;
   const uint64_t* const keys =
       reinterpret_cast<const uint64_t*>(static_cast<const RangeStats*>(a.scratch) + (size_t)a.rows * n) + (size_t)row * n * top;
   const float token_logit = logit_of(a, row);
   RangeStats s = {-__builtin_inff(), 0.0f, 0.0, 0.0};
-  uint64_t mine = 0;
-  if (t < n) {
-    s = stats[t];
-    if (top) mine = keys[(size_t)t * top];
-  }
+  uint64_t mine = 0, key[kLogprobTop];
+  if (t < n) s = stats[t];
+  const int j = n >= top ? 1 : (top + n - 1) / n, q = n >= top ? top : (top + j - 1) / j;
+  if (top && t < n) mine = keys[(size_t)t * top + j - 1];
+#pragma unroll
+  for (int k = 0; k < kLogprobTop; ++k)  // the lists' keys, 256 at a time
+    if (256 * k < n * top) key[k] = 256 * k + t < n * top ? keys[256 * k + t] : 0;
   float m = s.m;
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) m = maximum(m, __shfl_xor(m, k));
   if (lane == 0) sh.wave_m[wave] = m;
   heads[t] = mine;
   if (t == 0) sh.count[0] = 0;
+  if (t == 0) least = 0;
   if (t < kLogprobTop) sh.keys[t] = 0;
   __syncthreads();
   const float* const w = sh.wave_m;
@@ -462,27 +474,15 @@ __global__ __launch_bounds__(256) void k_logprob_join(LogprobArgs a) {
     sh.sum[1][wave] = d;
   }
   if (top) {
-    // a list's place among the first keys; only one range can be empty, so that no two are equal
-    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
-    int place = 0;
-#pragma unroll 2
-    for (int i = 0; i < n; i += 8) {
-      const u64x2* const at = reinterpret_cast<const u64x2*>(&heads[i]);
-      const u64x2 k0 = at[0], k1 = at[1], k2 = at[2], k3 = at[3];
-      place += (k0[0] > mine) + (k0[1] > mine) + (k1[0] > mine) + (k1[1] > mine);
-      place += (k2[0] > mine) + (k2[1] > mine) + (k3[0] > mine) + (k3[1] > mine);
-    }
-    if (t < n && place < top) lists[place] = t;
+    // of lists shorter than that the j-th key is 0, and then all keys may be wanted
+    if (mine && larger<4>(heads, n, mine) == q - 1) least = mine;
     __syncthreads();
-    const int many = min(n, top);
-    const uint64_t last = n >= top ? heads[lists[top - 1]] : 0;
-    for (int i = t; i < many * top; i += 256) {
-      const int list = i / top;
-      const uint64_t key = keys[(size_t)lists[list] * top + (i - list * top)];
-      if (key && key >= last) sh.keys[kLogprobTop + atomicAdd(&sh.count[0], 1)] = key;
-    }
+    const uint64_t reach = least;
+#pragma unroll
+    for (int k = 0; k < kLogprobTop; ++k)
+      if (256 * k < n * top && key[k] && key[k] >= reach) sh.keys[kLogprobTop + atomicAdd(&sh.count[0], 1)] = key[k];
     __syncthreads();
-    rank_all(sh, 0, sh.count[0], top);
+    rank_all<4>(sh, 0, sh.count[0], top);
   } else {
     __syncthreads();
   }
