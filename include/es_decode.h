@@ -428,9 +428,9 @@ size_t es_attn_tree_scratch_bytes(int q_heads, int kv_heads, int rows);
  * path (keys k_tree, values v_proj); gated [rows, q_heads, 256] = bf16(o *
  * sigmoid(gate)), o = softmax(q.K^T / 16) V. q_proj [rows, q_heads, 512]
  * (query|gate), k_proj, v_proj [rows, kv_heads, 256], inv_freq 32 device floats;
- * query head h reads KV head h / (q_heads / kv_heads). Norms and angles in 64 bits
- * up to 32, softmax in 32, the probabilities rounded to bf16 for the products, eps
- * 1e-6. rows 1 .. ES_TREE_MAX, kv_heads 1 .. 256, q_heads a multiple of it up to
+ * query head h reads KV head h / (q_heads / kv_heads). Angles in 64 bits, norms
+ * (also of heads whose squares pass fp32's range) and softmax in 32, the probabilities
+ * rounded to bf16 for their sum and the products, eps 1e-6. rows 1 .. ES_TREE_MAX, kv_heads 1 .. 256, q_heads a multiple of it up to
  * 1024, capacity 1 .. 2^22, position 0 .. capacity. Pointers 16-byte aligned,
  * outputs apart from the inputs. Scratch must not be used by two calls at once. */
 int es_attn_tree(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t* v_proj, const uint16_t* q_gain,
@@ -452,8 +452,9 @@ int es_kv_tree_keep(const uint16_t* k_tree, const uint16_t* v_proj, const uint64
  * log g = -exp(A_log) softplus(a + dt_bias), beta = sigmoid(b), and with S the state
  * behind the node's parent u = beta (v - g S k), S' = g S + u k^T, y [rows, 2048] =
  * bf16(S' q). keys and updates [rows, 16, 128] fp32 take k and u, log_decay [rows, 16]
- * fp32 log g, as es_gdn_tree_keep wants them. In fp32 (squares of the norms and sums
- * of log g in 64 bits), without the reference's roundings to bf16 on the way.
+ * fp32 log g, as es_gdn_tree_keep wants them. In fp32 (sums of log g in 64 bits, in which
+ * one below -300 counts as -300: such a gate is 0), without the reference's roundings to
+ * bf16 on the way.
  * position >= 0, rows 1 .. ES_TREE_MAX; pointers 16-byte aligned, outputs apart
  * from each other and the inputs. */
 int es_gdn_tree(const uint16_t* raw, const uint16_t* ring, const uint16_t* conv_w, const uint16_t* a_proj,
