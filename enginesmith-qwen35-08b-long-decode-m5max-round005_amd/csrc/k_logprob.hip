@@ -130,7 +130,7 @@ __device__ __forceinline__ float logit_of(const LogprobArgs& a, int row) {
 __device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, float x, float m, double r, double d,
                                            const uint64_t* list) {
   const bool finite = fabsf(m) < __builtin_inff();
-  const double log_sum = finite ? (double)log1pf((float)r) : (double)__builtin_nanf("");
+  const double log_sum = finite ? log1p(r) : (double)__builtin_nanf("");
   if (threadIdx.x == 0) {
     if (a.logprob) a.logprob[row] = (float)(((double)x - (double)m) - log_sum);
     if (a.entropy) a.entropy[row] = (float)(log_sum - d * 0.69314718055994530942 / (1.0 + r));
