@@ -543,6 +543,24 @@ int es_attn_kv8(const uint16_t* query, int q_heads, const es_kv8* cache, int pos
 }
 
 // ---- trees of drafted tokens ----
+struct Span {
+  const void* at;
+  size_t bytes;
+};
+bool meet(const Span& a, const Span& b) {
+  const uintptr_t x = (uintptr_t)a.at, y = (uintptr_t)b.at;
+  return x && y && x < y + b.bytes && y < x + a.bytes;
+}
+// Whether an output shares memory with another or with an input.
+bool any_meet(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+  for (const Span& a : outputs) {
+    for (const Span& b : outputs)
+      if (&a != &b && meet(a, b)) return true;
+    for (const Span& b : inputs)
+      if (meet(a, b)) return true;
+  }
+  return false;
+}
 static_assert(ES_TREE_MAX == es::kTree, "the header's limit is the kernels'");
 
 int es_tree_paths(const int32_t* parents, int rows, uint64_t* paths) {
@@ -576,11 +594,14 @@ int es_attn_tree(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t*
     return fail(ES_ERR_INVALID, "es_attn_tree: q_heads a multiple of kv_heads and at most 1024 required");
   if (!aligned16({q_proj, k_proj, v_proj, q_gain, k_gain, inv_freq, kcache, vcache, scratch, k_tree, gated}))
     return fail(ES_ERR_INVALID, "es_attn_tree: pointers must be 16-byte aligned");
-  if (gated == q_proj || gated == k_proj || gated == v_proj || gated == k_tree || k_tree == q_proj || k_tree == k_proj ||
-      k_tree == v_proj)
-    return fail(ES_ERR_INVALID, "es_attn_tree: k_tree and gated must not alias the projections or each other");
-  if (!scratch || scratch_bytes < es::tree_attn_scratch_bytes(q_heads, kv_heads, rows))
+  const size_t need = es::tree_attn_scratch_bytes(q_heads, kv_heads, rows);
+  if (!scratch || scratch_bytes < need)
     return fail(ES_ERR_INVALID, "es_attn_tree: scratch smaller than es_attn_tree_scratch_bytes(q_heads, kv_heads, rows)");
+  const size_t row = es::kHeadDim * 2, cache = (size_t)kv_heads * capacity * row;
+  if (any_meet({{scratch, need}, {k_tree, rows * kv_heads * row}, {gated, rows * q_heads * row}},
+               {{q_proj, 2 * rows * q_heads * row}, {k_proj, rows * kv_heads * row}, {v_proj, rows * kv_heads * row}, {q_gain, row},
+                {k_gain, row}, {inv_freq, 128}, {paths, 8 * (size_t)rows}, {kcache, cache}, {vcache, cache}}))
+    return fail(ES_ERR_INVALID, "es_attn_tree: k_tree, gated and scratch must not alias the inputs or each other");
   es::TreeAttn a{};
   a.q_proj = q_proj;
   a.k_proj = k_proj;
@@ -612,6 +633,9 @@ int es_kv_tree_keep(const uint16_t* k_tree, const uint16_t* v_proj, const uint64
     return fail(ES_ERR_INVALID, "es_kv_tree_keep: node 0 .. rows-1 and a position below the capacity required");
   if (!aligned16({k_tree, v_proj, kcache, vcache}))
     return fail(ES_ERR_INVALID, "es_kv_tree_keep: pointers must be 16-byte aligned");
+  const size_t all = (size_t)rows * kv_heads * es::kHeadDim * 2, cache = (size_t)kv_heads * capacity * es::kHeadDim * 2;
+  if (any_meet({{kcache, cache}, {vcache, cache}}, {{k_tree, all}, {v_proj, all}, {paths, 8 * (size_t)rows}}))
+    return fail(ES_ERR_INVALID, "es_kv_tree_keep: the caches must not alias the draft's tensors or each other");
   const es::TreeKeepKv a{k_tree, v_proj, paths, node, kv_heads, kcache, vcache, capacity, position};
   return hip_status(es::launch_tree_keep_kv(a, S(stream)), "es_kv_tree_keep");
 }
@@ -627,7 +651,10 @@ int es_gdn_tree(const uint16_t* raw, const uint16_t* ring, const uint16_t* conv_
   if (position < 0) return fail(ES_ERR_INVALID, "es_gdn_tree: position >= 0 required");
   if (!aligned16({raw, ring, conv_w, a_proj, b_proj, a_log, dt_bias, state, y, keys, updates, log_decay}))
     return fail(ES_ERR_INVALID, "es_gdn_tree: pointers must be 16-byte aligned");
-  if (keys == updates || keys == state || updates == state || y == raw)
+  const size_t n = (size_t)rows;
+  if (any_meet({{y, n * 4096}, {keys, n * 8192}, {updates, n * 8192}, {log_decay, n * 64}},
+               {{raw, n * es::kConv * 2}, {ring, 8 * es::kConv}, {conv_w, 8 * es::kConv}, {a_proj, n * 32}, {b_proj, n * 32},
+                {a_log, 64}, {dt_bias, 32}, {paths, 8 * n}, {state, 1 << 20}}))
     return fail(ES_ERR_INVALID, "es_gdn_tree: outputs must not alias the inputs or each other");
   const es::TreeGdn a{raw, ring, conv_w, a_proj, b_proj, a_log, dt_bias, paths, position, rows, state, y, keys, updates, log_decay};
   return hip_status(es::launch_tree_gdn(a, S(stream)), "es_gdn_tree");
@@ -644,8 +671,12 @@ int es_gdn_tree_keep(const uint16_t* raw, const float* keys, const float* update
     return fail(ES_ERR_INVALID, "es_gdn_tree_keep: node 0 .. rows-1 and position >= 0 required");
   if (!aligned16({raw, keys, updates, log_decay, ring, state, state_out}))
     return fail(ES_ERR_INVALID, "es_gdn_tree_keep: pointers must be 16-byte aligned");
-  if (state_out == keys || state_out == updates || raw == ring)
-    return fail(ES_ERR_INVALID, "es_gdn_tree_keep: outputs must not alias the draft's tensors");
+  const size_t n = (size_t)rows;
+  const Span from{state, 1 << 20}, to{state_out, 1 << 20};
+  if (any_meet({to, {ring, 8 * es::kConv}}, {{raw, n * es::kConv * 2}, {keys, n * 8192}, {updates, n * 8192}, {log_decay, n * 64},
+                                             {paths, 8 * n}}) ||
+      meet(from, {ring, 8 * es::kConv}) || (state != state_out && meet(from, to)))
+    return fail(ES_ERR_INVALID, "es_gdn_tree_keep: outputs must not alias the draft's tensors or each other; state_out may be state");
   const es::TreeKeepGdn a{raw, keys, updates, log_decay, paths, node, position, ring, state, state_out};
   return hip_status(es::launch_tree_keep_gdn(a, S(stream)), "es_gdn_tree_keep");
 }
@@ -670,6 +701,10 @@ int es_logprob_rows(const uint16_t* logits, int64_t row_stride, int rows, int vo
   const size_t need = es::logprob_scratch_bytes(rows, vocab, top);
   if (!aligned16({scratch}) || (need && (!scratch || scratch_bytes < need)))
     return fail(ES_ERR_INVALID, "es_logprob_rows: scratch smaller than es_logprob_scratch_bytes(rows, vocab, top) or not 16-byte aligned");
+  const size_t n = (size_t)rows;
+  if (any_meet({{logprob, 4 * n}, {entropy, 4 * n}, {lse, 4 * n}, {top_ids, 4 * n * top}, {top_logprobs, 4 * n * top}, {scratch, need}},
+               {{logits, 2 * ((n - 1) * (size_t)row_stride + vocab)}, {tokens, 4 * n}}))
+    return fail(ES_ERR_INVALID, "es_logprob_rows: outputs and scratch must not alias logits, tokens or each other");
   es::LogprobArgs a{};
   a.logits = logits;
   a.stride = row_stride;

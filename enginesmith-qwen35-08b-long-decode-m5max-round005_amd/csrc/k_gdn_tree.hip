@@ -117,7 +117,7 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
     for (int back = 0; back < 4; ++back) {
       const int j = up ? 63 - __clzll(up) : 0;
       if (back == 1 && up) parent = j;
-      taps |= (uint32_t)(back <= depth ? 4 + j : (a.position + depth - back) & 3) << (24 - 8 * back);
+      taps |= (uint32_t)(back <= depth ? 4 + j : ((uint32_t)a.position + depth - back) & 3) << (24 - 8 * back);
       up &= ~(1ull << j);
     }
     tap[lane] = taps;
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(256) void k_gdn_tree_keep(TreeKeepGdn a) {
     for (int place = __popcll(p) - 1, k = 0; k < 4 && p; ++k, --place) {
       const int j = 63 - __clzll(p);
       p &= ~(1ull << j);
-      *reinterpret_cast<u32x4*>(a.ring + ((a.position + place) & 3) * kConv + c) =
+      *reinterpret_cast<u32x4*>(a.ring + (((uint32_t)a.position + place) & 3) * kConv + c) =
           *reinterpret_cast<const u32x4*>(a.raw + (size_t)j * kConv + c);
     }
     return;

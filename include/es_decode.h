@@ -403,7 +403,8 @@ int es_attn_kv8(const uint16_t* query, int q_heads, const es_kv8* cache, int pos
  * from parents). A node's position is `position` + the number of its ancestors.
  * Bits above i count for nothing, and a word without bit i leaves the node out: its
  * outputs are zeros, whatever its inputs hold, and no other node may have it on
- * its path. Infinities and NaN of a node reach only the nodes whose path holds it.
+ * its path. Infinities and NaN of a node reach only the nodes whose path holds it;
+ * those of the context, cache or state reach every node.
  *
  * A draft's pass: for each layer es_attn_tree or es_gdn_tree, which change neither
  * cache nor state; for the accepted node's path es_kv_tree_keep or
@@ -430,9 +431,10 @@ size_t es_attn_tree_scratch_bytes(int q_heads, int kv_heads, int rows);
  * (query|gate), k_proj, v_proj [rows, kv_heads, 256], inv_freq 32 device floats;
  * query head h reads KV head h / (q_heads / kv_heads). Angles in 64 bits, norms
  * (also of heads whose squares pass fp32's range) and softmax in 32, the probabilities
- * rounded to bf16 for their sum and the products, eps 1e-6. rows 1 .. ES_TREE_MAX, kv_heads 1 .. 256, q_heads a multiple of it up to
- * 1024, capacity 1 .. 2^22, position 0 .. capacity. Pointers 16-byte aligned,
- * outputs apart from the inputs. Scratch must not be used by two calls at once. */
+ * rounded to bf16 for their sum and the products, eps 1e-6. rows 1 .. ES_TREE_MAX,
+ * kv_heads 1 .. 256, q_heads a multiple of it up to 1024, capacity 1 .. 2^22,
+ * position 0 .. capacity. Pointers 16-byte aligned, outputs and scratch apart from the
+ * inputs (whole caches) and each other. Scratch must not be used by two calls at once. */
 int es_attn_tree(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t* v_proj, const uint16_t* q_gain,
                  const uint16_t* k_gain, const float* inv_freq, const uint64_t* paths, int rows, int q_heads,
                  int kv_heads, const uint16_t* kcache, const uint16_t* vcache, int capacity, int position,
@@ -440,8 +442,9 @@ int es_attn_tree(const uint16_t* q_proj, const uint16_t* k_proj, const uint16_t*
 
 /* K and V rows of an accepted path into the cache: rows position, position + 1, ...
  * take the rows of `node`'s path in k_tree and v_proj [rows, kv_heads, 256], in order.
- * Rows from the capacity on are dropped; nothing else changes. node 0 .. rows-1, as
- * for es_attn_tree otherwise (position below the capacity). */
+ * Rows from the capacity on are dropped; nothing else changes. The caches lie apart from
+ * each other and the rest. node 0 .. rows-1, as for es_attn_tree otherwise (position
+ * below the capacity). */
 int es_kv_tree_keep(const uint16_t* k_tree, const uint16_t* v_proj, const uint64_t* paths, int node, int rows,
                     int kv_heads, uint16_t* kcache, uint16_t* vcache, int capacity, int position, void* stream);
 
@@ -464,8 +467,9 @@ int es_gdn_tree(const uint16_t* raw, const uint16_t* ring, const uint16_t* conv_
 
 /* State and ring behind an accepted path: state_out (may be state) = S' of `node`
  * above, from what es_gdn_tree left, and the ring's slots of the path's last four
- * positions take their raw rows. A node left out changes nothing. node 0 ..
- * rows-1; position and rows as for es_gdn_tree. */
+ * positions take their raw rows. A node left out leaves the ring and the state's values
+ * as they are. node 0 .. rows-1; position and rows as for es_gdn_tree; outputs apart
+ * from each other and the rest. */
 int es_gdn_tree_keep(const uint16_t* raw, const float* keys, const float* updates, const float* log_decay,
                      const uint64_t* paths, int node, int rows, int position, uint16_t* ring, const float* state,
                      float* state_out, void* stream);
@@ -510,8 +514,8 @@ size_t es_logprob_scratch_bytes(int rows, int vocab, int top);
  * and, without a NaN, its lse of +-infinity; so does the log probability of a token
  * that is not below vocab. logprob (with tokens), entropy and lse are optional;
  * top 0 .. 32 and at most vocab, 0 without top_ids and top_logprobs. rows 1 .. 2^20,
- * vocab 1 .. 2^22. scratch 16-byte aligned, not used by two calls at once. No
- * reference counterpart. */
+ * vocab 1 .. 2^22. Outputs and scratch (16-byte aligned, not used by two calls
+ * at once) apart from the inputs and each other. No reference counterpart. */
 int es_logprob_rows(const uint16_t* logits, int64_t row_stride, int rows, int vocab, const uint32_t* tokens, int top,
                     void* scratch, size_t scratch_bytes, float* logprob, float* entropy, float* lse,
                     uint32_t* top_ids, float* top_logprobs, void* stream);

@@ -6,7 +6,7 @@ import pytest
 
 import esdecode as E
 
-P = 4096  # any 16-byte aligned address
+P = 1 << 33  # any 16-byte aligned address; its multiples lie apart whatever the sizes
 
 
 def refused(rc, text):
@@ -37,14 +37,14 @@ def test_paths_arguments():
 
 
 ATTN = dict(q_proj=P, k_proj=2 * P, v_proj=3 * P, q_gain=P, k_gain=P, inv_freq=P, paths=P, rows=4, q_heads=8, kv_heads=2,
-            kcache=P, vcache=P, capacity=100, position=50, scratch=P, size=1 << 40, k_tree=4 * P, gated=5 * P)
+            kcache=P, vcache=P, capacity=100, position=50, scratch=6 * P, size=1 << 40, k_tree=4 * P, gated=5 * P)
 KEEP_KV = dict(k_tree=P, v_proj=P, paths=P, node=3, rows=4, kv_heads=2, kcache=2 * P, vcache=3 * P, capacity=100, position=50)
 GDN = dict(raw=P, ring=P, conv_w=P, a_proj=P, b_proj=P, a_log=P, dt_bias=P, paths=P, position=50, rows=4, state=P, y=2 * P,
            keys=3 * P, updates=4 * P, log_decay=5 * P)
 KEEP_GDN = dict(raw=P, keys=P, updates=P, log_decay=P, paths=P, node=3, rows=4, position=50, ring=2 * P, state=3 * P,
                 state_out=3 * P)
-LOGPROB = dict(logits=P, stride=100, rows=3, vocab=100, tokens=P, top=5, scratch=P, size=1 << 40, logprob=P, entropy=P, lse=P,
-               top_ids=P, top_logprobs=P)
+LOGPROB = dict(logits=P, stride=100, rows=3, vocab=100, tokens=2 * P, top=5, scratch=3 * P, size=1 << 40, logprob=4 * P,
+               entropy=5 * P, lse=6 * P, top_ids=7 * P, top_logprobs=8 * P)
 CALLS = {"es_attn_tree": ATTN, "es_kv_tree_keep": KEEP_KV, "es_gdn_tree": GDN, "es_gdn_tree_keep": KEEP_GDN,
          "es_logprob_rows": LOGPROB}
 
@@ -94,17 +94,29 @@ def test_caches_and_heads():
         refused(call("es_attn_tree", q_heads=heads), "q_heads")
 
 
-def test_aliasing():
-    for k_tree in (P, 2 * P, 3 * P):
-        refused(call("es_attn_tree", k_tree=k_tree), "alias")
-    for gated in (P, 2 * P, 3 * P, 4 * P):
-        refused(call("es_attn_tree", gated=gated), "alias")
-    refused(call("es_gdn_tree", updates=3 * P), "alias")
-    refused(call("es_gdn_tree", keys=P), "alias")
-    refused(call("es_gdn_tree", updates=P), "alias")
-    refused(call("es_gdn_tree", y=P), "alias")
-    refused(call("es_gdn_tree_keep", state_out=P), "alias")
-    refused(call("es_gdn_tree_keep", ring=P), "alias")
+OUTPUTS = {  # with their bytes
+    "es_attn_tree": dict(k_tree=4 * 2 * 512, gated=4 * 8 * 512, scratch=None),
+    "es_kv_tree_keep": dict(kcache=2 * 100 * 512, vcache=2 * 100 * 512),
+    "es_gdn_tree": dict(y=4 * 4096, keys=4 * 8192, updates=4 * 8192, log_decay=4 * 64),
+    "es_gdn_tree_keep": dict(ring=4 * 12288, state_out=1 << 20),
+    "es_logprob_rows": dict(logprob=12, entropy=12, lse=12, top_ids=60, top_logprobs=60, scratch=None)}
+
+
+@pytest.mark.parametrize("name", OUTPUTS)
+def test_aliasing(name):
+    """Every output over every other tensor: at its start, and its last 16 bytes over the other's first."""
+    wide = {"vocab": 248320, "stride": 248320} if name == "es_logprob_rows" else {}
+    for out, size in OUTPUTS[name].items():
+        if size is None:
+            size = int(E.lib().es_attn_tree_scratch_bytes(8, 2, 4) if name == "es_attn_tree" else
+                       E.lib().es_logprob_scratch_bytes(3, 248320, 5))
+            assert size > 0
+        for other, at in CALLS[name].items():
+            if other in NOT_POINTERS or other == out:
+                continue
+            if not (out == "state_out" and other == "state"):
+                refused(call(name, **{out: at}, **wide), "alias")
+            refused(call(name, **{out: at - (size - 1) // 16 * 16}, **wide), "alias")
 
 
 def test_scratch_sizes():
