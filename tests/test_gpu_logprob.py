@@ -260,3 +260,22 @@ def test_a_row_alone_and_among_others_in_graphs_and_on_a_stream():
             torch.cuda.synchronize()
             for a, b in zip(out + [ids, alt], want):
                 assert torch.equal(a, b)
+
+
+def test_beside_the_greedy_token_of_each_row():
+    """es_greedy_bf16 rounds its log sum, and logit less log sum, to bf16: half a step of each."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    x = T.bf(torch.empty(9, 5003, device="cuda").normal_(0, 3, generator=g))
+    tokens = torch.zeros(9, dtype=torch.int32, device="cuda")
+    need = int(E.lib().es_head_scratch_bytes(5003))
+    scratch, token, lse = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.empty(9, dtype=torch.int32, device="cuda"), \
+        torch.empty(9, device="cuda")
+    for r in range(9):
+        T.call("es_greedy_bf16", x[r].contiguous(), 5003, scratch, need, token[r:], lse[r:])
+    torch.cuda.synchronize()
+    got = run(x, 5003, token, 1)
+    assert torch.allclose(got[2], lse, rtol=T.BF, atol=0)
+    assert torch.allclose(got[0], got[4][:, 0], rtol=2 * T.BF, atol=T.BF * float(lse.max()))
+    exact = x.double().log_softmax(1)
+    assert torch.allclose(got[0].double(), exact[torch.arange(9), token.long()], rtol=8 * T.EPS, atol=0)

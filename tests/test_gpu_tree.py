@@ -435,3 +435,29 @@ def test_graphs_and_other_streams():
         for run in (graph.replay, on_side, graph.replay):
             for g, w in zip(answer(run), want):
                 assert torch.equal(g, w)
+
+
+def test_two_drafts_at_once():
+    """Two streams, each with scratch and outputs of its own, over the same cache and state."""
+    rows = [(64, "random"), (9, "wide")]
+    gdn = [T.gdn_case(m, 12, T.parents_of(kind, m, 1), seed=5) for m, kind in rows]
+    attn = [T.attn_case(m, 8, 2, 9000, T.parents_of(kind, m, 1), seed=6) for m, kind in rows]
+    attn[1].update(k_cache=attn[0]["k_cache"], v_cache=attn[0]["v_cache"], capacity=attn[0]["capacity"])
+    gdn[1].update(ring=gdn[0]["ring"], state=gdn[0]["state"])
+    want = [(T.run_gdn(s), T.run_attn(a)) for s, a in zip(gdn, attn)]
+    streams = [torch.cuda.Stream() for _ in rows]
+    sizes = [int(E.lib().es_attn_tree_scratch_bytes(8, 2, m)) for m, _ in rows]
+    got = [([torch.empty_like(t) for t in w[0]], [torch.empty_like(t) for t in w[1]],
+            torch.empty(size, dtype=torch.uint8, device="cuda")) for w, size in zip(want, sizes)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, a, stream, (m, _), (y, o, scratch), size in zip(gdn, attn, streams, rows, got, sizes):
+            with torch.cuda.stream(stream):
+                T.call("es_gdn_tree", s["raw"], s["ring"], s["conv_w"], s["a_proj"], s["b_proj"], s["a_log"], s["dt_bias"],
+                       s["paths"], 12, m, s["state"], *y)
+                T.call("es_attn_tree", a["q_proj"], a["k_proj"], a["v_proj"], a["q_gain"], a["k_gain"], a["inv_freq"],
+                       a["paths"], m, 8, 2, a["k_cache"], a["v_cache"], a["capacity"], 9000, scratch, size, o[1], o[0])
+    torch.cuda.synchronize()
+    for (y, o, _), w in zip(got, want):
+        for t, u in zip(y + o, list(w[0]) + list(w[1])):
+            assert torch.equal(t, u)
