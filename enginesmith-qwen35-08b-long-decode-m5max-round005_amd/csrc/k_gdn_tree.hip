@@ -42,6 +42,14 @@ __device__ __forceinline__ void substitute(const float (&low)[16], float& x) {
     substitute<I + 1>(low, x);
   }
 }
+// The double of the lane that a DPP control within 16 lanes names.
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
 // A gate's log as it enters the sums: from -300 down it is a gate of 0 (32 bits end
 // at -104), and a bound keeps the differences of sums behind it exact.
 __device__ __forceinline__ double bounded(float log_g) { return log_g < -300.0f ? -300.0 : (double)log_g; }
@@ -68,19 +76,20 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
   __shared__ float y[kTree][kSlice + 1], u[kTree][kSlice + 1];  // u: v, then what is left of it
   __shared__ uint64_t path[kTree];
   __shared__ double total[kTree];
-  __shared__ float beta[kTree];
+  __shared__ float beta[kTree], log_gate[kTree];
   __shared__ uint32_t tap[kTree];
   __shared__ int odd[kTree / 16];  // by block of nodes: whether its u holds an infinity or a NaN
   const int t = threadIdx.x, lane = t & 63, n16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int h = blockIdx.x >> 3, v0 = (blockIdx.x & 7) * kSlice;
+  // a head's blocks on one XCD (a launch's blocks go to the 8 XCDs in turn), which fetches its rows once
+  const int h = (blockIdx.x & 7) | blockIdx.x >> 6 << 3, v0 = (blockIdx.x >> 3 & 7) * kSlice;
   const int own = t >> 4, column = t & 15;  // a thread's node and value column, where it has one
   const int rows = a.rows, tiles = (rows + 15) >> 4;
-  // wave 0: paths and gates, a node a lane; their chain is the longest of this part
+  // wave 0: paths and taps, wave 1: gates, a node a lane
   uint64_t my_word = 0;
   float my_a = 0.0f, my_b = 0.0f, rate = 0.0f;
-  if (wave == 0 && lane < rows) {
-    my_word = a.paths[lane];
+  if (wave < 2 && lane < rows) my_word = a.paths[lane];
+  if (wave == 1 && lane < rows) {
     my_a = bf2f(a.a_proj[lane * 16 + h]) + bf2f(a.dt_bias[h]);
     my_b = bf2f(a.b_proj[lane * 16 + h]);
     rate = a.a_log[h];
@@ -112,32 +121,20 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
     const int depth = __popcll(p) - 1;
     uint64_t up = p;
     uint32_t taps = 0;
-    int parent = -1;
 #pragma unroll
     for (int back = 0; back < 4; ++back) {
       const int j = up ? 63 - __clzll(up) : 0;
-      if (back == 1 && up) parent = j;
       taps |= (uint32_t)(back <= depth ? 4 + j : ((uint32_t)a.position + depth - back) & 3) << (24 - 8 * back);
       up &= ~(1ull << j);
     }
     tap[lane] = taps;
     if (lane < kTree / 16) odd[lane] = 0;
-    float log_g = 0.0f;
-    if (p) log_g = -expf(rate) * (fmaxf(my_a, 0.0f) + log1pf(expf(-fabsf(my_a))));
-    beta[lane] = p ? sigmoid(my_b) : 0.0f;
+  } else if (wave == 1) {
+    const bool used = tree_path(my_word, lane) != 0;
+    const float log_g = used ? -expf(rate) * (fmaxf(my_a, 0.0f) + log1pf(expf(-fabsf(my_a)))) : 0.0f;
+    log_gate[lane] = log_g;
+    beta[lane] = used ? sigmoid(my_b) : 0.0f;
     if (v0 == 0 && lane < rows) a.log_decay[lane * 16 + h] = log_g;
-    // sums along the path: each round adds what twice as many ancestors sum to
-    double sum = p ? bounded(log_g) : 0.0;
-#pragma unroll 1
-    while (__any(parent >= 0)) {
-      const double more = __shfl(sum, parent & 63);
-      const int next = __shfl(parent, parent & 63);
-      if (parent >= 0) {
-        sum += more;
-        parent = next;
-      }
-    }
-    total[lane] = sum;
   }
 #pragma unroll
   for (int k = 0; k < kLoads; ++k) {
@@ -201,7 +198,17 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
       x = fmaf(bf2f(un.staged[taps >> 8 & 255][c]), bf_hi(wv.x), x);
       x = fmaf(bf2f(un.staged[taps >> 16 & 255][c]), bf_lo(wv.y), x);
       x = fmaf(bf2f(un.staged[taps >> 24][c]), bf_hi(wv.y), x);
-      u[r][column] = path[r] ? silu(x) : 0.0f;
+      const uint64_t on = path[r];
+      u[r][column] = on ? silu(x) : 0.0f;
+      // the sum of log gates along the node's path, four nodes of it a lane
+      double sum = 0.0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += on >> (4 * column + e) & 1 ? bounded(log_gate[4 * column + e]) : 0.0;
+      sum += dpp<0xb1>(sum);   // lane ^ 1
+      sum += dpp<0x4e>(sum);   // lane ^ 2
+      sum += dpp<0x141>(sum);  // the other four of eight
+      sum += dpp<0x140>(sum);  // the other eight
+      if (column == 0) total[r] = sum;
     }
   }
   __syncthreads();
@@ -342,7 +349,8 @@ __global__ __launch_bounds__(256) void k_gdn_tree_keep(TreeKeepGdn a) {
   }
   __shared__ float weight[kTree], decay;
   __shared__ int node[kTree];
-  const int h = blockIdx.x >> 4, v = (blockIdx.x & 15) * 8 + (t >> 5), k = 4 * (t & 31);
+  // a head's blocks on one XCD
+  const int h = (blockIdx.x & 7) | blockIdx.x >> 7 << 3, v = (blockIdx.x >> 3 & 15) * 8 + (t >> 5), k = 4 * (t & 31);
   const size_t at = ((size_t)h * 128 + v) * 128 + k;
   f32x4 s = *reinterpret_cast<const f32x4*>(a.state + at);
   const int many = __popcll(path);
