@@ -24,31 +24,33 @@ constexpr int kSlice = 16;               // value rows of a block
 constexpr int kStaged = 256 + kSlice;    // channels of a head that a block takes: q, k, its part of v
 constexpr int kStagedRow = kStaged + 8;  // bf16 elements between staged rows
 constexpr int kQk = 132;                 // floats between rows of q and of k
-constexpr int kPair = 65;                // floats between rows of the pair matrices
+constexpr int kPair = 68;                // floats between rows of the pair matrices
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(-x * kLog2e)); }
 __device__ __forceinline__ float finite_or_0(float x) { return fabsf(x) < INFINITY ? x : 0.0f; }
 __device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e)); }
-// x of the lane's node less low[i] times that of each node i before it, in order; the
-// 16 nodes lie in the 16 lanes of a row, from which DPP hands out one. 0 times
-// anything is 0 here.
+// x of the lane's node less low[i] times that of each of 16 nodes, in order; those lie in
+// the 16 lanes of a row, from which DPP hands out one. 0 times anything is 0 here.
 template <int I>
-__device__ __forceinline__ void substitute(const float (&low)[16], float& x) {
+__device__ __forceinline__ void less(const f32x4 (&low)[4], float others, float& x) {
   if constexpr (I < 16) {
-    const float xi = __builtin_amdgcn_update_dpp(0.0f, x, 0x150 + I, 0xf, 0xf, false);
+    const float xi = __builtin_amdgcn_update_dpp(0.0f, others, 0x150 + I, 0xf, 0xf, false), by = low[I >> 2][I & 3];
     float part;
-    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(part) : "v"(low[I]), "v"(xi));
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(part) : "v"(by), "v"(xi));
+    x = x - part;
+    less<I + 1>(low, others, x);
+  }
+}
+// The same where the lane's node is one of them and those before it change likewise.
+template <int I>
+__device__ __forceinline__ void substitute(const f32x4 (&low)[4], float& x) {
+  if constexpr (I < 16) {
+    const float xi = __builtin_amdgcn_update_dpp(0.0f, x, 0x150 + I, 0xf, 0xf, false), by = low[I >> 2][I & 3];
+    float part;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(part) : "v"(by), "v"(xi));
     x = x - part;
     substitute<I + 1>(low, x);
   }
-}
-// The double of the lane that a DPP control within 16 lanes names.
-template <int CTRL>
-__device__ __forceinline__ double dpp(double x) {
-  const uint64_t b = (uint64_t)__double_as_longlong(x);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
-  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 // A gate's log as it enters the sums: from -300 down it is a gate of 0 (32 bits end
 // at -104), and a bound keeps the differences of sums behind it exact.
@@ -59,11 +61,12 @@ __device__ __forceinline__ double bounded(float log_g) { return log_g < -300.0f 
 //   - the raw rows to LDS, all loads at once; paths and gates
 //   - convolution, SiLU and norms, a row a wave, four channels of q or k a lane
 //   - k S0^T, q S0^T, k k^T and q k^T in 16 x 16 tiles on 32-bit products
-//   - u by substitution: a 16-node block of the triangle in registers, four value
-//     columns a wave, what it gives to later blocks by products again
+//   - u by substitution: four value columns a wave, each with all nodes in the
+//     registers of 16 lanes, no barrier (in turns of 16 nodes with products between them
+//     64 nodes took 5800 cycles of 34000, so XXXX)
 //   - y = q S0^T + (pairs) u by products
 // A 0 for what is not on a node's path would carry a NaN or an infinity of u to it:
-// the substitution multiplies by the rule that 0 times anything is 0, the products
+// the substitution multiplies by the rule that 0 times anything is 0, the last products
 // take 0 for such a u, and where there is one it is added to those behind it alone.
 __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
   __shared__ __attribute__((aligned(16))) float qs[kTree][kQk], ks[kTree][kQk];
@@ -76,9 +79,9 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
   __shared__ float y[kTree][kSlice + 1], u[kTree][kSlice + 1];  // u: v, then what is left of it
   __shared__ uint64_t path[kTree];
   __shared__ double total[kTree];
-  __shared__ float beta[kTree], log_gate[kTree];
+  __shared__ float beta[kTree];
   __shared__ uint32_t tap[kTree];
-  __shared__ int odd[kTree / 16];  // by block of nodes: whether its u holds an infinity or a NaN
+  __shared__ int odd;  // whether u holds an infinity or a NaN
   const int t = threadIdx.x, lane = t & 63, n16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   // a head's blocks on one XCD (a launch's blocks go to the 8 XCDs in turn), which fetches its rows once
@@ -128,13 +131,26 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
       up &= ~(1ull << j);
     }
     tap[lane] = taps;
-    if (lane < kTree / 16) odd[lane] = 0;
+    if (lane == 0) odd = 0;
   } else if (wave == 1) {
-    const bool used = tree_path(my_word, lane) != 0;
-    const float log_g = used ? -expf(rate) * (fmaxf(my_a, 0.0f) + log1pf(expf(-fabsf(my_a)))) : 0.0f;
-    log_gate[lane] = log_g;
-    beta[lane] = used ? sigmoid(my_b) : 0.0f;
+    const uint64_t p = tree_path(my_word, lane);
+    const float log_g = p ? -expf(rate) * (fmaxf(my_a, 0.0f) + log1pf(expf(-fabsf(my_a)))) : 0.0f;
+    beta[lane] = p ? sigmoid(my_b) : 0.0f;
     if (v0 == 0 && lane < rows) a.log_decay[lane * 16 + h] = log_g;
+    // sums along the path: each round adds what twice as many ancestors sum to
+    double sum = p ? bounded(log_g) : 0.0;
+    const uint64_t ancestors = p & ~(1ull << lane);
+    int parent = ancestors ? 63 - __clzll(ancestors) : -1;
+#pragma unroll 1
+    while (__any(parent >= 0)) {
+      const double more = __shfl(sum, parent & 63);
+      const int next = __shfl(parent, parent & 63);
+      if (parent >= 0) {
+        sum += more;
+        parent = next;
+      }
+    }
+    total[lane] = sum;
   }
 #pragma unroll
   for (int k = 0; k < kLoads; ++k) {
@@ -198,17 +214,7 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
       x = fmaf(bf2f(un.staged[taps >> 8 & 255][c]), bf_hi(wv.x), x);
       x = fmaf(bf2f(un.staged[taps >> 16 & 255][c]), bf_lo(wv.y), x);
       x = fmaf(bf2f(un.staged[taps >> 24][c]), bf_hi(wv.y), x);
-      const uint64_t on = path[r];
-      u[r][column] = on ? silu(x) : 0.0f;
-      // the sum of log gates along the node's path, four nodes of it a lane
-      double sum = 0.0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += on >> (4 * column + e) & 1 ? bounded(log_gate[4 * column + e]) : 0.0;
-      sum += dpp<0xb1>(sum);   // lane ^ 1
-      sum += dpp<0x4e>(sum);   // lane ^ 2
-      sum += dpp<0x141>(sum);  // the other four of eight
-      sum += dpp<0x140>(sum);  // the other eight
-      if (column == 0) total[r] = sum;
+      u[r][column] = path[r] ? silu(x) : 0.0f;
     }
   }
   __syncthreads();
@@ -275,38 +281,33 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
     }
   }
   __syncthreads();
-  for (int c = 0; c < tiles; ++c) {
-    if (wave < 4) {  // lane: node 16 c + n16, value column 4 wave + g
-      float x = u[16 * c + n16][4 * wave + g], low[16];
+  if (wave < 4) {  // lane: node n16 of each 16, value column 4 wave + g
+    float x[4];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) low[i] = un.m.low[16 * c + n16][16 * c + i];
-      substitute<0>(low, x);
-      u[16 * c + n16][4 * wave + g] = x;
-      if (__any(!(fabsf(x) < INFINITY)) && lane == 0) odd[c] = 1;
-    }
-    __syncthreads();
-    if (c + 1 < tiles) {
-      const int ti = c + 1 + wave;
-      if (ti < tiles) {
-        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < 4; ++c) x[c] = c < tiles ? u[16 * c + n16][4 * wave + g] : 0.0f;
+    bool is_odd = false;
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          acc = __builtin_amdgcn_mfma_f32_16x16x4f32(un.m.low[16 * ti + n16][16 * c + 4 * s + g], finite_or_0(u[16 * c + 4 * s + g][n16]), acc, 0, 0, 0);
+    for (int c = 0; c < 4; ++c)
+      if (c < tiles) {
+        f32x4 low[4];
+        auto block = [&](int ti) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u[16 * ti + 4 * g + e][n16] -= acc[e];
+          for (int k = 0; k < 4; ++k) low[k] = *reinterpret_cast<const f32x4*>(&un.m.low[16 * ti + n16][16 * c + 4 * k]);
+        };
+        block(c);
+        substitute<0>(low, x[c]);
+        u[16 * c + n16][4 * wave + g] = x[c];
+        is_odd |= !(fabsf(x[c]) < INFINITY);
+#pragma unroll
+        for (int ti = c + 1; ti < 4; ++ti)
+          if (ti < tiles) {
+            block(ti);
+            less<0>(low, x[c], x[ti]);
+          }
       }
-      __syncthreads();
-      if (odd[c]) {
-        if (own >= 16 * (c + 1) && own < 16 * tiles) {
-          float x = u[own][column];
-          for (int j = 16 * c; j < 16 * (c + 1); ++j)
-            if (path[own] >> j & 1 && !(fabsf(u[j][column]) < INFINITY)) x -= un.m.low[own][j] * u[j][column];
-          u[own][column] = x;
-        }
-        __syncthreads();
-      }
-    }
+    if (__any(is_odd) && lane == 0) odd = 1;
   }
+  __syncthreads();
   if (wave < tiles) {
     f32x4 acc;
 #pragma unroll
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
   if (own < rows) {
     const size_t at = ((size_t)own * 16 + h) * 128 + v0 + column;
     float z = y[own][column];
-    if (odd[0] | odd[1] | odd[2] | odd[3])
+    if (odd)
       for (int j = 0; j <= own; ++j)
         if (path[own] >> j & 1 && !(fabsf(u[j][column]) < INFINITY)) z += un.m.pair[own][j] * u[j][column];
     a.updates[at] = u[own][column];
