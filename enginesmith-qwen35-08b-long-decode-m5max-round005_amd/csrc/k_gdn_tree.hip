@@ -10,10 +10,12 @@
 // writes a state. The products of gates are exponentials of differences of sums of
 // log gates (in 64 bits), which never overflow and need no division.
 //
-// Latency bounds both kernels (2 to 3 MB in all): in a graph 5 nodes take 6.3 us, 16
-// 6.5, 32 9.5 and 64 16.4, a path of 2 into the state 2.8 and of 48 5.5. The draft's are
-// the five parts below, with 64 nodes the 32-bit products of the pairs and the four
-// turns of the substitution most of it.
+// Latency bounds both kernels (2 to 3 MB in all): in a graph 5 nodes take 6.1 us, 16
+// 6.2, 32 9.0 and 64 15.3, a path of 2 into the state 2.8 and of 48 5.5. The draft's are
+// the five parts below: with 64 nodes 7000 cycles, 7200, 11400 (of which 32-bit products
+// 7200), 3900 and 1700.
+#include <type_traits>
+
 #include "es_kernels.hpp"
 
 namespace es {
@@ -62,8 +64,8 @@ __device__ __forceinline__ double bounded(float log_g) { return log_g < -300.0f 
 //   - convolution, SiLU and norms, a row a wave, four channels of q or k a lane
 //   - k S0^T, q S0^T, k k^T and q k^T in 16 x 16 tiles on 32-bit products
 //   - u by substitution: four value columns a wave, each with all nodes in the
-//     registers of 16 lanes, no barrier (in turns of 16 nodes with products between them
-//     64 nodes took 5800 cycles of 34000, so XXXX)
+//     registers of 16 lanes, no barrier: 64 nodes take 3900 cycles, in turns of 16 with
+//     products and barriers between them 5800
 //   - y = q S0^T + (pairs) u by products
 // A 0 for what is not on a node's path would carry a NaN or an infinity of u to it:
 // the substitution multiplies by the rule that 0 times anything is 0, the last products
@@ -282,30 +284,39 @@ __global__ __launch_bounds__(1024) void k_gdn_tree(TreeGdn a) {
   }
   __syncthreads();
   if (wave < 4) {  // lane: node n16 of each 16, value column 4 wave + g
-    float x[4];
+    auto solve = [&](auto blocks) {
+      constexpr int T = decltype(blocks)::value;
+      float x[T];
+      f32x4 low[T][4];
+      auto fetch = [&](int ti, int c, f32x4 (&to)[4]) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) x[c] = c < tiles ? u[16 * c + n16][4 * wave + g] : 0.0f;
-    bool is_odd = false;
+        for (int k = 0; k < 4; ++k) to[k] = *reinterpret_cast<const f32x4*>(&un.m.low[16 * ti + n16][16 * c + 4 * k]);
+      };
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c < tiles) {
-        f32x4 low[4];
-        auto block = [&](int ti) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) low[k] = *reinterpret_cast<const f32x4*>(&un.m.low[16 * ti + n16][16 * c + 4 * k]);
-        };
-        block(c);
-        substitute<0>(low, x[c]);
-        u[16 * c + n16][4 * wave + g] = x[c];
-        is_odd |= !(fabsf(x[c]) < INFINITY);
-#pragma unroll
-        for (int ti = c + 1; ti < 4; ++ti)
-          if (ti < tiles) {
-            block(ti);
-            less<0>(low, x[c], x[ti]);
-          }
+      for (int c = 0; c < T; ++c) {
+        x[c] = u[16 * c + n16][4 * wave + g];
+        fetch(c, 0, low[c]);
       }
-    if (__any(is_odd) && lane == 0) odd = 1;
+      bool is_odd = false;
+#pragma unroll
+      for (int c = 0; c < T; ++c) {
+        substitute<0>(low[c], x[c]);
+        is_odd |= c < tiles && !(fabsf(x[c]) < INFINITY);
+        u[16 * c + n16][4 * wave + g] = x[c];
+#pragma unroll
+        for (int ti = c + 1; ti < T; ++ti) {
+          less<0>(low[ti], x[c], x[ti]);
+          fetch(ti, c + 1, low[ti]);
+        }
+      }
+      if (__any(is_odd) && lane == 0) odd = 1;
+    };
+    if (tiles == 1)
+      solve(std::integral_constant<int, 1>());
+    else if (tiles == 2)
+      solve(std::integral_constant<int, 2>());
+    else
+      solve(std::integral_constant<int, 4>());
   }
   __syncthreads();
   if (wave < tiles) {
